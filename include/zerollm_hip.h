@@ -214,6 +214,102 @@ int zl_mat_gemv_noalloc(zl_mat *m, const float *x, int M, float *y, void *stream
 /* quantizeAct of M rows of length K (src/compute/ref-kernels.js:44-62). */
 int zl_quant_act(const float *x, int64_t K, int M, int8_t *q, float *d, int32_t *s);
 
+/* ---------------------------------------------------------------------------------------------- long contexts
+ * Operators on the caller's device memory: a KV cache held in 4 bits with the attention over it, rotary positions scaled
+ * beyond the trained context, and log probabilities of logits rows. None has a counterpart in the reference, whose caches
+ * are f32 or f16 and whose positions are unscaled. Models run the first two in their own passes (zl_model_load_ext).
+ *
+ * Every call checks its arguments, enqueues on `stream` (a hipStream_t; NULL is the device's default stream) and returns;
+ * nothing is allocated and nothing waited for, so calls may be captured into a graph. Value types are ggml ids: 0 F32,
+ * 1 F16, 30 BF16; strides count values, and the values of a head are contiguous. Positions, counts and slots are read on
+ * the device when the work runs, so a captured graph serves any position. Work space is the caller's: calls that may
+ * overlap (other streams, graphs replayed side by side) need work spaces of their own. */
+
+/* Rows of several sequences: the value of (sequence, token, head) starts at p + sequence * seq + token * tok + head * head. */
+typedef struct {
+  void *p;
+  int64_t seq, tok, head;
+} zl_rows;
+
+/* The tokens of a call: n_seq sequences of up to n_tok tokens each. Device arrays of n_seq int32: pos, the position of each
+ * sequence's first token (its others follow); count, how many of its n_tok tokens there are (NULL: all; more than n_tok
+ * counts as n_tok; rows behind a count are not read and outputs there are left as they were); slot, the cache slot of each
+ * sequence (NULL: 0 .. n_seq - 1; not used by zl_rope_apply). */
+typedef struct {
+  int n_seq, n_tok;
+  const int32_t *pos, *count, *slot;
+} zl_batch;
+
+/* ---- KV cache in 4 bits. n_slot sequences of up to `capacity` positions, n_head_kv heads of head_dim (64, 128 or 256)
+ * values. Keys and values are held as this library's Q4_0 blocks of 32 along the head (as zl_synth_tensor_bytes quantises,
+ * src/compute/quant.js:52-74): 1.125 bytes per (position, head, dim), key and value together. A block with a value that is
+ * not finite or above 65504 in magnitude reads as NaN. */
+typedef struct zl_kv4 zl_kv4;
+int zl_kv4_create(int n_slot, int n_head_kv, int head_dim, int64_t capacity, zl_kv4 **out);
+/* Waits for the device, since calls on any stream may still use the cache; safe on NULL. */
+int zl_kv4_free(zl_kv4 *c);
+int zl_kv4_bytes(const zl_kv4 *c, int64_t *bytes);
+/* Puts the batch's keys and values at their positions. Tokens at positions outside 0 .. capacity - 1 or of slots that do
+ * not exist are dropped. A slot that occurs more than once in a batch takes its sequences in order. Appends to one slot
+ * must not overlap each other nor reads of the same 32 positions (multiples of 32 on). */
+int zl_kv4_append(zl_kv4 *c, const zl_batch *b, int type, const zl_rows *k, const zl_rows *v, void *stream);
+/* What the cache holds at the batch's positions, as values of `type`; NaN for positions and slots that do not exist. */
+int zl_kv4_read(const zl_kv4 *c, const zl_batch *b, int type, const zl_rows *k, const zl_rows *v, void *stream);
+/* Causal attention of the batch's queries over the cache: the token at position p sees positions 0 .. p of its slot (their
+ * keys and values appended before, its own among them). n_head is a multiple of the cache's n_head_kv, consecutive query
+ * heads share a KV head; scale 0 means 1/sqrt(head_dim). A token at a negative position sees nothing: zeros. One at a
+ * position past the capacity, or of a slot that does not exist: NaN. A row's bits depend on its query, its position and
+ * the cache alone, not on the batch it comes in. q and out may be the same rows. work: zl_kv4_attention_work bytes of
+ * device memory, contents of no matter before or after. */
+int zl_kv4_attention(const zl_kv4 *c, const zl_batch *b, int type, const zl_rows *q, int n_head, float scale, const zl_rows *out,
+                     void *work, int64_t work_bytes, void *stream);
+int zl_kv4_attention_work(const zl_kv4 *c, int n_seq, int n_tok, int n_head, int64_t *bytes);
+
+/* ---- rotary positions. n_rot values of a head are rotated, the rest pass through. neox: pairs (i, i + n_rot/2), else
+ * (2i, 2i + 1), by pos * base^(-2i/n_rot), divided by freq_factors[i] where set (host array of n_rot/2, copied).
+ * scaling 1 (linear): angles divided by factor. scaling 2 (YaRN): pairs that turn more than beta_fast times (0: 32) within
+ * orig_ctx positions keep their angle, those that turn less than beta_slow times (0: 1) have it divided by factor, with a
+ * linear ramp over the pairs between, and cos and sin are multiplied by attn_factor (0: 0.1 ln(factor) + 1). */
+typedef struct zl_rope zl_rope;
+typedef struct {
+  int n_rot, neox;
+  double base;
+  int scaling, orig_ctx;
+  double factor, beta_fast, beta_slow, attn_factor;
+  const float *freq_factors;
+} zl_rope_opts;
+int zl_rope_create(const zl_rope_opts *o, zl_rope **out);
+/* Waits for the device; safe on NULL. */
+int zl_rope_free(zl_rope *r);
+/* Rotates n_head query heads and n_head_kv key heads (k, k_out NULL: queries alone) of the batch's tokens to their
+ * positions (negative ones turn backwards). An output may be its input; otherwise no output may overlap an input. */
+int zl_rope_apply(const zl_rope *r, const zl_batch *b, int type, int head_dim, const zl_rows *q, const zl_rows *q_out, int n_head,
+                  const zl_rows *k, const zl_rows *k_out, int n_head_kv, void *stream);
+
+/* ---- log probabilities of logits rows (device, row stride ld values): lp[r] of tokens[r] (device; NULL with lp NULL;
+ * NaN for an id outside the vocabulary), the entropy in nats, and the n_top (0 .. 64, at most the vocabulary) largest
+ * logits' ids and log probabilities, largest first, the lowest id first among equals. Any output may be NULL. Logits of
+ * -inf have probability 0. A row that holds NaN or +inf, or nothing above -inf, has NaN for every float output (top_ids:
+ * NaN below all). work: zl_logprobs_work bytes. */
+int zl_logprobs(const void *logits, int type, int64_t ld, int rows, int vocab, const int32_t *tokens, int n_top, float *lp,
+                float *entropy, int32_t *top_ids, float *top_lp, void *work, int64_t work_bytes, void *stream);
+int zl_logprobs_work(int rows, int vocab, int n_top, int64_t *bytes);
+/* The same on rows [row0, row0 + nrows) of the model's last logits, with host arrays (beside zl_sample and
+ * zl_distribution); returns when they are filled. */
+int zl_model_logprobs(zl_model *m, int row0, int nrows, const int32_t *tokens, int n_top, float *lp, float *entropy,
+                      int32_t *top_ids, float *top_lp);
+
+/* ---- models with either. kv_q4: the KV cache is held in 4 bits (kv_f16 is ignored; zl_model_info.kv_f16 reads 2). rope:
+ * scaling, orig_ctx (0: the trained context), factor, beta_fast, beta_slow and attn_factor as above, NULL for none; the
+ * other fields come from the model. A scaled model's ctx is capped at factor times the trained context. */
+typedef struct {
+  int kv_q4;
+  const zl_rope_opts *rope;
+} zl_model_ext;
+int zl_model_load_ext(const char *gguf_path, const zl_model_opts *opts, const zl_model_ext *ext, zl_model **out);
+int zl_model_synth_ext(const zl_config *cfg, const zl_synth_tensor *tensors, int n, const zl_model_opts *opts,
+                       const zl_model_ext *ext, zl_model **out);
+
 /* ---------------------------------------------------------------------------------------------- timing probe */
 /* Mean duration of `iters` back-to-back launches of one GEMV of the forward pass (which: 0 first q/k/v group, 1 wo,
  * 2 gate+up, 3 down, 4 output head) with M tokens, cycling through the layers' weights, timed with HIP events on the

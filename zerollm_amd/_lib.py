@@ -62,7 +62,30 @@ class zl_spec_result(C.Structure):
                 ("ms_draft", C.c_float)]
 
 
+class zl_rows(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("seq", C.c_int64), ("tok", C.c_int64), ("head", C.c_int64)]
+
+
+class zl_batch(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("n_tok", C.c_int), ("pos", C.c_void_p), ("count", C.c_void_p), ("slot", C.c_void_p)]
+
+
+class zl_rope_opts(C.Structure):
+    _fields_ = [("n_rot", C.c_int), ("neox", C.c_int), ("base", C.c_double), ("scaling", C.c_int), ("orig_ctx", C.c_int),
+                ("factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("attn_factor", C.c_double),
+                ("freq_factors", C.POINTER(C.c_float))]
+
+
+class zl_model_ext(C.Structure):
+    _fields_ = [("kv_q4", C.c_int), ("rope", C.POINTER(zl_rope_opts))]
+
+
+DEVICE = 0  # the library's GPU (model.init)
+
 P = C.c_void_p
+ROWS = C.POINTER(zl_rows)
+BATCH = C.POINTER(zl_batch)
+I64P = C.POINTER(C.c_int64)
 I32P = C.POINTER(C.c_int32)
 F32P = C.POINTER(C.c_float)
 F64P = C.POINTER(C.c_double)
@@ -104,6 +127,22 @@ SIGNATURES = [
     ("zl_mat_gemv_time", C.c_int, [P, C.c_int, C.c_int, F32P]),
     ("zl_mat_gemv_noalloc", C.c_int, [P, P, C.c_int, P, P]),
     ("zl_quant_act", C.c_int, [F32P, C.c_int64, C.c_int, C.POINTER(C.c_int8), F32P, I32P]),
+    ("zl_kv4_create", C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int64, C.POINTER(P)]),
+    ("zl_kv4_free", C.c_int, [P]),
+    ("zl_kv4_bytes", C.c_int, [P, I64P]),
+    ("zl_kv4_append", C.c_int, [P, BATCH, C.c_int, ROWS, ROWS, P]),
+    ("zl_kv4_read", C.c_int, [P, BATCH, C.c_int, ROWS, ROWS, P]),
+    ("zl_kv4_attention", C.c_int, [P, BATCH, C.c_int, ROWS, C.c_int, C.c_float, ROWS, P, C.c_int64, P]),
+    ("zl_kv4_attention_work", C.c_int, [P, C.c_int, C.c_int, C.c_int, I64P]),
+    ("zl_rope_create", C.c_int, [C.POINTER(zl_rope_opts), C.POINTER(P)]),
+    ("zl_rope_free", C.c_int, [P]),
+    ("zl_rope_apply", C.c_int, [P, BATCH, C.c_int, C.c_int, ROWS, ROWS, C.c_int, ROWS, ROWS, C.c_int, P]),
+    ("zl_logprobs", C.c_int, [P, C.c_int, C.c_int64, C.c_int, C.c_int, P, C.c_int, P, P, P, P, P, C.c_int64, P]),
+    ("zl_logprobs_work", C.c_int, [C.c_int, C.c_int, C.c_int, I64P]),
+    ("zl_model_logprobs", C.c_int, [P, C.c_int, C.c_int, I32P, C.c_int, F32P, F32P, I32P, F32P]),
+    ("zl_model_load_ext", C.c_int, [C.c_char_p, C.POINTER(zl_model_opts), C.POINTER(zl_model_ext), C.POINTER(P)]),
+    ("zl_model_synth_ext", C.c_int, [C.POINTER(zl_config), C.POINTER(zl_synth_tensor), C.c_int, C.POINTER(zl_model_opts),
+                                     C.POINTER(zl_model_ext), C.POINTER(P)]),
     ("zl_probe_gemv", C.c_int, [P, C.c_int, C.c_int, C.c_int, F32P, C.POINTER(C.c_int64)]),
 ]
 

@@ -20,14 +20,18 @@
 
 #include "zerollm_hip.h"
 #include "gguf.h"
-#include "zl_kernels.h"
+#include "zl_api.h"
+#include "zl_ops.h"
+#include "zl_rope_freq.h"
 
 namespace zl {
 
 static thread_local std::string g_err;
 static int g_device = -1;
 
-static void ensure_init() {
+std::string &last_error() { return g_err; }
+int device() { return g_device; }
+void ensure_init() {
   if (g_device < 0) {
     int n = 0;
     ZL_HIP(hipGetDeviceCount(&n));
@@ -42,7 +46,7 @@ static int pad64(int n) { return (n + 63) / 64 * 64; }
 // ---------------------------------------------------------------------------------------------- allocations
 // Zero device memory before any stream uses it: hipMemset runs on the null stream, which does not order with the
 // library's non-blocking streams, so it is waited for here.
-static void zero_now(void *p, size_t n) {
+void zero_now(void *p, size_t n) {
   ZL_HIP(hipMemset(p, 0, n));
   ZL_HIP(hipDeviceSynchronize());
 }
@@ -225,6 +229,7 @@ struct zl_model {
   float *outputNorm = nullptr;
   std::vector<zl::Layer> layers;
   float *cosT = nullptr, *sinT = nullptr;
+  zl_rope_opts rope{};  // position scaling (rope.scaling 0: none)
   void *kcache = nullptr, *vcache = nullptr;
   float *x = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *hb = nullptr, *logits = nullptr;
   float *scores = nullptr;  // attention scores [maxBatch][n_head][ctx]
@@ -254,6 +259,9 @@ struct zl_model {
   float *dqkv = nullptr, *dz = nullptr, *dalpha = nullptr, *dbeta = nullptr;
   float *dxcore = nullptr;      // DeltaNet: the heads' output rows, between the recurrence and the gated norm
   zl::Step *dstep = nullptr;
+  // zl_model_logprobs: [tokens | lp | entropy | top_ids | top_lp] of logitsBatch rows and a work space, on first use
+  int32_t *lpDev = nullptr, *lpHost = nullptr;
+  void *lpWork = nullptr;
   hipStream_t st = nullptr;
   hipStream_t cst = nullptr;  // graphs are captured on their own stream
   std::vector<int> tokens;
@@ -325,6 +333,7 @@ zl_model::~zl_model() {
   for (auto &g : graphs) hipGraphExecDestroy(g.second);
   for (auto &g : graphDefs) hipGraphDestroy(g.second);
   ar.release();
+  if (lpHost) hipHostFree(lpHost);
   if (st) hipStreamDestroy(st);
   if (cst) hipStreamDestroy(cst);
 }
@@ -416,12 +425,21 @@ static void finish_model(zl_model *m, const float *ropeFreqs) {
   const int half = c.n_rot / 2;
   // RoPE tables exactly as ropeTables (src/compute/ref-kernels.js:329-342), in f64 on the host, stored f32
   std::vector<float> cs((size_t)m->ctx * half), sn((size_t)m->ctx * half);
+  std::vector<double> scaled;  // angles of scaled positions
+  double gain = 1.0;
+  if (m->rope.scaling) {
+    zl_rope_opts r = m->rope;
+    r.n_rot = c.n_rot; r.base = (double)c.rope_base; r.freq_factors = ropeFreqs;
+    if (!r.orig_ctx) r.orig_ctx = c.n_ctx_train;
+    rope_angles(r, &scaled, &gain);
+  }
   for (int i = 0; i < half; i++) {
     double freq = pow((double)c.rope_base, (-2.0 * i) / c.n_rot);
     if (ropeFreqs) freq /= (double)ropeFreqs[i];
+    if (m->rope.scaling) freq = scaled[i];
     for (int p = 0; p < m->ctx; p++) {
-      cs[(size_t)p * half + i] = (float)cos(p * freq);
-      sn[(size_t)p * half + i] = (float)sin(p * freq);
+      cs[(size_t)p * half + i] = (float)(cos(p * freq) * gain);
+      sn[(size_t)p * half + i] = (float)(sin(p * freq) * gain);
     }
   }
   m->cosT = (float *)m->ar.alloc(cs.size() * 4);
@@ -1060,6 +1078,22 @@ static zl_model *new_model(const zl_model_opts *o) {
   return m.release();
 }
 
+// The options of zl_model_ext; returns the context. Scaled positions reach factor times the trained context.
+static int take_ext(zl_model *m, const zl_model_ext *ext, int want_ctx) {
+  double most = m->cfg.n_ctx_train;
+  if (ext && ext->rope && ext->rope->scaling) {
+    zl_rope_opts r = *ext->rope;
+    r.n_rot = m->cfg.n_rot; r.base = (double)m->cfg.rope_base; r.freq_factors = nullptr;
+    if (!r.orig_ctx) r.orig_ctx = m->cfg.n_ctx_train;
+    std::vector<double> th;
+    double gain;
+    rope_angles(r, &th, &gain);  // its checks
+    m->rope = r;
+    most *= r.factor;
+  }
+  return (int)std::min((double)want_ctx, floor(most));
+}
+
 static void check_config(const zl_config &c) {
   ZL_REQUIRE(c.n_embd > 0 && c.n_layer > 0 && c.n_ff > 0 && c.n_head > 0 && c.n_head_kv > 0 && c.head_dim > 0 && c.vocab > 0,
              ZL_ERR_ARG, "bad model config");
@@ -1081,7 +1115,7 @@ static float *upload_vec(zl_model *m, const std::vector<float> &v) {
 }
 
 // ---- from GGUF (modelConfig, src/model/config.js:275-325; tensors as RefModel, src/model/forward.js:114-132)
-static zl_model *load_gguf(const char *path, const zl_model_opts *o) {
+static zl_model *load_gguf(const char *path, const zl_model_opts *o, const zl_model_ext *ext = nullptr) {
   GGUF g = read_gguf(path);
   const GGUFValue *av = g.get("general.architecture");
   ZL_REQUIRE(av && av->type == 8, ZL_ERR_FORMAT, "GGUF has no general.architecture");
@@ -1134,7 +1168,7 @@ static zl_model *load_gguf(const char *path, const zl_model_opts *o) {
   std::unique_ptr<zl_model> m(new_model(o));
   m->cfg = c;
   int want_ctx = o && o->ctx > 0 ? o->ctx : 2048;
-  m->ctx = std::min(want_ctx, c.n_ctx_train);
+  m->ctx = take_ext(m.get(), ext, want_ctx);
   FILE *f = fopen(path, "rb");
   ZL_REQUIRE(f != nullptr, ZL_ERR_IO, std::string("cannot open ") + path);
   struct Closer { FILE *f; ~Closer() { fclose(f); } } closer{f};
@@ -1251,7 +1285,8 @@ static void synth_to_device(const zl_synth_tensor &t, uint8_t *out, hipStream_t 
   launch_synth(t.type, t.seed, t.std, (uint64_t)(t.src_cols > 0 ? t.src_cols : t.cols), (uint64_t)t.col0, (int)t.rows, (int)t.cols, out, st);
 }
 
-static zl_model *build_synth(const zl_config *cfg, const zl_synth_tensor *ts, int n, const zl_model_opts *o) {
+static zl_model *build_synth(const zl_config *cfg, const zl_synth_tensor *ts, int n, const zl_model_opts *o,
+                             const zl_model_ext *ext = nullptr) {
   zl_config c = *cfg;
   check_config(c);
   std::map<std::string, const zl_synth_tensor *> byName;
@@ -1259,7 +1294,7 @@ static zl_model *build_synth(const zl_config *cfg, const zl_synth_tensor *ts, in
   std::unique_ptr<zl_model> m(new_model(o));
   m->cfg = c;
   int want_ctx = o && o->ctx > 0 ? o->ctx : 2048;
-  m->ctx = std::min(want_ctx, c.n_ctx_train);
+  m->ctx = take_ext(m.get(), ext, want_ctx);
   size_t maxBytes = 16;
   for (int i = 0; i < n; i++) if (!ts[i].fill) maxBytes = std::max(maxBytes, (size_t)ggml_row_bytes(ts[i].type, ts[i].cols) * (size_t)ts[i].rows);
   uint8_t *dstage = nullptr;
@@ -1449,6 +1484,40 @@ static void dist_of_row(zl_sampler *s, zl_model *m, int row, const int32_t *hist
   const int keep = upload_hist(s, m->st, hist, nh);
   launch_dist_rows(m->logits + (size_t)row * m->cfg.vocab, m->cfg.vocab, 1, m->cfg.vocab, s->sp, keep ? s->dhist : nullptr, keep, 0,
                    s->scratch, s->am, s->wide ? &s->ww : nullptr, &s->cw, out, m->st);
+}
+
+// Log probabilities of logits rows [row0, row0 + n), to host arrays.
+static void model_logprobs(zl_model *m, int row0, int n, const int32_t *tokens, int ntop, float *lp, float *ent, int32_t *ids,
+                           float *toplp) {
+  ZL_REQUIRE(!m->closed, ZL_ERR_STATE, "model is closed");
+  ZL_REQUIRE(row0 >= 0 && n >= 0 && row0 <= m->logitsBatch - n, ZL_ERR_ARG, "logits rows out of range");
+  ZL_REQUIRE(ntop >= 0 && ntop <= LOGPROB_MAX_TOP && ntop <= m->cfg.vocab, ZL_ERR_ARG,
+             "logprobs: n_top must be 0 to " + std::to_string(LOGPROB_MAX_TOP) + " and at most the vocabulary (got " + std::to_string(ntop) + ")");
+  ZL_REQUIRE(!lp || tokens, ZL_ERR_ARG, "log probabilities of given tokens need the tokens");
+  if (n == 0) return;
+  const int R = m->logitsBatch, top = std::min(LOGPROB_MAX_TOP, m->cfg.vocab);
+  if (!m->lpDev) {
+    const size_t words = (size_t)R * (3 + 2 * top);
+    long work = 0;  // (fewer rows split into more parts: the most of any count)
+    for (int r = 1; r <= R; r++) work = std::max({work, logprobs_work(r, m->cfg.vocab, top), logprobs_work(r, m->cfg.vocab, 0)});
+    m->lpWork = m->ar.alloc(work);
+    ZL_HIP(hipHostMalloc((void **)&m->lpHost, words * 4));
+    m->lpDev = (int32_t *)m->ar.alloc(words * 4);
+  }
+  int32_t *d = m->lpDev, *h = m->lpHost;
+  // [tokens n][lp n][entropy n][ids n ntop][top n ntop]
+  if (tokens) {
+    memcpy(h, tokens, (size_t)n * 4);
+    ZL_HIP(hipMemcpyAsync(d, h, (size_t)n * 4, hipMemcpyHostToDevice, m->st));
+  }
+  launch_logprobs(LogprobArgs{m->logits + (size_t)row0 * m->cfg.vocab, m->cfg.vocab, n, m->cfg.vocab, ntop, d, tokens ? (float *)(d + n) : nullptr,
+                              (float *)(d + 2 * n), d + 3 * n, (float *)(d + 3 * n + n * ntop), m->lpWork}, T_F32, m->st);
+  ZL_HIP(hipMemcpyAsync(h + n, d + n, (size_t)n * (2 + 2 * ntop) * 4, hipMemcpyDeviceToHost, m->st));
+  ZL_HIP(hipStreamSynchronize(m->st));
+  if (lp) memcpy(lp, h + n, (size_t)n * 4);
+  if (ent) memcpy(ent, h + 2 * n, (size_t)n * 4);
+  if (ids) memcpy(ids, h + 3 * n, (size_t)n * ntop * 4);
+  if (toplp) memcpy(toplp, h + 3 * n + n * ntop, (size_t)n * ntop * 4);
 }
 
 // ---------------------------------------------------------------------------------------------- speculative cycle
@@ -1751,20 +1820,6 @@ static void mat_gemv_noalloc(zl_mat *m, const float *x, int M, float *y, hipStre
 // ================================================================================================ C ABI
 using namespace zl;
 
-#define ZL_API_BEGIN try {
-#define ZL_API_END                              \
-  g_err.clear();                                \
-  return ZL_OK;                                 \
-  }                                             \
-  catch (const zl::Error &e) {                  \
-    g_err = e.what();                           \
-    return e.code;                              \
-  }                                             \
-  catch (const std::exception &e) {             \
-    g_err = e.what();                           \
-    return ZL_ERR_HIP;                          \
-  }
-
 extern "C" {
 
 const char *zl_last_error(void) { return g_err.c_str(); }
@@ -1801,6 +1856,23 @@ int zl_model_load(const char *path, const zl_model_opts *opts, zl_model **out) {
   ZL_REQUIRE(path && out, ZL_ERR_ARG, "null argument");
   ensure_init();
   *out = load_gguf(path, opts);
+  ZL_API_END
+}
+
+int zl_model_load_ext(const char *path, const zl_model_opts *opts, const zl_model_ext *ext, zl_model **out) {
+  ZL_API_BEGIN
+  ZL_REQUIRE(path && out, ZL_ERR_ARG, "null argument");
+  ensure_init();
+  *out = load_gguf(path, opts, ext);
+  ZL_API_END
+}
+
+int zl_model_synth_ext(const zl_config *cfg, const zl_synth_tensor *tensors, int n, const zl_model_opts *opts, const zl_model_ext *ext,
+                       zl_model **out) {
+  ZL_API_BEGIN
+  ZL_REQUIRE(cfg && tensors && out && n > 0, ZL_ERR_ARG, "null argument");
+  ensure_init();
+  *out = build_synth(cfg, tensors, n, opts, ext);
   ZL_API_END
 }
 
@@ -2046,6 +2118,14 @@ int zl_distribution(zl_sampler *s, zl_model *m, int row, const int32_t *hist, in
     for (int i = 0; i < d.n; i++) { ids[i] = d.ids[i]; probs[i] = d.probs[i]; }
   }
   *n = d.n; *total = d.total; *greedy = d.greedy;
+  ZL_API_END
+}
+
+int zl_model_logprobs(zl_model *m, int row0, int nrows, const int32_t *tokens, int n_top, float *lp, float *entropy,
+                      int32_t *top_ids, float *top_lp) {
+  ZL_API_BEGIN
+  ZL_REQUIRE(m, ZL_ERR_ARG, "null argument");
+  model_logprobs(m, row0, nrows, tokens, n_top, lp, entropy, top_ids, top_lp);
   ZL_API_END
 }
 

@@ -218,6 +218,7 @@ def verify_limit(model) -> int:
 
 def init(device: int = 0):
     call("zl_init", int(device))
+    _lib.DEVICE = int(device)
 
 
 def device_info():

@@ -1,0 +1,282 @@
+"""Operators of long contexts on device tensors: a KV cache held in 4 bits with the attention over it, rotary positions
+scaled beyond the trained context, log probabilities of logits rows (the C ABI's zl_kv4_*, zl_rope_*, zl_logprobs).
+
+Tensors are torch's (this module imports no torch of its own: it takes any tensor with torch's interface), on the library's
+GPU, float32, float16 or bfloat16, with any strides as long as the values of a head (of a logits row) are contiguous. Rows of
+several sequences are [sequence, token, head, dim], or [sequence, head, dim] for one token each. Positions, counts and slots
+are int32 tensors on the GPU, one entry per sequence, read when the work runs. Calls are enqueued on torch's current stream
+and return at once; with `out` and `work` given they allocate nothing and may be captured into a graph. Wrong shapes, types or
+places raise ValueError, what the library refuses ZLError.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import sys
+from dataclasses import dataclass
+
+import numpy as np
+
+from . import _lib
+from ._lib import call
+
+_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
+
+
+def _place(x, name):
+    d = getattr(x, "device", None)
+    if getattr(d, "type", None) != "cuda" or (d.index or 0) != _lib.DEVICE:
+        raise ValueError(f"{name} must be a tensor on GPU {_lib.DEVICE} (got {d})")
+
+
+def _type(x, name):
+    _place(x, name)
+    t = _TYPES.get(str(x.dtype))
+    if t is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16 (got {x.dtype})")
+    return t
+
+
+def _ints(x, n, name):
+    if x is None:
+        return None
+    _place(x, name)
+    if str(x.dtype) != "torch.int32" or tuple(x.shape) != (n,) or not x.is_contiguous():
+        raise ValueError(f"{name} must be {n} contiguous int32 values (got {x.dtype} {tuple(x.shape)})")
+    return x.data_ptr()
+
+
+def _rows(x, name, shape=None, type_=None, written=False):
+    """(zl_rows, type, shape as [sequence, token, head, dim]) of a tensor."""
+    t = _type(x, name)
+    s, st = tuple(x.shape), x.stride()
+    if len(s) == 3:
+        s, st = (s[0], 1, *s[1:]), (st[0], 0, *st[1:])
+    if len(s) != 4:
+        raise ValueError(f"{name} must be [sequence, token, head, dim] or [sequence, head, dim] (got {tuple(x.shape)})")
+    if st[3] != 1 and s[3] > 1:
+        raise ValueError(f"the values of a head of {name} must be contiguous (stride {st[3]})")
+    if shape is not None and s != shape:
+        raise ValueError(f"{name} must be {shape} (got {s})")
+    if type_ is not None and t != type_:
+        raise ValueError(f"{name} must have the type of the other rows (got {x.dtype})")
+    if written and any(n > 1 and d == 0 for n, d in zip(s, st)):
+        raise ValueError(f"{name} is written, so its rows must not share memory")
+    return _lib.zl_rows(x.data_ptr(), st[0], st[1], st[2]), t, s
+
+
+def _batch(n_seq, n_tok, pos, count, slot=None):
+    if pos is None:
+        raise ValueError("positions missing")
+    return _lib.zl_batch(n_seq, n_tok, _ints(pos, n_seq, "pos"), _ints(count, n_seq, "count"), _ints(slot, n_seq, "slot"))
+
+
+def _torch():
+    t = sys.modules.get("torch")
+    if t is None:
+        raise ValueError("these calls take torch tensors: import torch first")
+    return t
+
+
+def _stream():
+    return _torch().cuda.current_stream(_lib.DEVICE).cuda_stream
+
+
+def _work(work, nbytes, like):
+    """A work space of at least nbytes: the caller's, or one of torch's for this call."""
+    if work is None:
+        return _torch().empty(nbytes, dtype=_torch().uint8, device=like.device)
+    _place(work, "work")
+    if not work.is_contiguous() or work.numel() * work.element_size() < nbytes:
+        raise ValueError(f"work must be contiguous, {nbytes} bytes or more")
+    return work
+
+
+class KVCacheQ4:
+    """A KV cache of n_slot sequences of up to `capacity` positions, held as Q4_0 blocks: 1.125 bytes per (position, KV head,
+    dimension) for key and value together, where float16 takes 4."""
+
+    def __init__(self, n_slot: int, n_head_kv: int, head_dim: int, capacity: int):
+        self._h = C.c_void_p()
+        call("zl_kv4_create", int(n_slot), int(n_head_kv), int(head_dim), int(capacity), C.byref(self._h))
+        self.n_slot, self.n_head_kv, self.head_dim, self.capacity = int(n_slot), int(n_head_kv), int(head_dim), int(capacity)
+        self.closed = False
+
+    @property
+    def nbytes(self) -> int:
+        n = C.c_int64()
+        call("zl_kv4_bytes", self._handle(), C.byref(n))
+        return n.value
+
+    def _handle(self):
+        if self.closed:
+            raise _lib.ZLError(5, "cache is closed")
+        return self._h
+
+    def _kv(self, k, v, written):
+        kr, t, s = _rows(k, "k", written=written)
+        if s[2:] != (self.n_head_kv, self.head_dim):
+            raise ValueError(f"k must hold {self.n_head_kv} heads of {self.head_dim} values (got {s[2:]})")
+        return kr, _rows(v, "v", s, t, written)[0], t, s
+
+    def append(self, k, v, pos, count=None, slot=None):
+        """Put k and v at positions pos[s], pos[s] + 1, ... of each sequence s (of its slot: s itself without `slot`); only
+        the first count[s] tokens where `count` is given."""
+        kr, vr, t, s = self._kv(k, v, False)
+        call("zl_kv4_append", self._handle(), _batch(s[0], s[1], pos, count, slot), t, kr, vr, _stream())
+
+    def read(self, k, v, pos, count=None, slot=None):
+        """Fill k and v with what the cache holds at those positions; returns (k, v)."""
+        kr, vr, t, s = self._kv(k, v, True)
+        call("zl_kv4_read", self._handle(), _batch(s[0], s[1], pos, count, slot), t, kr, vr, _stream())
+        return k, v
+
+    def work_bytes(self, n_seq: int, n_tok: int, n_head: int) -> int:
+        n = C.c_int64()
+        call("zl_kv4_attention_work", self._handle(), int(n_seq), int(n_tok), int(n_head), C.byref(n))
+        return n.value
+
+    def attend(self, q, pos, count=None, slot=None, scale=None, out=None, work=None):
+        """Causal attention of the queries over the cache: token j of sequence s sees positions 0 .. pos[s] + j, which must
+        have been appended, its own key and value among them. scale None: 1/sqrt(head_dim). A token at a negative position
+        gets zeros, one past the capacity or of a slot that does not exist NaN. Returns `out` (may be q itself)."""
+        qr, t, s = _rows(q, "q")
+        if s[3] != self.head_dim:
+            raise ValueError(f"q must have heads of {self.head_dim} values (got {s[3]})")
+        if scale is not None and not scale > 0:
+            raise ValueError(f"scale must be positive (got {scale})")
+        b = _batch(s[0], s[1], pos, count, slot)
+        if out is None:
+            out = _torch().empty(tuple(q.shape), dtype=q.dtype, device=q.device)
+        o = _rows(out, "out", s, t, True)[0]
+        n = C.c_int64()
+        call("zl_kv4_attention_work", self._handle(), s[0], s[1], s[2], C.byref(n))
+        w = _work(work, n.value, q)
+        call("zl_kv4_attention", self._h, b, t, qr, s[2], scale or 0.0, o, w.data_ptr(), w.numel() * w.element_size(), _stream())
+        return out
+
+    def close(self):
+        """Release the cache once the GPU is done with it (idempotent)."""
+        if not self.closed:
+            self.closed = True
+            call("zl_kv4_free", self._h)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+SCALINGS = {None: 0, "none": 0, "linear": 1, "yarn": 2}
+
+
+def rope_opts(n_rot=0, neox=True, base=10000.0, scaling=None, factor=1.0, orig_ctx=0, beta_fast=0.0, beta_slow=0.0,
+              attn_factor=0.0, freq_factors=None):
+    """zl_rope_opts from names (the meanings are Rope's)."""
+    if scaling not in SCALINGS:
+        raise ValueError(f'scaling must be none, linear or yarn (got "{scaling}")')
+    ff = None
+    if freq_factors is not None:
+        ff = np.ascontiguousarray(freq_factors, np.float32)
+        if ff.shape != (n_rot // 2,):
+            raise ValueError(f"freq_factors must be {n_rot // 2} values (got {ff.shape})")
+    o = _lib.zl_rope_opts(n_rot=int(n_rot), neox=1 if neox else 0, base=float(base), scaling=SCALINGS[scaling],
+                          orig_ctx=int(orig_ctx), factor=float(factor), beta_fast=float(beta_fast or 0.0),
+                          beta_slow=float(beta_slow or 0.0), attn_factor=float(attn_factor or 0.0),
+                          freq_factors=_lib.ptr(ff, C.c_float) if ff is not None else None)
+    o._keep = ff
+    return o
+
+
+class Rope:
+    """Rotary positions of the first n_rot values of a head: pairs (i, i + n_rot/2) (neox) or (2i, 2i + 1), by
+    pos * base^(-2i/n_rot) / freq_factors[i] radians. scaling "linear": angles divided by factor; "yarn": by parts, between
+    pairs that turn beta_fast (32) and beta_slow (1) times within orig_ctx positions, and everything times attn_factor
+    (0.1 ln factor + 1)."""
+
+    def __init__(self, n_rot, neox=True, base=10000.0, scaling=None, factor=1.0, orig_ctx=0, beta_fast=0.0, beta_slow=0.0,
+                 attn_factor=0.0, freq_factors=None):
+        o = rope_opts(n_rot, neox, base, scaling, factor, orig_ctx, beta_fast, beta_slow, attn_factor, freq_factors)
+        self._h = C.c_void_p()
+        call("zl_rope_create", C.byref(o), C.byref(self._h))
+        self.n_rot = int(n_rot)
+        self.closed = False
+
+    def apply(self, q, k, pos, count=None, out=None):
+        """q and k (or None) rotated to positions pos[s], pos[s] + 1, ... of each sequence, in one launch. out: (q', k'), which
+        may be q and k themselves; new tensors without it. Returns (q', k')."""
+        if self.closed:
+            raise _lib.ZLError(5, "rope is closed")
+        qr, t, s = _rows(q, "q")
+        if out is None:
+            out = tuple(None if x is None else _torch().empty(tuple(x.shape), dtype=x.dtype, device=x.device) for x in (q, k))
+        qo = _rows(out[0], "out[0]", s, t, True)[0]
+        kr = ko = None
+        nk = 0
+        if k is not None:
+            nk = k.shape[-2] if len(k.shape) >= 3 else 0
+            ks = (s[0], s[1], nk, s[3])
+            kr, ko = _rows(k, "k", ks, t)[0], _rows(out[1], "out[1]", ks, t, True)[0]
+        call("zl_rope_apply", self._h, _batch(s[0], s[1], pos, count), t, s[3], qr, qo, s[2], kr, ko, nk, _stream())
+        return out
+
+    def close(self):
+        """Release the tables once the GPU is done with them (idempotent)."""
+        if not self.closed:
+            self.closed = True
+            call("zl_rope_free", self._h)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+@dataclass
+class LogProbs:
+    """Of each row: the log probability of its given token (None without tokens), the entropy in nats, and the ids and log
+    probabilities of the largest logits, largest first, the lowest id first among equals (None with top 0)."""
+    logprobs: object
+    entropy: object
+    top_ids: object
+    top_logprobs: object
+
+
+def logprobs_work_bytes(rows: int, vocab: int, top: int = 0) -> int:
+    n = C.c_int64()
+    call("zl_logprobs_work", int(rows), int(vocab), int(top), C.byref(n))
+    return n.value
+
+
+def logprobs(logits, tokens=None, top: int = 0, out=None, work=None) -> LogProbs:
+    """LogProbs of logits rows [rows, vocab] (any row stride). tokens: int32 [rows]; an id outside the vocabulary gives NaN.
+    top: 0 to 64 alternatives. Logits of -inf have probability 0; a row with NaN or +inf, or with nothing above -inf, is NaN."""
+    t = _type(logits, "logits")
+    if len(logits.shape) != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    tok = _ints(tokens, rows, "tokens")
+    torch = _torch()
+    n = C.c_int64()
+    call("zl_logprobs_work", rows, vocab, int(top), C.byref(n))
+    if out is None:
+        def new(shape, dtype):
+            return torch.empty(shape, dtype=dtype, device=logits.device)
+
+        out = LogProbs(new(rows, torch.float32) if tokens is not None else None, new(rows, torch.float32),
+                       new((rows, top), torch.int32) if top else None, new((rows, top), torch.float32) if top else None)
+    p = []
+    for x, shape, dtype in ((out.logprobs, (rows,), torch.float32), (out.entropy, (rows,), torch.float32),
+                            (out.top_ids, (rows, top), torch.int32), (out.top_logprobs, (rows, top), torch.float32)):
+        if x is None:
+            p.append(None)
+            continue
+        _place(x, "out")
+        if tuple(x.shape) != shape or x.dtype != dtype or not x.is_contiguous():
+            raise ValueError(f"out must be contiguous {dtype} {shape} (got {x.dtype} {tuple(x.shape)})")
+        p.append(x.data_ptr())
+    w = _work(work, n.value, logits)
+    call("zl_logprobs", logits.data_ptr(), t, logits.stride(0) if rows > 1 else vocab, rows, vocab, tok, int(top), *p,
+         w.data_ptr(), w.numel() * w.element_size(), _stream())
+    return out
