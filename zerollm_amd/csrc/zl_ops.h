@@ -67,7 +67,9 @@ struct Kv4Attn {
   int nhead;
   float scale;
   void *work;
+  int nrec;        // records per row in work (set by the launcher)
 };
+void kv4_prepare(int hd);  // once before launches of this head size
 long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead);
 void launch_kv4_attention(const Kv4Attn &a, int type, hipStream_t st);
 
