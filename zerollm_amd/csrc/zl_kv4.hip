@@ -145,18 +145,11 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// The eight codes of a word as f16 operands: pair r of (word >> 4 r). As they lie they are f16 denormals, code 2^-24, which
-// the matrix cores take as they are: the keys' form, whose queries carry the 2^24 and whose sums start at -8 sum q.
-__device__ __forceinline__ h8 unpack_tiny(uint32_t w) {
-  u4 x;
-  #pragma unroll
-  for (int r = 0; r < 4; r++) x[r] = (w >> (4 * r)) & 0x000f000fu;
-  return __builtin_bit_cast(h8, x);
-}
-// Codes less 8: under the exponent of 1024, less 1032. (The values' form: their weights are all positive, so that sums of
-// codes would be far larger than the sums of codes less 8 and lose bits.) k: 0x64006400 in a vector register, so that and
-// and or are one instruction (which takes a single scalar operand).
-__device__ __forceinline__ h8 unpack_signed(uint32_t w, uint32_t k) {
+// The eight codes of a word less 8, as f16: pair r of (word >> 4 r) under the exponent of 1024, less 1032. k: 0x64006400 in a
+// vector register, so that and and or are one instruction (which takes a single scalar operand). Codes as they lie are f16
+// denormals, which the matrix cores take as well and which cost no and-or and no subtraction; but sums that start at -8 sum q
+// to make up for it lose five bits (outputs 7e-6 off float64's, against 2e-7), and the time is the same.
+__device__ __forceinline__ h8 unpack8(uint32_t w, uint32_t k) {
   h8 x;
   #pragma unroll
   for (int r = 0; r < 4; r++) {
@@ -232,10 +225,9 @@ struct Sum {
 template <int NB>
 struct Queries {
   h8 hi[NB], lo[NB];
-  f4 z[NB];  // -8 2^-24 times the sum of block b of the lane's row: where the scores' sums start
   float c;
 };
-template <int NB, int TYPE, bool LOQ>
+template <int NB, int TYPE>
 __device__ __forceinline__ void load_queries(Queries<NB> &q, const typename ValueOf<TYPE>::t *row, float scale, int lane) {
   typedef typename ValueOf<TYPE>::t T;
   float v[NB][8], am = 0.0f;
@@ -259,18 +251,14 @@ __device__ __forceinline__ void load_queries(Queries<NB> &q, const typename Valu
   const bool fine = am < INFINITY;  // (a row with a value that is not finite is NaN)
   #pragma unroll
   for (int b = 0; b < NB; b++) {
-    float sum = 0.0f;
     #pragma unroll
     for (int e = 0; e < 8; e++) {
       const float x = fine ? ldexpf(v[b][e], ex) : NAN;
       q.hi[b][e] = (_Float16)x;
       q.lo[b][e] = (_Float16)(x - (float)q.hi[b][e]);
-      sum += LOQ ? x : (float)q.hi[b][e];
     }
-    sum = sum4(sum) * -4.76837158203125e-07f;  // -8 2^-24
-    q.z[b] = f4{sum, sum, sum, sum};
   }
-  q.c = fmaxf((float)ldexp((double)scale * 1.4426950408889634, 24 - ex), 1.17549435e-38f);  // (not 0: it multiplies -inf)
+  q.c = fmaxf((float)ldexp((double)scale * 1.4426950408889634, -ex), 1.17549435e-38f);  // (not 0: it multiplies -inf)
 }
 
 // One span: records rec and rec + 36 HD, of which the lane's row sees positions 0 .. lim (63 or more: all). o[4 j + v] is
@@ -308,8 +296,8 @@ __device__ __forceinline__ void span_sum(Sum<8 * NB> &r, const uint8_t *rec, con
       s[i][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
       #pragma unroll
       for (int b = 0; b < NB; b++) {
-        const h8 k = unpack_tiny(kw[i][(t * NB + b) >> 2][(t * NB + b) & 3]);
-        f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.hi[b], q.z[b], 0, 0, 0);
+        const h8 k = unpack8(kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], k1024);
+        f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.hi[b], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
         if (LOQ) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.lo[b], acc, 0, 0, 0);
         #pragma unroll
         for (int v = 0; v < 4; v++) s[i][t][v] = fmaf(acc[v], scale_at(ks[i], t * NB + b, v), s[i][t][v]);
@@ -374,7 +362,7 @@ __device__ __forceinline__ void span_sum(Sum<8 * NB> &r, const uint8_t *rec, con
       const h8 hi = __builtin_bit_cast(h8, hu), lo = __builtin_bit_cast(h8, lu);
       #pragma unroll
       for (int j = 2 * b; j < 2 * b + 2; j++) {
-        const h8 x = unpack_signed(vw[i][j >> 2][j & 3], k1024);
+        const h8 x = unpack8(vw[i][j >> 2][j & 3], k1024);
         o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, o[j], 0, 0, 0);
         if (LOW) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, o[j], 0, 0, 0);
       }
@@ -442,7 +430,7 @@ __global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int 
   if (most < 0 || (int)blockIdx.x * CHUNK > most) return;
   typedef typename ValueOf<TYPE>::t T;
   Queries<NB> q;
-  load_queries<NB, TYPE, LOQ>(q, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.scale, lane);
+  load_queries<NB, TYPE>(q, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.scale, lane);
   float2 *ml = (float2 *)(lds + SPANS * nr * LDO);
   for (int c = blockIdx.x; c * CHUNK <= most; c += gridDim.x) {
     const int p0 = c * CHUNK + wave * SPAN;
@@ -533,7 +521,7 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int tiles4) 
   if (most < part * PART) return;
   typedef typename ValueOf<TYPE>::t T;
   Queries<NB> q;
-  load_queries<NB, TYPE, LOQ>(q, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.scale, lane);
+  load_queries<NB, TYPE>(q, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.scale, lane);
   Sum<8 * NB> f, u, r;
   f.clear();
   for (int c = part * CHUNKS; c < (part + 1) * CHUNKS && c * CHUNK <= most; c++) {
