@@ -261,117 +261,100 @@ __device__ __forceinline__ void load_queries(Queries<NB> &q, const typename Valu
   q.c = fmaxf((float)ldexp((double)scale * 1.4426950408889634, -ex), 1.17549435e-38f);  // (not 0: it multiplies -inf)
 }
 
-// One span: records rec and rec + 36 HD, of which the lane's row sees positions 0 .. lim (63 or more: all). o[4 j + v] is
-// dimension 16 j + 4 (l / 16) + v of row l % 16.
-template <int NB, bool LOQ, bool LOW>
-__device__ __forceinline__ void span_sum(Sum<8 * NB> &r, const uint8_t *rec, const Queries<NB> &q, int lim, int lane) {
-  constexpr int HD = 32 * NB, REC = 36 * HD, NV = NB / 2;
-  const int g = lane >> 4;
-  uint32_t k1024 = 0x64006400u;
-  __asm__("" : "+v"(k1024));
-  u4 kw[2][NV], vw[2][NV], ks[2][NB], vs[2][NB];
-  #pragma unroll
-  for (int i = 0; i < 2; i++) {
+// A lane's share of a span (two records): code words and scales, loaded with every lane's 16-byte loads side by side.
+template <int NB>
+struct SpanWords {
+  static constexpr int HD = 32 * NB, REC = 36 * HD, NV = NB / 2;
+  u4 kw[2][NV], ks[2][NB], vw[2][NV], vs[2][NB];
+  __device__ __forceinline__ void load_keys(const uint8_t *rec, int lane) {
     #pragma unroll
-    for (int j = 0; j < NV; j++) kw[i][j] = ((const u4 *)(rec + i * REC))[j * 64 + lane];
-    #pragma unroll
-    for (int j = 0; j < NB; j++) ks[i][j] = ((const u4 *)(rec + i * REC + 32 * HD))[g * NB + j];
+    for (int i = 0; i < 2; i++) {
+      #pragma unroll
+      for (int j = 0; j < NV; j++) kw[i][j] = ((const u4 *)(rec + i * REC))[j * 64 + lane];
+      #pragma unroll
+      for (int j = 0; j < NB; j++) ks[i][j] = ((const u4 *)(rec + i * REC + 32 * HD))[(lane >> 4) * NB + j];
+    }
   }
-  auto load_values = [&]() {
+  __device__ __forceinline__ void load_values(const uint8_t *rec, int lane) {
     #pragma unroll
     for (int i = 0; i < 2; i++) {
       #pragma unroll
       for (int j = 0; j < NV; j++) vw[i][j] = ((const u4 *)(rec + i * REC + 16 * HD))[j * 64 + lane];
       #pragma unroll
-      for (int j = 0; j < NB; j++) vs[i][j] = ((const u4 *)(rec + i * REC + 34 * HD))[g * NB + j];
+      for (int j = 0; j < NB; j++) vs[i][j] = ((const u4 *)(rec + i * REC + 34 * HD))[(lane >> 4) * NB + j];
     }
-  };
-  if (NB <= 4) load_values();  // (heads of 256 would not leave registers for them)
-  __builtin_amdgcn_sched_barrier(0);
-  f4 s[2][2];
-  #pragma unroll
-  for (int i = 0; i < 2; i++)
-    #pragma unroll
-    for (int t = 0; t < 2; t++) {
-      s[i][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-      #pragma unroll
-      for (int b = 0; b < NB; b++) {
-        const h8 k = unpack8(kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], k1024);
-        f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.hi[b], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-        if (LOQ) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.lo[b], acc, 0, 0, 0);
-        #pragma unroll
-        for (int v = 0; v < 4; v++) s[i][t][v] = fmaf(acc[v], scale_at(ks[i], t * NB + b, v), s[i][t][v]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  if (NB > 4) load_values();
-  // positions that a row of the tile does not see: no weight, and a scale of 0 (a stale one may be NaN)
-  if (__ballot(lim < SPAN - 1)) {
-    #pragma unroll
-    for (int i = 0; i < 2; i++)
-      #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const int n = lim - 32 * i - 16 * t - 4 * g;  // the last of the lane's four positions that is seen
-        #pragma unroll
-        for (int v = 0; v < 4; v++) s[i][t][v] = v > n ? -INFINITY : s[i][t][v];
-        const uint32_t m0 = n >= 1 ? 0xffffffffu : n >= 0 ? 0xffffu : 0u, m1 = n >= 3 ? 0xffffffffu : n >= 2 ? 0xffffu : 0u;
-        #pragma unroll
-        for (int b = 0; b < NB; b++) {
-          const int e = t * NB + b;
-          vs[i][e >> 1][2 * (e & 1)] &= m0;
-          vs[i][e >> 1][2 * (e & 1) + 1] &= m1;
-        }
-      }
   }
-  float m = -INFINITY;
+};
+
+// Scores of 16 positions (tile t of a record) in code units, from the tile's operands k(b) and key scales.
+template <int NB, bool LOQ, class K>
+__device__ __forceinline__ f4 tile_scores(const K &k, const u4 (&ks)[NB], int t, const Queries<NB> &q) {
+  f4 s = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  #pragma unroll
+  for (int b = 0; b < NB; b++) {
+    const h8 x = k(b);
+    f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[b], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+    if (LOQ) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.lo[b], acc, 0, 0, 0);
+    #pragma unroll
+    for (int v = 0; v < 4; v++) s[v] = fmaf(acc[v], scale_at(ks, t * NB + b, v), s[v]);
+  }
+  return s;
+}
+
+// Positions that the lane's row does not see (those behind lim of the span): no weight, ...
+__device__ __forceinline__ void mask_scores(f4 (&s)[2][2], int lim, int g) {
+  #pragma unroll
+  for (int i = 0; i < 2; i++)
+    #pragma unroll
+    for (int t = 0; t < 2; t++)
+      #pragma unroll
+      for (int v = 0; v < 4; v++) s[i][t][v] = 32 * i + 16 * t + 4 * g + v > lim ? -INFINITY : s[i][t][v];
+}
+// ... and a scale of 0 (a stale one may be NaN): d, the pairs of block b in record i.
+__device__ __forceinline__ void mask_scales(uint32_t (&d)[4], int i, int lim, int g) {
+  #pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int n = lim - 32 * i - 16 * t - 4 * g;  // the last of the lane's four positions that is seen
+    d[2 * t] &= n >= 1 ? 0xffffffffu : n >= 0 ? 0xffffu : 0u;
+    d[2 * t + 1] &= n >= 3 ? 0xffffffffu : n >= 2 ? 0xffffu : 0u;
+  }
+}
+
+// Scores to weights, in place; the span's reference and the sum of its weights.
+__device__ __forceinline__ void span_softmax(f4 (&s)[2][2], float c, float &m, float &l) {
+  float x = -INFINITY;
+  #pragma unroll
+  for (int i = 0; i < 2; i++)
+    #pragma unroll
+    for (int t = 0; t < 2; t++)
+      #pragma unroll
+      for (int v = 0; v < 4; v++) x = fmaxf(x, s[i][t][v]);
+  x = max4(x);
+  const float ref = x == -INFINITY ? 0.0f : x;
+  l = 0.0f;
   #pragma unroll
   for (int i = 0; i < 2; i++)
     #pragma unroll
     for (int t = 0; t < 2; t++)
       #pragma unroll
       for (int v = 0; v < 4; v++) {
-        m = fmaxf(m, s[i][t][v]);
-      }
-  m = max4(m);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
-  #pragma unroll
-  for (int i = 0; i < 2; i++)
-    #pragma unroll
-    for (int t = 0; t < 2; t++)
-      #pragma unroll
-      for (int v = 0; v < 4; v++) {
-        s[i][t][v] = exp2_(fmaf(s[i][t][v] - ref, q.c, 3.0f));
+        s[i][t][v] = exp2_(fmaf(s[i][t][v] - ref, c, 3.0f));
         l += s[i][t][v];
       }
-  r.m = m * q.c - 3.0f;
-  r.l = sum4(l);
-  __builtin_amdgcn_sched_barrier(0);
-  f4 o[2 * NB];
-  #pragma unroll
-  for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  #pragma unroll
-  for (int i = 0; i < 2; i++)
-    #pragma unroll
-    for (int b = 0; b < NB; b++) {
-      u4 hu, lu;
-      const float p[8] = {s[i][0][0], s[i][0][1], s[i][0][2], s[i][0][3], s[i][1][0], s[i][1][1], s[i][1][2], s[i][1][3]};
-      const uint32_t d[4] = {vs[i][b >> 1][2 * (b & 1)], vs[i][b >> 1][2 * (b & 1) + 1], vs[i][(NB + b) >> 1][2 * (b & 1)],
-                             vs[i][(NB + b) >> 1][2 * (b & 1) + 1]};
-      weigh8<LOW>(p, d, hu, lu);
-      const h8 hi = __builtin_bit_cast(h8, hu), lo = __builtin_bit_cast(h8, lu);
-      #pragma unroll
-      for (int j = 2 * b; j < 2 * b + 2; j++) {
-        const h8 x = unpack8(vw[i][j >> 2][j & 3], k1024);
-        o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, o[j], 0, 0, 0);
-        if (LOW) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, o[j], 0, 0, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  #pragma unroll
-  for (int j = 0; j < 2 * NB; j++)
-    #pragma unroll
-    for (int v = 0; v < 4; v++) r.o[4 * j + v] = o[j][v];
+  m = x * c - 3.0f;
+  l = sum4(l);
+}
+
+// Weights of record i times the value scales of block b, as right operands.
+template <int NB, bool LOW>
+__device__ __forceinline__ void weigh(const f4 (&s)[2][2], const u4 (&vs)[NB], int i, int b, bool masked, int lim, int g, h8 &hi, h8 &lo) {
+  const float p[8] = {s[i][0][0], s[i][0][1], s[i][0][2], s[i][0][3], s[i][1][0], s[i][1][1], s[i][1][2], s[i][1][3]};
+  uint32_t d[4] = {vs[b >> 1][2 * (b & 1)], vs[b >> 1][2 * (b & 1) + 1], vs[(NB + b) >> 1][2 * (b & 1)], vs[(NB + b) >> 1][2 * (b & 1) + 1]};
+  if (masked) mask_scales(d, i, lim, g);
+  u4 hu, lu;
+  weigh8<LOW>(p, d, hu, lu);
+  hi = __builtin_bit_cast(h8, hu);
+  lo = __builtin_bit_cast(h8, lu);
 }
 
 // The rows of a block: tile t of KV head kvh of sequence s. A row's last position; below 0 it sees nothing.
@@ -409,12 +392,18 @@ __device__ __forceinline__ void emit(const Kv4Attn &a, int s, int tok, int head,
 }
 
 // Few rows: a block takes one tile of 16 rows and a chunk at a time (chunks x, x + X, ...), one span per wave, and folds the
-// spans in LDS. Rows that see a single chunk are finished here, the others leave the chunk's record.
+// spans in LDS. Rows that see a single chunk are finished here, the others leave the chunk's record. The next chunk's keys are
+// requested when the scores are done with this one's, its values after the weighted sums, so that the loads run under the
+// rest; two buffers in LDS, so that a block meets once per chunk.
+template <int NB>
+constexpr int chunk_buffers() { return NB <= 4 ? 2 : 1; }  // (heads of 256: 133 KB each)
+template <int NB>
+constexpr size_t chunk_lds(int nr) { return (size_t)chunk_buffers<NB>() * SPANS * (nr * (32 * NB + 4) + 32) * 4; }
 template <int NB, int TYPE>
 __global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int tiles) {
-  constexpr int HD = 32 * NB, LDO = HD + 4;
+  constexpr int HD = 32 * NB, LDO = HD + 4, NBUF = chunk_buffers<NB>();
   constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16;
-  extern __shared__ __align__(16) float lds[];  // [spans][rows][LDO], then (m, l) [spans][16]
+  extern __shared__ __align__(16) float lds_all[];  // per buffer: [spans][rows][LDO], then (m, l) [spans][16]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
   const Tile tl(a, blockIdx.z, blockIdx.y / tiles, blockIdx.y % tiles * 16);
   const int nr = min(16, a.b.ntok * tl.group - tl.base);
@@ -429,22 +418,65 @@ __global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int 
     for (int i = 0; i < NB; i++) emit<TYPE>(a, tl.s, ft, fh, 32 * i + fl, flast == ROW_NONE ? 0.0f : NAN);
   if (most < 0 || (int)blockIdx.x * CHUNK > most) return;
   typedef typename ValueOf<TYPE>::t T;
+  uint32_t k1024 = 0x64006400u;
+  __asm__("" : "+v"(k1024));
+  // (a wave whose span lies behind the last position reads its chunk's first record, for nothing)
+  const uint8_t *head0 = record_of(a.c, tl.slot, tl.kvh, 0);
+  auto record_at = [&](int c) {
+    const int p0 = c * CHUNK + wave * SPAN;
+    return head0 + (long)((p0 <= most ? p0 : min(c * CHUNK, most)) / SPAN) * (2 * kv4_record(HD));
+  };
+  SpanWords<NB> w;
+  w.load_keys(record_at(blockIdx.x), lane);
+  if (NB <= 4) w.load_values(record_at(blockIdx.x), lane);
   Queries<NB> q;
   load_queries<NB, TYPE>(q, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.scale, lane);
-  float2 *ml = (float2 *)(lds + SPANS * nr * LDO);
+  int buf = 0;
   for (int c = blockIdx.x; c * CHUNK <= most; c += gridDim.x) {
-    const int p0 = c * CHUNK + wave * SPAN;
-    if (p0 <= most) {
-      Sum<8 * NB> r;
-      const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, p0 / KV4_GROUP);
-      const int lim = last - p0;
-      span_sum<NB, LOQ, LOW>(r, rec, q, lim, lane);
-      if (n < nr) {
-        float *d = lds + (wave * nr + n) * LDO + 4 * g;
-        #pragma unroll
-        for (int j = 0; j < 2 * NB; j++) *(float4 *)(d + 16 * j) = make_float4(r.o[4 * j], r.o[4 * j + 1], r.o[4 * j + 2], r.o[4 * j + 3]);
-        if (g == 0) ml[wave * 16 + n] = make_float2(r.m, r.l);
+    float *lds = lds_all + buf * SPANS * (nr * LDO + 32);
+    float2 *ml = (float2 *)(lds + SPANS * nr * LDO);
+    const int p0 = c * CHUNK + wave * SPAN, lim = last - p0;
+    const uint8_t *next = record_at(c + gridDim.x);
+    const bool masked = __ballot(lim < SPAN - 1) != 0;
+    f4 s[2][2];
+    #pragma unroll
+    for (int i = 0; i < 2; i++)
+      #pragma unroll
+      for (int t = 0; t < 2; t++) {
+        s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], k1024); }, w.ks[i], t, q);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    if (NB <= 4) w.load_keys(next, lane);
+    else w.load_values(record_at(c), lane);  // (heads of 256 leave no registers for loads ahead)
+    __builtin_amdgcn_sched_barrier(0);
+    if (masked) mask_scores(s, lim, g);
+    float m, l;
+    span_softmax(s, q.c, m, l);
+    f4 o[2 * NB];
+    #pragma unroll
+    for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    #pragma unroll
+    for (int i = 0; i < 2; i++)
+      #pragma unroll
+      for (int b = 0; b < NB; b++) {
+        h8 hi, lo;
+        weigh<NB, LOW>(s, w.vs[i], i, b, masked, lim, g, hi, lo);
+        #pragma unroll
+        for (int j = 2 * b; j < 2 * b + 2; j++) {
+          const h8 x = unpack8(w.vw[i][j >> 2][j & 3], k1024);
+          o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, o[j], 0, 0, 0);
+          if (LOW) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, o[j], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    if (NB <= 4) w.load_values(next, lane);
+    else w.load_keys(next, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    if (p0 <= most && n < nr) {
+      float *d = lds + (wave * nr + n) * LDO + 4 * g;
+      #pragma unroll
+      for (int j = 0; j < 2 * NB; j++) *(f4 *)(d + 16 * j) = o[j];
+      if (g == 0) ml[wave * 16 + n] = make_float2(m, l);
     }
     __syncthreads();
     if (flast >= c * CHUNK) {
@@ -470,82 +502,234 @@ __global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int 
         if (fl == 0) *record_ml(a, row, c) = make_float2(f.m, f.l);
       }
     }
-    __syncthreads();
+    if (NBUF == 2) buf ^= 1;
+    else __syncthreads();
   }
 }
 
-// Rows of several records: 32 lanes per row; `per` records fold into a part, parts into the row. Rows that see at most
-// `done` positions have been finished.
-template <int NB, int TYPE>
-__global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a, int done, int reclen) {
-  const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int fl = threadIdx.x & 31;
-  if (row >= (long)a.b.nseq * a.b.ntok * a.nhead) return;
+// Rows of several records: a block per (row, 32 dimensions), a dimension per lane. Eight groups of 32 lanes fold the records
+// of JOIN_PARTS parts side by side (a group's loads issued together), then one folds the parts into the row, in order.
+constexpr int JOIN_PARTS = 32;
+template <int PER, int TYPE>
+__global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a) {
+  __shared__ float po[JOIN_PARTS][32];
+  __shared__ float2 pml[JOIN_PARTS];
+  constexpr int LEN = PART / PER;  // positions per record
+  const long row = blockIdx.x;
+  const int fl = threadIdx.x & 31, grp = threadIdx.x >> 5, dim = blockIdx.y * 32 + fl;
   const int head = (int)(row % a.nhead), tok = (int)(row / a.nhead % a.b.ntok), s = (int)(row / a.nhead / a.b.ntok);
   const Tile tl(a, s, 0, 0);
   const long last = (long)a.b.pos[s] + tok;
-  if (!tl.ok || tok >= tl.ntok || last < done || last >= a.c.cap) return;
-  const int nrec = (int)(last / reclen) + 1, per = PART / reclen;
-  Sum<NB> f, u, p;
+  if (!tl.ok || tok >= tl.ntok || last < LEN || last >= a.c.cap) return;
+  const int nrec = (int)(last / LEN) + 1, np = (nrec + PER - 1) / PER;
+  const float *o = record_o(a, row, 0) + dim;
+  const float2 *ml = record_ml(a, row, 0);
+  Sum<1> f;
   f.clear();
-  u.clear();
-  for (int c = 0; c < nrec; c++) {
-    const float2 v = *record_ml(a, row, c);
-    const float *o = record_o(a, row, c);
-    p.m = v.x;
-    p.l = v.y;
+  for (int b0 = 0; b0 < np; b0 += JOIN_PARTS) {
+    constexpr int R = JOIN_PARTS / 8;  // parts per group: grp, grp + 8, ...
+    float x[R][PER];
+    float2 v[R][PER];
     #pragma unroll
-    for (int i = 0; i < NB; i++) p.o[i] = o[32 * i + fl];
-    u.fold(p);
-    if (c % per == per - 1 || c == nrec - 1) {
-      f.fold(u);
+    for (int r = 0; r < R; r++)
+      #pragma unroll
+      for (int k = 0; k < PER; k++) {
+        const int c = min((b0 + grp + 8 * r) * PER + k, nrec - 1);
+        x[r][k] = o[(long)c * a.c.hd];
+        v[r][k] = ml[c];
+      }
+    #pragma unroll
+    for (int r = 0; r < R; r++) {
+      Sum<1> u, p;
       u.clear();
+      #pragma unroll
+      for (int k = 0; k < PER; k++) {
+        p.m = v[r][k].x;
+        p.l = v[r][k].y;
+        p.o[0] = x[r][k];
+        if ((b0 + grp + 8 * r) * PER + k < nrec) u.fold(p);
+      }
+      po[grp + 8 * r][fl] = u.o[0];
+      if (fl == 0) pml[grp + 8 * r] = make_float2(u.m, u.l);
     }
+    __syncthreads();
+    if (grp == 0)
+      for (int i = 0; i < min(JOIN_PARTS, np - b0); i++) {
+        Sum<1> p;
+        p.m = pml[i].x;
+        p.l = pml[i].y;
+        p.o[0] = po[i][fl];
+        f.fold(p);
+      }
+    __syncthreads();
   }
-  #pragma unroll
-  for (int i = 0; i < NB; i++) emit<TYPE>(a, s, tok, head, 32 * i + fl, f.o[i] / f.l);
+  if (grp == 0) emit<TYPE>(a, s, tok, head, dim, f.o[0] / f.l);
 }
 
-// Many rows: a wave takes a tile of 16 rows through the spans of one part, a block four tiles; the parts' records are joined.
-template <int NB, int TYPE>
-__global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int tiles4) {
+// Many rows: a block takes four waves of RT tiles of 16 rows each through the spans of one part. The waves unpack a span's
+// codes to f16 operands in LDS, a quarter each, and read all of them, so that a span is unpacked once for 64 RT rows; the
+// next span's words are on their way meanwhile, and two buffers let the block meet once per span. A wave folds its rows'
+// spans, chunks and part in registers; the parts' records are joined.
+template <int NB>
+struct SpanOperands {
+  h8 k[2][2 * NB][64], v[2][2 * NB][64];  // [record][word][lane]
+  u4 ks[2][4 * NB], vs[2][4 * NB];        // the records' scales as they are
+};
+template <int NB, int TYPE, int RT>
+__global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) {
+  constexpr int HD = 32 * NB, REC = 36 * HD, NW = 2 * NB / 4;  // NW: 16-byte loads of a lane per wave (of 8 per record pair and NB / 2)
   constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  const Tile tl(a, blockIdx.z, blockIdx.y / tiles4, (blockIdx.y % tiles4 * 4 + wave) * 16);
-  int tok, head;
-  const int last = tl.last(a, n, &tok, &head);
-  const int most = wave_max(last), part = blockIdx.x;
-  if (part == 0 && (last == ROW_NONE || last == ROW_BAD))
-    for (int j = 0; j < 2 * NB; j++)
-      for (int v = 0; v < 4; v++) emit<TYPE>(a, tl.s, tok, head, 16 * j + 4 * g + v, last == ROW_NONE ? 0.0f : NAN);
-  if (most < part * PART) return;
-  typedef typename ValueOf<TYPE>::t T;
-  Queries<NB> q;
-  load_queries<NB, TYPE>(q, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.scale, lane);
-  Sum<8 * NB> f, u, r;
-  f.clear();
-  for (int c = part * CHUNKS; c < (part + 1) * CHUNKS && c * CHUNK <= most; c++) {
-    u.clear();
-    for (int p0 = c * CHUNK; p0 < (c + 1) * CHUNK && p0 <= most; p0 += SPAN) {
-      const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, p0 / KV4_GROUP);
-      const int lim = last - p0;
-      span_sum<NB, LOQ, LOW>(r, rec, q, lim, lane);
-      u.fold(r);
-    }
-    f.fold(u);
+  extern __shared__ __align__(16) uint8_t lds_raw[];
+  SpanOperands<NB> *buf = (SpanOperands<NB> *)lds_raw;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4, part = blockIdx.x;
+  const int row0 = blockIdx.y % blocks * (64 * RT) + wave * (16 * RT);
+  int last[RT], tok[RT], head[RT], most = ROW_ABSENT, blockmost;
+  const Tile tl(a, blockIdx.z, blockIdx.y / blocks, 0);
+  #pragma unroll
+  for (int r = 0; r < RT; r++) {
+    last[r] = tl.last(a, row0 + 16 * r + n, &tok[r], &head[r]);
+    most = max(most, wave_max(last[r]));
+    if (part == 0 && (last[r] == ROW_NONE || last[r] == ROW_BAD))
+      for (int j = 0; j < 2 * NB; j++)
+        for (int v = 0; v < 4; v++) emit<TYPE>(a, tl.s, tok[r], head[r], 16 * j + 4 * g + v, last[r] == ROW_NONE ? 0.0f : NAN);
   }
-  if (last < part * PART) return;
-  if (last < PART) {
+  {
+    int *red = (int *)lds_raw;
+    if (lane == 0) red[wave] = most;
+    __syncthreads();
+    blockmost = max(max(red[0], red[1]), max(red[2], red[3]));
+    __syncthreads();
+  }
+  if (blockmost < part * PART) return;
+  typedef typename ValueOf<TYPE>::t T;
+  uint32_t k1024 = 0x64006400u;
+  __asm__("" : "+v"(k1024));
+  // the wave's quarter of a span: records' key words then value words, NW 16-byte loads (of NB / 2 per record and kind)
+  const int npos = min(blockmost + 1, (part + 1) * PART), nspan = (npos - part * PART + SPAN - 1) / SPAN;
+  const uint8_t *base = record_of(a.c, tl.slot, tl.kvh, (long)part * (PART / KV4_GROUP));
+  u4 words[NW], scales;
+  auto load = [&](int sp) {
+    const uint8_t *rec = base + (long)sp * (2 * REC);
     #pragma unroll
-    for (int j = 0; j < 2 * NB; j++)
+    for (int x = 0; x < NW; x++) {
+      const int idx = wave * NW + x, i = idx / NB, kv = idx / (NB / 2) & 1, j = idx % (NB / 2);
+      words[x] = ((const u4 *)(rec + i * REC + kv * 16 * HD))[j * 64 + lane];
+    }
+    // 16 NB pieces of scales: [record][keys | values][4 NB]
+    const int e = tid, i = e / (8 * NB), r = e % (8 * NB);
+    if (e < 16 * NB) scales = ((const u4 *)(rec + i * REC + 32 * HD))[r];
+  };
+  auto stage = [&](SpanOperands<NB> &d) {
+    #pragma unroll
+    for (int x = 0; x < NW; x++) {
+      const int idx = wave * NW + x, i = idx / NB, kv = idx / (NB / 2) & 1, j = idx % (NB / 2);
       #pragma unroll
-      for (int v = 0; v < 4; v++) emit<TYPE>(a, tl.s, tok, head, 16 * j + 4 * g + v, f.o[4 * j + v] / f.l);
-  } else {
-    const long row = row_index(a, tl.s, tok, head);
-    float *o = record_o(a, row, part);
-    #pragma unroll
-    for (int j = 0; j < 2 * NB; j++) *(float4 *)(o + 16 * j + 4 * g) = make_float4(f.o[4 * j], f.o[4 * j + 1], f.o[4 * j + 2], f.o[4 * j + 3]);
-    if (g == 0) *record_ml(a, row, part) = make_float2(f.m, f.l);
+      for (int y = 0; y < 4; y++) (kv ? d.v : d.k)[i][4 * j + y][lane] = unpack8(words[x][y], k1024);
+    }
+    const int e = tid, i = e / (8 * NB), r = e % (8 * NB);
+    if (e < 16 * NB) (r < 4 * NB ? d.ks : d.vs)[i][r % (4 * NB)] = scales;
+  };
+  load(0);
+  Queries<NB> q[RT];
+  #pragma unroll
+  for (int r = 0; r < RT; r++)
+    load_queries<NB, TYPE>(q[r], (const T *)a.q.p + tl.s * a.q.seq + (last[r] >= 0 ? tok[r] * a.q.tok + head[r] * a.q.head : 0), a.scale, lane);
+  Sum<8 * NB> f[RT], u[RT];
+  #pragma unroll
+  for (int r = 0; r < RT; r++) f[r].clear(), u[r].clear();
+  stage(buf[0]);
+  load(min(1, nspan - 1));
+  __syncthreads();
+  for (int sp = 0; sp < nspan; sp++) {
+    const SpanOperands<NB> &d = buf[sp & 1];
+    const int p0 = part * PART + sp * SPAN;
+    if (p0 <= most) {
+      f4 s[RT][2][2];
+      #pragma unroll
+      for (int i = 0; i < 2; i++) {
+        u4 ks[NB];
+        #pragma unroll
+        for (int j = 0; j < NB; j++) ks[j] = d.ks[i][g * NB + j];
+        #pragma unroll
+        for (int t = 0; t < 2; t++) {
+          h8 k[NB];
+          #pragma unroll
+          for (int b = 0; b < NB; b++) k[b] = d.k[i][t * NB + b][lane];
+          #pragma unroll
+          for (int r = 0; r < RT; r++) s[r][i][t] = tile_scores<NB, LOQ>([&](int b) { return k[b]; }, ks, t, q[r]);
+        }
+      }
+      Sum<8 * NB> z[RT];
+      bool masked[RT];
+      #pragma unroll
+      for (int r = 0; r < RT; r++) {
+        masked[r] = __ballot(last[r] - p0 < SPAN - 1) != 0;
+        if (masked[r]) mask_scores(s[r], last[r] - p0, g);
+        span_softmax(s[r], q[r].c, z[r].m, z[r].l);
+      }
+      f4 o[RT][2 * NB];
+      #pragma unroll
+      for (int r = 0; r < RT; r++)
+        #pragma unroll
+        for (int j = 0; j < 2 * NB; j++) o[r][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      #pragma unroll
+      for (int i = 0; i < 2; i++) {
+        u4 vs[NB];
+        #pragma unroll
+        for (int j = 0; j < NB; j++) vs[j] = d.vs[i][g * NB + j];
+        #pragma unroll
+        for (int b = 0; b < NB; b++) {
+          const h8 x0 = d.v[i][2 * b][lane], x1 = d.v[i][2 * b + 1][lane];
+          #pragma unroll
+          for (int r = 0; r < RT; r++) {
+            h8 hi, lo;
+            weigh<NB, LOW>(s[r], vs, i, b, masked[r], last[r] - p0, g, hi, lo);
+            o[r][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, hi, o[r][2 * b], 0, 0, 0);
+            o[r][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, hi, o[r][2 * b + 1], 0, 0, 0);
+            if (LOW) {
+              o[r][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, lo, o[r][2 * b], 0, 0, 0);
+              o[r][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, lo, o[r][2 * b + 1], 0, 0, 0);
+            }
+          }
+        }
+      }
+      #pragma unroll
+      for (int r = 0; r < RT; r++) {
+        #pragma unroll
+        for (int j = 0; j < 2 * NB; j++)
+          #pragma unroll
+          for (int v = 0; v < 4; v++) z[r].o[4 * j + v] = o[r][j][v];
+        u[r].fold(z[r]);
+      }
+    }
+    if ((sp & (SPANS - 1)) == SPANS - 1 || sp == nspan - 1) {
+      #pragma unroll
+      for (int r = 0; r < RT; r++) {
+        f[r].fold(u[r]);
+        u[r].clear();
+      }
+    }
+    if (sp + 1 < nspan) {
+      stage(buf[(sp + 1) & 1]);
+      load(min(sp + 2, nspan - 1));
+    }
+    __syncthreads();
+  }
+  #pragma unroll
+  for (int r = 0; r < RT; r++) {
+    if (last[r] < part * PART) continue;
+    if (last[r] < PART) {
+      #pragma unroll
+      for (int j = 0; j < 2 * NB; j++)
+        #pragma unroll
+        for (int v = 0; v < 4; v++) emit<TYPE>(a, tl.s, tok[r], head[r], 16 * j + 4 * g + v, f[r].o[4 * j + v] / f[r].l);
+    } else {
+      const long row = row_index(a, tl.s, tok[r], head[r]);
+      float *o = record_o(a, row, part);
+      #pragma unroll
+      for (int j = 0; j < 2 * NB; j++) *(float4 *)(o + 16 * j + 4 * g) = make_float4(f[r].o[4 * j], f[r].o[4 * j + 1], f[r].o[4 * j + 2], f[r].o[4 * j + 3]);
+      if (g == 0) *record_ml(a, row, part) = make_float2(f[r].m, f[r].l);
+    }
   }
 }
 
@@ -561,24 +745,30 @@ long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead) {
   return std::max(16L, rows * rec * (c.hd + 2) * 4);
 }
 
+constexpr int parts_tiles(int nb) { return nb <= 4 ? 2 : 1; }  // RT: row tiles per wave (heads of 256: registers for one)
+
 template <int NB, int TYPE>
 static void launch_attention_k(Kv4Attn a, hipStream_t st) {
   const bool many = many_rows(a.c, a.b.nseq, a.b.ntok, a.nhead);
-  const int group = a.nhead / a.c.nkv, reclen = many ? PART : CHUNK;
+  const int group = a.nhead / a.c.nkv;
   a.nrec = record_count(a.c, many);
   const long rows = (long)a.b.ntok * group;
   if (many) {
-    const long t4 = (rows + 63) / 64;
-    hipLaunchKernelGGL((k_kv4_parts<NB, TYPE>), dim3(a.nrec, (unsigned)(t4 * a.c.nkv), a.b.nseq), dim3(256), 0, st, a, (int)t4);
+    constexpr int RT = parts_tiles(NB);
+    const long nb = (rows + 64 * RT - 1) / (64 * RT);
+    hipLaunchKernelGGL((k_kv4_parts<NB, TYPE, RT>), dim3(a.nrec, (unsigned)(nb * a.c.nkv), a.b.nseq), dim3(256), 2 * sizeof(SpanOperands<NB>), st, a, (int)nb);
   } else {
-    const int tiles = (int)((rows + 15) / 16);
-    const size_t lds = (SPANS * std::min(16L, rows) * (32 * NB + 4) + SPANS * 16 * 2) * 4;
-    hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3(a.nrec, tiles * a.c.nkv, a.b.nseq), dim3(64 * SPANS), lds, st, a, tiles);
+    // as many blocks as stay resident (one per CU, two of heads of 64), each with an even share of the chunks
+    const int tiles = (int)((rows + 15) / 16), slots = NB <= 2 ? 512 : 256;
+    const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (a.nrec * y + slots - 1) / slots;
+    const int gx = (int)((a.nrec + rounds - 1) / rounds);
+    hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3(gx, tiles * a.c.nkv, a.b.nseq), dim3(64 * SPANS), chunk_lds<NB>((int)std::min(16L, rows)), st, a, tiles);
   }
   ZL_HIP(hipGetLastError());
   if (a.nrec > 1) {
-    const long n = rows * a.c.nkv * a.b.nseq;
-    hipLaunchKernelGGL((k_kv4_join<NB, TYPE>), dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, a, reclen, reclen);
+    const dim3 grid((unsigned)(rows * a.c.nkv * a.b.nseq), NB);
+    if (many) hipLaunchKernelGGL((k_kv4_join<1, TYPE>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_kv4_join<CHUNKS, TYPE>), grid, dim3(256), 0, st, a);
     ZL_HIP(hipGetLastError());
   }
 }
@@ -586,8 +776,8 @@ static void launch_attention_k(Kv4Attn a, hipStream_t st) {
 // Dynamic LDS above 64 KB is requested per kernel, once per GPU, when a cache is created: no launch changes an attribute.
 template <int NB, int TYPE>
 static void prepare_k() {
-  const int lds = (SPANS * 16 * (32 * NB + 4) + SPANS * 16 * 2) * 4;
-  ZL_HIP(hipFuncSetAttribute((const void *)k_kv4_chunks<NB, TYPE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  ZL_HIP(hipFuncSetAttribute((const void *)k_kv4_chunks<NB, TYPE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_lds<NB>(16)));
+  ZL_HIP(hipFuncSetAttribute((const void *)k_kv4_parts<NB, TYPE, parts_tiles(NB)>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * sizeof(SpanOperands<NB>))));
 }
 template <int NB>
 static void prepare_nb() {
