@@ -1,81 +1,305 @@
-// Log probabilities of logits rows.
+// Log probabilities of logits rows: the log-sum-exp, the entropy and the top alternatives in one pass over the logits.
+//
+// With m the largest logit seen so far, l = sum e^(x - m) and e = sum e^(x - m) (x - m): a larger m' scales l by f = e^(m - m')
+// and takes e to f (e + l (m - m')). Then lse = m + ln l and the entropy is ln l - e / l: differences from the maximum all
+// along, so that nothing cancels. -inf counts for nothing; NaN and +inf make l NaN, and with it every float output.
+//
+// Alternatives are 64-bit numbers, the ordered value above the complement of the id, so that a larger one is a better one
+// and equal values go to the lowest id. Every wave keeps a list of candidates in LDS with a threshold that the n_top-th
+// best so far has reached: a lane whose 16 logits hold nothing at the threshold costs one comparison. The first threshold is
+// the n_top-th largest of the lanes' maxima. Full lists are cut to their n_top best (a search for the n_top-th largest
+// number, bit by bit with ballots).
+//
+// Bound by HBM (each logit is read once) for many rows, by the latency of two launches for few.
 #include "zl_ops.h"
+#include <algorithm>
 
 namespace zl {
 
-// Order of the alternatives: larger value first, lower id first among equals, NaN below all, as one number.
-__device__ __forceinline__ unsigned long long rank_key(float x, int id) {
-  return ((unsigned long long)(x != x ? 0u : fkey(x)) << 32) | (uint32_t)~id;
+typedef unsigned long long rank_t;
+__device__ __forceinline__ rank_t rank_key(float x, int id) {
+  return ((rank_t)(x != x ? 0u : fkey(x)) << 32) | (uint32_t)~id;
+}
+__device__ __forceinline__ float rank_value(rank_t k) { return keyf((uint32_t)(k >> 32)); }
+
+struct RowSum {
+  float m = -INFINITY, l = 0.0f, e = 0.0f;
+  __device__ __forceinline__ void raise(float to) {  // to >= m, above -inf
+    if (m == -INFINITY) { m = to; return; }
+    const float d = m - to, f = __builtin_amdgcn_exp2f(d * 1.44269504f);
+    e = d == -INFINITY ? 0.0f : f * fmaf(l, d, e);
+    l *= f;
+    m = to;
+  }
+  __device__ __forceinline__ void add(const RowSum &o) {
+    RowSum p = o;
+    const float M = fmaxf(m, p.m);
+    if (M > -INFINITY) {
+      raise(M);
+      p.raise(M);
+    }
+    l += p.l;
+    e += p.e;
+  }
+  __device__ __forceinline__ void join_wave() {
+    const float M = group_fmax(m, 64);
+    if (M > -INFINITY) raise(M);
+    l = wave_sum_xor(l, 64);
+    e = wave_sum_xor(e, 64);
+  }
+};
+
+constexpr int LP_CAP = 256;      // candidates of a wave
+constexpr int LP_TILE = 4096;    // logits of a block at a time: 16 per lane
+
+// A wave's candidate list: n entries in LDS, the threshold t (an entry must be larger), k wanted.
+struct Candidates {
+  rank_t *buf;
+  int n, k;
+  rank_t t;
+  // The first threshold: the k-th largest of the lanes' largest values kx (0: a lane that has none).
+  __device__ __forceinline__ void start(uint32_t kx) {
+    uint32_t kth = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+      const int cnt = __popcll(__ballot(kx >= (kth | (1u << bit))));
+      if (cnt >= k) kth |= 1u << bit;
+      if (cnt == k) break;
+    }
+    t = kth ? ((rank_t)kth << 32) - 1 : 0;
+  }
+  // Cut to the k largest (n > k). Entries are distinct, none is 0.
+  template <int N>
+  __device__ __forceinline__ void cut_n(int lane) {
+    rank_t x[N];
+    #pragma unroll
+    for (int i = 0; i < N; i++) x[i] = lane + 64 * i < n ? buf[lane + 64 * i] : 0;
+    rank_t v = 0;
+    for (int bit = 63; bit >= 0; bit--) {
+      const rank_t c = v | (1ull << bit);
+      int cnt = 0;
+      #pragma unroll
+      for (int i = 0; i < N; i++) cnt += __popcll(__ballot(x[i] >= c));
+      if (cnt >= k) v = c;
+      if (cnt == k) break;
+    }
+    int at = 0;
+    rank_t mn = ~0ull;  // the k-th largest itself: the smallest that is kept
+    #pragma unroll
+    for (int i = 0; i < N; i++) {
+      const bool keep = x[i] >= v && x[i] != 0;
+      const unsigned long long b = __ballot(keep);
+      if (keep) buf[at + __popcll(b & ((1ull << lane) - 1))] = x[i];
+      if (keep && x[i] < mn) mn = x[i];
+      at += __popcll(b);
+    }
+    n = at;
+    t = group_reduce(mn, 64, [](rank_t a, rank_t b) { return a < b ? a : b; });
+  }
+  __device__ __forceinline__ void cut(int lane) {
+    if (n <= 64) cut_n<1>(lane);
+    else cut_n<LP_CAP / 64>(lane);
+  }
+  __device__ __forceinline__ void offer(bool have, rank_t x, int lane) {  // by all lanes of the wave
+    const bool take = have && x > t;
+    const unsigned long long b = __ballot(take);
+    if (!b) return;
+    if (take) buf[n + __popcll(b & ((1ull << lane) - 1))] = x;
+    n += __popcll(b);
+    if (n > LP_CAP - 64) cut(lane);
+  }
+};
+
+// The k best of the four waves' lists, in wave 0's list, by the whole block.
+__device__ __forceinline__ void merge_waves(Candidates &c, rank_t (*lists)[LP_CAP], int *counts, int lane, int wave) {
+  if (c.n > (wave == 0 ? c.k : 64)) c.cut(lane);  // (wave 0 for its threshold, the others to fit one offer)
+  if (lane == 0) counts[wave] = c.n;
+  __syncthreads();
+  if (wave == 0) {
+    for (int w = 1; w < 4; w++) c.offer(lane < counts[w], lists[w][min(lane, LP_CAP - 1)], lane);
+    if (c.n > c.k) c.cut(lane);
+  }
 }
 
-// One block per row, a pass over the row for the maximum, one for the sums and one for each alternative.
+// Outputs of a row, by one wave: its sums and its k best.
 template <int TYPE>
-__global__ __launch_bounds__(256) void k_logprobs(const LogprobArgs a) {
+__device__ __forceinline__ void finish_row(const LogprobArgs &a, int row, const RowSum &s, rank_t mine, int lane) {
   typedef typename ValueOf<TYPE>::t T;
-  __shared__ float redf[4];
-  __shared__ double redd[8];
-  __shared__ unsigned long long redk[4];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const T *x = (const T *)a.x + (long)r * a.ld;
-  float m = -INFINITY;
-  bool nan = false;
-  for (int i = tid; i < a.vocab; i += 256) { const float v = load_value<TYPE>(x[i]); m = fmaxf(m, v); nan |= v != v; }
-  if (nan) m = NAN;
-  m = group_reduce(m, 64, [](float p, float q) { return p != p || q != q ? NAN : fmaxf(p, q); });
-  if (lane == 0) redf[wave] = m;
-  __syncthreads();
-  m = redf[0];
-  for (int w = 1; w < 4; w++) m = m != m || redf[w] != redf[w] ? NAN : fmaxf(m, redf[w]);
-  double l = 0, e = 0;
-  for (int i = tid; i < a.vocab; i += 256) {
-    const double d = (double)load_value<TYPE>(x[i]) - (double)m;
-    if (d == -INFINITY) continue;
-    const double p = exp(d);
-    l += p;
-    e += p * d;
-  }
-  l = wave_sum_xor(l, 64);
-  e = wave_sum_xor(e, 64);
-  if (lane == 0) { redd[wave] = l; redd[4 + wave] = e; }
-  __syncthreads();
-  l = (redd[0] + redd[1]) + (redd[2] + redd[3]);
-  e = (redd[4] + redd[5]) + (redd[6] + redd[7]);
-  const double lz = m > -INFINITY ? log(l) : NAN;
-  if (tid == 0) {
+  const T *x = (const T *)a.x + (long)row * a.ld;
+  const double lz = s.m > -INFINITY ? log((double)s.l) : NAN;
+  if (lane == 0) {
     if (a.lp) {
-      const int id = a.tokens[r];
-      a.lp[r] = id >= 0 && id < a.vocab ? (float)((double)load_value<TYPE>(x[id]) - (double)m - lz) : NAN;
+      const int id = a.tokens[row];
+      a.lp[row] = id >= 0 && id < a.vocab ? (float)((double)load_value<TYPE>(x[id]) - (double)s.m - lz) : NAN;
     }
-    if (a.ent) a.ent[r] = (float)(lz - e / l);
+    if (a.ent) a.ent[row] = (float)(lz - (double)s.e / (double)s.l);
   }
-  unsigned long long prev = ~0ull;
-  for (int k = 0; k < a.ntop; k++) {
-    unsigned long long best = 0;
-    for (int i = tid; i < a.vocab; i += 256) {
-      const unsigned long long c = rank_key(load_value<TYPE>(x[i]), i);
-      if (c < prev && c > best) best = c;
-    }
-    best = group_reduce(best, 64, [](unsigned long long p, unsigned long long q) { return p > q ? p : q; });
-    __syncthreads();
-    if (lane == 0) redk[wave] = best;
-    __syncthreads();
-    for (int w = 0; w < 4; w++) best = redk[w] > best ? redk[w] : best;
-    prev = best;
-    if (tid == 0) {
-      const int id = (int)~(uint32_t)best;
-      if (a.ids) a.ids[(long)r * a.ntop + k] = id;
-      if (a.toplp) a.toplp[(long)r * a.ntop + k] = (float)((double)load_value<TYPE>(x[id]) - (double)m - lz);
-    }
+  if (a.ntop == 0) return;
+  int place = 0;
+  for (int j = 0; j < a.ntop; j++) place += __shfl(mine, j, 64) > mine;
+  if (lane < a.ntop) {
+    const int id = (int)~(uint32_t)mine;
+    if (a.ids) a.ids[(long)row * a.ntop + place] = id;
+    if (a.toplp) a.toplp[(long)row * a.ntop + place] = (float)((double)rank_value(mine) - (double)s.m - lz);
   }
 }
 
-long logprobs_work(int rows, int vocab, int ntop) { return 16; }
+// Work space: the parts' sums [row][part], then their candidates [row][part][ntop].
+__device__ __forceinline__ float4 *part_sum(const LogprobArgs &a, int parts, long row) { return (float4 *)a.work + row * parts; }
+__device__ __forceinline__ rank_t *part_top(const LogprobArgs &a, int parts, long row) {
+  return (rank_t *)((float4 *)a.work + (long)a.rows * parts) + row * parts * a.ntop;
+}
 
-void launch_logprobs(const LogprobArgs &a, int type, hipStream_t st) {
-  if (type == T_F32) hipLaunchKernelGGL((k_logprobs<T_F32>), dim3(a.rows), dim3(256), 0, st, a);
-  else if (type == T_F16) hipLaunchKernelGGL((k_logprobs<T_F16>), dim3(a.rows), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_logprobs<T_BF16>), dim3(a.rows), dim3(256), 0, st, a);
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_logprobs(const LogprobArgs a, int parts, int span) {
+  typedef typename ValueOf<TYPE>::t T;
+  constexpr int VE = 16 / sizeof(T), NV = 16 / VE;  // values per 16-byte load, loads per lane
+  typedef T vec __attribute__((ext_vector_type(VE)));
+  __shared__ rank_t lists[4][LP_CAP];
+  __shared__ float sums[4][3];
+  __shared__ int counts[4];
+  const int row = blockIdx.x / parts, part = blockIdx.x - row * parts, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const T *x = (const T *)a.x + (long)row * a.ld;
+  const int off = (int)(((uintptr_t)x % 16) / sizeof(T));  // indexes count from the 16-byte boundary at or before the row
+  const T *base = x - off;
+  const int i0 = part * span, i1 = min(a.vocab + off, i0 + span);
+  RowSum s;
+  Candidates c{lists[wave], 0, a.ntop, 0};
+  bool first = true;
+  for (int t0 = i0; t0 < i1; t0 += LP_TILE) {
+    float v[16];
+    #pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = t0 + (j * 256 + tid) * VE;
+      if (i >= off && i + VE <= a.vocab + off && i + VE <= i1) {
+        const vec u = *(const vec *)(base + i);
+        #pragma unroll
+        for (int e = 0; e < VE; e++) v[j * VE + e] = load_value<TYPE>(u[e]);
+      } else {
+        #pragma unroll
+        for (int e = 0; e < VE; e++) v[j * VE + e] = i + e >= off && i + e < i1 ? load_value<TYPE>(base[i + e]) : -INFINITY;
+      }
+    }
+    float mx = v[0];
+    #pragma unroll
+    for (int e = 1; e < 16; e++) mx = fmaxf(mx, v[e]);
+    if (mx > s.m) s.raise(mx);
+    const float ref = s.m == -INFINITY ? 0.0f : s.m;
+    #pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const float d = v[e] - ref, p = __builtin_amdgcn_exp2f(d * 1.44269504f);
+      s.l += p;
+      s.e = fmaf(p, fmaxf(d, -3.0e38f), s.e);
+    }
+    if (a.ntop) {
+      if (first) {
+        // at least ntop logits are at or above the ntop-th largest of the lanes' maxima (0: a lane with none but NaN)
+        uint32_t kx = 0;
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+          #pragma unroll
+          for (int e = 0; e < VE; e++) {
+            const int i = t0 + (j * 256 + tid) * VE + e;
+            if (i >= off && i < i1 && v[j * VE + e] == v[j * VE + e]) kx = max(kx, fkey(v[j * VE + e]));
+          }
+        c.start(kx);
+        first = false;
+      }
+      const uint32_t tv = (uint32_t)(c.t >> 32);
+      const float tf = tv ? keyf(tv) : NAN;  // (NaN: every logit is offered)
+      if (__ballot(!(mx < tf))) {
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+          #pragma unroll
+          for (int e = 0; e < VE; e++) {
+            if (!__ballot(!(v[j * VE + e] < tf))) continue;
+            const int i = t0 + (j * 256 + tid) * VE + e;
+            c.offer(i >= off && i < i1, rank_key(v[j * VE + e], i - off), lane);
+          }
+      }
+    }
+  }
+  s.join_wave();
+  if (lane == 0) { sums[wave][0] = s.m; sums[wave][1] = s.l; sums[wave][2] = s.e; }
+  if (a.ntop) merge_waves(c, lists, counts, lane, wave);
+  else __syncthreads();
+  if (wave) return;
+  for (int w = 1; w < 4; w++) {
+    RowSum o;
+    o.m = sums[w][0];
+    o.l = sums[w][1];
+    o.e = sums[w][2];
+    s.add(o);
+  }
+  const rank_t mine = lane < c.n ? lists[0][lane] : 0;
+  if (parts == 1) {
+    finish_row<TYPE>(a, row, s, mine, lane);
+    return;
+  }
+  if (lane == 0) part_sum(a, parts, row)[part] = make_float4(s.m, s.l, s.e, 0.0f);
+  if (lane < a.ntop) part_top(a, parts, row)[part * a.ntop + lane] = mine;
+}
+
+// The parts of a row.
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_logprobs_join(const LogprobArgs a, int parts) {
+  __shared__ rank_t lists[4][LP_CAP];
+  __shared__ int counts[4];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Candidates c{lists[wave], 0, a.ntop, 0};
+  if (a.ntop) {
+    const rank_t *top = part_top(a, parts, row);
+    const int total = parts * a.ntop;
+    for (int i0 = 0; i0 < total; i0 += 1024) {
+      rank_t x[4];
+      #pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = i0 + 256 * j + tid < total ? top[i0 + 256 * j + tid] : 0;
+      if (i0 == 0) c.start(max(max((uint32_t)(x[0] >> 32), (uint32_t)(x[1] >> 32)), max((uint32_t)(x[2] >> 32), (uint32_t)(x[3] >> 32))));
+      #pragma unroll
+      for (int j = 0; j < 4; j++) c.offer(x[j] != 0, x[j], lane);
+    }
+    merge_waves(c, lists, counts, lane, wave);
+  }
+  if (wave) return;
+  RowSum s;
+  for (int p = lane; p < parts; p += 64) {
+    const float4 v = part_sum(a, parts, row)[p];
+    RowSum o;
+    o.m = v.x;
+    o.l = v.y;
+    o.e = v.z;
+    s.add(o);
+  }
+  s.join_wave();
+  finish_row<TYPE>(a, row, s, lane < c.n ? lists[0][lane] : 0, lane);
+}
+
+// Parts of a row: blocks of whole tiles, about a thousand blocks in all where the rows alone are fewer (four of a CU's size, to
+// have loads of many waves in flight), one block per row beyond.
+static int lp_span(int rows, int vocab) {
+  const long tiles = (vocab + 7 + LP_TILE - 1) / LP_TILE;  // (a row may start up to 7 values behind a 16-byte boundary)
+  return (int)std::max(1L, std::min(tiles, (tiles * rows + 512) / 1024)) * LP_TILE;
+}
+static int lp_parts(int rows, int vocab) { return (vocab + 7 + lp_span(rows, vocab) - 1) / lp_span(rows, vocab); }
+
+long logprobs_work(int rows, int vocab, int ntop) {
+  const long parts = lp_parts(std::max(rows, 1), vocab);
+  return std::max(16L, parts == 1 ? 0L : rows * parts * (16 + 8L * ntop));
+}
+
+template <int TYPE>
+static void launch_logprobs_t(const LogprobArgs &a, hipStream_t st) {
+  const int span = lp_span(a.rows, a.vocab), parts = lp_parts(a.rows, a.vocab);
+  hipLaunchKernelGGL((k_logprobs<TYPE>), dim3((unsigned)((long)a.rows * parts)), dim3(256), 0, st, a, parts, span);
   ZL_HIP(hipGetLastError());
+  if (parts > 1) {
+    hipLaunchKernelGGL((k_logprobs_join<TYPE>), dim3(a.rows), dim3(256), 0, st, a, parts);
+    ZL_HIP(hipGetLastError());
+  }
+}
+void launch_logprobs(const LogprobArgs &a, int type, hipStream_t st) {
+  if (type == T_F32) launch_logprobs_t<T_F32>(a, st);
+  else if (type == T_F16) launch_logprobs_t<T_F16>(a, st);
+  else launch_logprobs_t<T_BF16>(a, st);
 }
 
 }  // namespace zl

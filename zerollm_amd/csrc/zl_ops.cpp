@@ -57,7 +57,7 @@ static OpRows take_rows(const char *f, const zl_rows *r, int type) {
 }
 
 static void check_logprobs(int rows, int vocab, int n_top) {
-  ZL_REQUIRE(rows >= 0 && vocab >= 1, ZL_ERR_ARG, "logprobs: bad row count or vocabulary");
+  ZL_REQUIRE(rows >= 0 && rows <= (1 << 30) && vocab >= 1 && vocab <= (1 << 30), ZL_ERR_ARG, "logprobs: bad row count or vocabulary");
   ZL_REQUIRE(n_top >= 0 && n_top <= LOGPROB_MAX_TOP && n_top <= vocab, ZL_ERR_ARG,
              "logprobs: n_top must be 0 to " + std::to_string(LOGPROB_MAX_TOP) + " and at most the vocabulary (got " + std::to_string(n_top) + ")");
 }

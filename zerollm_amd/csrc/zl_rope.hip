@@ -1,5 +1,6 @@
 // Rotary positions: queries and keys of a batch rotated in one launch.
 #include "zl_ops.h"
+#include <algorithm>
 
 namespace zl {
 
@@ -16,47 +17,113 @@ __device__ __forceinline__ void turn_sincos(double t, float *c, float *s) {
   *s = k >= 2 ? -b : b;
 }
 
-// One block per (token, sequence): the pairs' cos and sin once, then every head.
-template <int TYPE>
-__global__ __launch_bounds__(256) void k_rope(const RopeArgs a) {
+template <class T, int W> struct Piece { typedef T t __attribute__((ext_vector_type(W))); };
+
+// A block takes `tb` tokens of a sequence and a share of their heads (blockIdx.z): the tokens' cos and sin go to LDS once, then
+// every lane takes pieces of W values: W pairs' firsts and seconds from the two halves, W / 2 neighbouring pairs, or W values
+// that pass through. W > 1 (16 bytes) where every row starts on a 16-byte boundary and the parts of a head do. Bound by HBM: each
+// value is read and written once.
+template <int TYPE, int W, bool HALF>
+__global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) {
   typedef typename ValueOf<TYPE>::t T;
-  __shared__ float cs[128], sn[128];
-  const int t = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
-  if (t >= (a.b.count ? max(0, min(a.b.count[s], a.b.ntok)) : a.b.ntok)) return;
-  const double pos = (double)a.b.pos[s] + t;
-  if (tid < a.half) {
+  typedef typename Piece<T, W>::t vec;
+  extern __shared__ float2 cs[];  // [tokens][half]
+  const int s = blockIdx.y, tid = threadIdx.x, t0 = blockIdx.x * tb, half = a.half, nrot = 2 * half;
+  const int nt = min(tb, (a.b.count ? max(0, min(a.b.count[s], a.b.ntok)) : a.b.ntok) - t0);
+  if (nt <= 0) return;
+  const int p0 = a.b.pos[s];
+  for (int i = tid; i < nt * half; i += 256) {
+    const int t = i / half, r = i - t * half;
     float c, n;
-    turn_sincos(pos * a.turns[tid], &c, &n);
-    cs[tid] = c * a.gain;
-    sn[tid] = n * a.gain;
+    turn_sincos(((double)p0 + (t0 + t)) * a.turns[r], &c, &n);
+    cs[i] = make_float2(c * a.gain, n * a.gain);
   }
   __syncthreads();
-  const int nrot = 2 * a.half, items = a.half + (a.hd - nrot);  // pairs, then the values that pass through
-  for (int i = tid; i < (a.nq + a.nk) * items; i += 256) {
-    const int h = i / items, r = i - h * items;
+  constexpr int PW = HALF || W > 1 ? W : 2;  // values of a neighbouring-pairs piece
+  const int rp = HALF ? half / W : nrot / PW, items = rp + (a.hd - nrot) / W;  // pieces of a head: rotated, then passed through
+  const int h0 = blockIdx.z * hb, nh = min(hb, a.nq + a.nk - h0), total = nt * nh * items;
+  for (int i = tid; i < total; i += 256) {
+    const int row = i / items, r = i - row * items, t = row / nh, h = h0 + row - t * nh;
     const bool isq = h < a.nq;
     const OpRows &x = isq ? a.q : a.k, &y = isq ? a.qo : a.ko;
-    const int hh = isq ? h : h - a.nq;
-    const T *xp = (const T *)x.p + s * x.seq + t * x.tok + hh * x.head;
-    T *yp = (T *)y.p + s * y.seq + t * y.tok + hh * y.head;
-    if (r >= a.half) {
-      const int d = nrot + r - a.half;
-      yp[d] = xp[d];
+    const long hh = isq ? h : h - a.nq;
+    const T *xp = (const T *)x.p + s * x.seq + (t0 + t) * x.tok + hh * x.head;
+    T *yp = (T *)y.p + s * y.seq + (t0 + t) * y.tok + hh * y.head;
+    if (r >= rp) {
+      const int d = nrot + (r - rp) * W;
+      *(vec *)(yp + d) = *(const vec *)(xp + d);
       continue;
     }
-    const int i0 = a.neox ? r : 2 * r, i1 = a.neox ? r + a.half : 2 * r + 1;
-    const float x0 = load_value<TYPE>(xp[i0]), x1 = load_value<TYPE>(xp[i1]), c = cs[r], n = sn[r];
-    yp[i0] = store_value<TYPE>(fmaf(x0, c, -(x1 * n)));
-    yp[i1] = store_value<TYPE>(fmaf(x0, n, x1 * c));
+    const float2 *f = cs + t * half;
+    if constexpr (HALF) {
+      const int d = r * W;
+      const vec u = *(const vec *)(xp + d), v = *(const vec *)(xp + d + half);
+      vec w, z;
+      #pragma unroll
+      for (int e = 0; e < W; e++) {
+        const float x0 = load_value<TYPE>(u[e]), x1 = load_value<TYPE>(v[e]);
+        const float2 g = f[d + e];
+        w[e] = store_value<TYPE>(fmaf(x0, g.x, -(x1 * g.y)));
+        z[e] = store_value<TYPE>(fmaf(x0, g.y, x1 * g.x));
+      }
+      *(vec *)(yp + d) = w;
+      *(vec *)(yp + d + half) = z;
+    } else if constexpr (W > 1) {
+      const int d = r * W;
+      const vec u = *(const vec *)(xp + d);
+      vec w;
+      #pragma unroll
+      for (int e = 0; e < W; e += 2) {
+        const float x0 = load_value<TYPE>(u[e]), x1 = load_value<TYPE>(u[e + 1]);
+        const float2 g = f[(d + e) >> 1];
+        w[e] = store_value<TYPE>(fmaf(x0, g.x, -(x1 * g.y)));
+        w[e + 1] = store_value<TYPE>(fmaf(x0, g.y, x1 * g.x));
+      }
+      *(vec *)(yp + d) = w;
+    } else {
+      const float x0 = load_value<TYPE>(xp[2 * r]), x1 = load_value<TYPE>(xp[2 * r + 1]);
+      const float2 g = f[r];
+      yp[2 * r] = store_value<TYPE>(fmaf(x0, g.x, -(x1 * g.y)));
+      yp[2 * r + 1] = store_value<TYPE>(fmaf(x0, g.y, x1 * g.x));
+    }
   }
 }
 
-void launch_rope(const RopeArgs &a, int type, hipStream_t st) {
-  const dim3 grid(a.b.ntok, a.b.nseq);
-  if (type == T_F32) hipLaunchKernelGGL((k_rope<T_F32>), grid, dim3(256), 0, st, a);
-  else if (type == T_F16) hipLaunchKernelGGL((k_rope<T_F16>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_rope<T_BF16>), grid, dim3(256), 0, st, a);
+// Rows of 16-byte pieces: every start and stride, and the head's parts.
+static bool whole_pieces(const RopeArgs &a, int vb) {
+  const int w = 16 / vb;
+  auto ok = [&](const OpRows &r) {
+    return (uintptr_t)r.p % 16 == 0 && r.seq % w == 0 && r.tok % w == 0 && r.head % w == 0;
+  };
+  return ok(a.q) && ok(a.qo) && (!a.nk || (ok(a.k) && ok(a.ko))) && (a.neox ? a.half : 2 * a.half) % w == 0 && (a.hd - 2 * a.half) % w == 0;
+}
+
+template <int TYPE, int W>
+static void launch_rope_k(const RopeArgs &a, hipStream_t st) {
+  // Tokens and heads per block: pieces for every lane a few times over where there are many tokens, as many blocks as CUs
+  // where there are few (each of which forms its tokens' cos and sin itself: 2 half values a block).
+  const int heads = a.nq + a.nk, pieces = std::max(1, a.hd / W);
+  const long all = (long)a.b.ntok * a.b.nseq * heads * pieces;
+  const long per = std::max(256L, std::min(4096L, all / 512));  // pieces per block
+  const int hb = (int)std::max(1L, std::min((long)heads, per / pieces));
+  const int tb = (int)std::max(1L, std::min({(long)a.b.ntok, per / ((long)hb * pieces), 16L}));
+  const dim3 grid((unsigned)((a.b.ntok + tb - 1) / tb), a.b.nseq, (heads + hb - 1) / hb);
+  const size_t lds = (size_t)tb * a.half * sizeof(float2);
+  if (a.neox) hipLaunchKernelGGL((k_rope<TYPE, W, true>), grid, dim3(256), lds, st, a, tb, hb);
+  else hipLaunchKernelGGL((k_rope<TYPE, W, false>), grid, dim3(256), lds, st, a, tb, hb);
   ZL_HIP(hipGetLastError());
+}
+
+template <int TYPE>
+static void launch_rope_t(const RopeArgs &a, hipStream_t st) {
+  constexpr int W = 16 / sizeof(typename ValueOf<TYPE>::t);
+  if (whole_pieces(a, sizeof(typename ValueOf<TYPE>::t))) launch_rope_k<TYPE, W>(a, st);
+  else launch_rope_k<TYPE, 1>(a, st);
+}
+void launch_rope(const RopeArgs &a, int type, hipStream_t st) {
+  if (type == T_F32) launch_rope_t<T_F32>(a, st);
+  else if (type == T_F16) launch_rope_t<T_F16>(a, st);
+  else launch_rope_t<T_BF16>(a, st);
 }
 
 }  // namespace zl
