@@ -11,16 +11,38 @@ __device__ __forceinline__ int count_of(const OpBatch &b, int s) { return b.coun
 __device__ __forceinline__ int slot_of(const OpBatch &b, int s) { return b.slot ? b.slot[s] : s; }
 
 // ---------------------------------------------------------------------------------------------- append
-// One block per (32-position record that a sequence may touch, KV head, sequence). 32 lanes hold one block of 32 values:
-// the value of largest magnitude (the lowest index among equals) gives d = mx / -8, and code = clamp(trunc(x / d + 8.5), 0, 15)
-// with 1/d, the product and the sum each rounded in f64, as the library's Q4_0 quantiser. Key words are put together across
-// 8 lanes; value words hold 8 positions, so the block gathers its record's codes in LDS and merges them into the words,
-// whose other positions it keeps. The block of the first sequence that touches a record of a slot takes all of them, in order.
-template <int TYPE>
+// One block per (32-position record that a sequence may touch, KV head, sequence). A lane takes 8 values, four lanes a block
+// of 32: the value of largest magnitude (the lowest index among equals) gives d = mx / -8, and code = clamp(trunc(x / d + 8.5),
+// 0, 15) with 1/d, the product and the sum each rounded in f64, as the library's Q4_0 quantiser. The codes go to LDS and from
+// there in whole words: a key word is one lane's 8 values; a value word holds 8 positions, and those that are not appended
+// keep their codes. The block of the first sequence that touches a record of a slot takes all of them, in order.
+// Bound by the loads' latency: all of a record's are requested together (2048 tokens of 8 heads of 128, bf16: 37 us with a
+// value per lane and a load at a time).
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void load8(const typename ValueOf<TYPE>::t *p, float (&x)[8]) {
+  typedef typename ValueOf<TYPE>::t T;
+  constexpr int W = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(W)));
+  if constexpr (VEC) {
+    #pragma unroll
+    for (int i = 0; i < 8 / W; i++) {
+      const vec v = ((const vec *)p)[i];
+      #pragma unroll
+      for (int e = 0; e < W; e++) x[i * W + e] = load_value<TYPE>(v[e]);
+    }
+  } else {
+    #pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = load_value<TYPE>(p[e]);
+  }
+}
+
+template <int NB, int TYPE, bool VEC>
 __global__ __launch_bounds__(256) void k_kv4_append(const Kv4View c, const OpBatch b, const OpRows k, const OpRows v) {
   typedef typename ValueOf<TYPE>::t T;
-  extern __shared__ uint8_t vn[];   // [32 positions][hd] value codes
-  const int s0 = blockIdx.z, head = blockIdx.y, tid = threadIdx.x, hd = c.hd, nb = hd >> 5;
+  constexpr int HD = 32 * NB, UNITS = 32 * 4 * NB / 256;  // a lane's pieces of 8 keys (of 8 values) of a whole record
+  __shared__ uint32_t kw[4 * HD];
+  __shared__ uint64_t vn[32][HD / 8];  // value codes, a byte each
+  const int s0 = blockIdx.z, head = blockIdx.y, tid = threadIdx.x;
   const int slot = slot_of(b, s0);
   if (slot < 0 || slot >= c.nslot || count_of(b, s0) == 0) return;
   // (in 64 bits: positions near the ends of int32 must not wrap)
@@ -39,87 +61,163 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4View c, const OpBat
       if (b.slot[s] == slot && touches(s, &x, &y)) return;
     }
   uint8_t *rec = record_of(c, slot, head, g);
-  const int grp = tid >> 5, e32 = tid & 31;
   for (int s = s0; s < (b.slot ? b.nseq : s0 + 1); s++) {
     if (s != s0 && (b.slot[s] != slot || !touches(s, &p0, &p1))) continue;
     const int n = (int)(p1 - p0), q0 = (int)(p0 - g * KV4_GROUP);
     const long t0 = p0 - b.pos[s];
-    for (int u = grp; u < 2 * n * nb; u += 8) {  // (key | value, position, block)
-      const int isv = u >= n * nb, r = isv ? u - n * nb : u, i = r / nb, blk = r - i * nb, p = q0 + i;
-      const OpRows &rows = isv ? v : k;
-      const float x = load_value<TYPE>(((const T *)rows.p)[s * rows.seq + (t0 + i) * rows.tok + head * rows.head + blk * 32 + e32]);
-      const float a = fabsf(x), am = group_fmax(a, 32);
-      const int half = tid & 32;
-      const uint32_t at = (uint32_t)(__ballot(a == am) >> half);
-      const bool bad = (uint32_t)(__ballot(!(a <= 65504.0f)) >> half) != 0;
-      const float mx = __shfl(x, at ? __ffs(at) - 1 : 0, 32);
-      const double d = (double)mx / -8.0, inv = d != 0.0 ? 1.0 / d : 0.0;
-      int code = bad ? 8 : (int)((double)x * inv + 8.5);
-      code = min(15, max(0, code));
-      const uint16_t dh = bad ? (uint16_t)0x7e00 : f2h((float)d);
-      if (e32 == 0) ((uint16_t *)(rec + (isv ? 34 : 32) * hd))[kv4_scale(p, blk, nb)] = dh;
-      if (isv) vn[p * hd + blk * 32 + e32] = (uint8_t)code;
-      else {
-        const int e = e32 & 7;
-        uint32_t w = (uint32_t)code << (4 * kv4_nibble(e));
-        w |= dpp_move<0xB1>(w); w |= dpp_move<0x4E>(w); w |= dpp_move<0x141>(w);
-        if (e == 0) ((uint32_t *)rec)[kv4_word((p >> 4) * nb + blk, (p & 15) + 16 * (e32 >> 3))] = w;
+    float x[2][UNITS][8];
+    #pragma unroll
+    for (int isv = 0; isv < 2; isv++)
+      #pragma unroll
+      for (int u = 0; u < UNITS; u++) {
+        const int i = u * 256 + tid, t = i / (4 * NB), d8 = i % (4 * NB);
+        const OpRows &r = isv ? v : k;
+        if (t < n) load8<TYPE, VEC>((const T *)r.p + s * r.seq + (t0 + t) * r.tok + head * r.head + 8 * d8, x[isv][u]);
       }
-    }
+    #pragma unroll
+    for (int isv = 0; isv < 2; isv++)
+      #pragma unroll
+      for (int u = 0; u < UNITS; u++) {
+        const int i = u * 256 + tid, t = i / (4 * NB), d8 = i % (4 * NB), p = q0 + t;
+        if (t >= n) continue;  // (four lanes of a block of 32 go together)
+        const float (&y)[8] = x[isv][u];
+        float am = 0.0f;
+        uint32_t neg = 0;
+        bool bad = false;
+        #pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float m = fabsf(y[e]);
+          bad |= !(m <= 65504.0f);
+          if (m > am) { am = m; neg = __float_as_uint(y[e]) >> 31; }
+        }
+        const float all = fmaxf(fmaxf(am, dpp_move<0xB1>(am)), dpp_move<0x4E>(fmaxf(am, dpp_move<0xB1>(am))));
+        // the first lane that reached it, and its sign, as one number; bad blocks
+        uint32_t first = am == all ? 2 * (tid & 3) + neg : 8;
+        first = min(first, dpp_move<0xB1>(first));
+        first = min(first, dpp_move<0x4E>(first));
+        uint32_t nan = bad;
+        nan |= dpp_move<0xB1>(nan);
+        nan |= dpp_move<0x4E>(nan);
+        const float mx = first & 1 ? -all : all;
+        const double d = (double)mx / -8.0, inv = d != 0.0 ? 1.0 / d : 0.0;
+        uint32_t w = 0;
+        uint64_t bytes = 0;
+        #pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int code = nan ? 8 : min(15, max(0, (int)((double)y[e] * inv + 8.5)));
+          w |= (uint32_t)code << (4 * kv4_nibble(e));
+          bytes |= (uint64_t)code << (8 * e);
+        }
+        if ((tid & 3) == 0) ((uint16_t *)(rec + (isv ? 34 : 32) * HD))[kv4_scale(p, d8 >> 2, NB)] = nan ? (uint16_t)0x7e00 : f2h((float)d);
+        if (isv) vn[p][d8] = bytes;
+        else kw[kv4_word((p >> 4) * NB + (d8 >> 2), (p & 15) + 16 * (d8 & 3))] = w;
+      }
     __syncthreads();
-    uint32_t *vw = (uint32_t *)(rec + 16 * hd);
-    for (int i = tid; i < 4 * hd; i += 256) {  // words: (dimension, four positions of each tile)
-      const int dim = i % hd, gq = i / hd;
+    uint32_t *kd = (uint32_t *)rec, *vd = (uint32_t *)(rec + 16 * HD);
+    #pragma unroll
+    for (int u = 0; u < 4 * HD / 256; u++) {
+      const int i = u * 256 + tid, lane = i >> 2 & 63, w4 = (i >> 8) * 4 + (i & 3);  // dword i of the words
+      const int p = (lane & 15) + 16 * (w4 / NB);
+      if (p >= q0 && p < q0 + n) kd[i] = kw[i];
+      const int dim = 16 * w4 + (lane & 15), gq = lane >> 4;
       uint32_t w = 0, m = 0;
       #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const int p = 16 * (e >> 2) + 4 * gq + (e & 3);
-        if (p >= q0 && p < q0 + n) {
-          w |= (uint32_t)vn[p * hd + dim] << (4 * kv4_nibble(e));
+        const int q = 16 * (e >> 2) + 4 * gq + (e & 3);
+        if (q >= q0 && q < q0 + n) {
+          w |= (uint32_t)((const uint8_t *)vn[q])[dim] << (4 * kv4_nibble(e));
           m |= 0xfu << (4 * kv4_nibble(e));
         }
       }
-      if (!m) continue;
-      uint32_t *at = vw + kv4_word(dim >> 4, (dim & 15) + 16 * gq);
-      *at = m == 0xffffffffu ? w : (*at & ~m) | w;
+      if (m) vd[i] = m == 0xffffffffu ? w : (vd[i] & ~m) | w;
     }
     __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------------------------- read-back
-__device__ __forceinline__ float kv4_value(const uint8_t *rec, int hd, int isv, int p, int dim) {
-  const int nb = hd >> 5;
-  const uint32_t *w = (const uint32_t *)(rec + isv * 16 * hd);
-  const float d = h2f(((const uint16_t *)(rec + (32 + 2 * isv) * hd))[kv4_scale(p, dim >> 5, nb)]);
-  uint32_t x;
-  int e;
-  if (isv) {
-    x = w[kv4_word(dim >> 4, (dim & 15) + 16 * ((p >> 2) & 3))];
-    e = 4 * (p >> 4) + (p & 3);
-  } else {
-    x = w[kv4_word((p >> 4) * nb + (dim >> 5), (p & 15) + 16 * ((dim >> 3) & 3))];
-    e = dim & 7;
-  }
-  return d * (float)((int)((x >> (4 * kv4_nibble(e))) & 15) - 8);
-}
-
-// One block per (token, head, sequence), a thread per dimension.
-template <int TYPE>
+// One block per (32 tokens, KV head, sequence); a lane takes 8 values of a token's key, then of its value.
+template <int NB, int TYPE, bool VEC>
 __global__ __launch_bounds__(256) void k_kv4_read(const Kv4View c, const OpBatch b, const OpRows k, const OpRows v) {
   typedef typename ValueOf<TYPE>::t T;
-  const int t = blockIdx.x, head = blockIdx.y, s = blockIdx.z, dim = threadIdx.x;
-  if (t >= count_of(b, s) || dim >= c.hd) return;
-  const int slot = slot_of(b, s);
-  const long p = (long)b.pos[s] + t;
-  const bool ok = slot >= 0 && slot < c.nslot && p >= 0 && p < c.cap;
-  const uint8_t *rec = ok ? record_of(c, slot, head, p >> 5) : nullptr;
+  constexpr int HD = 32 * NB, W = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(W)));
+  const int head = blockIdx.y, s = blockIdx.z, n = count_of(b, s), slot = slot_of(b, s);
   #pragma unroll
-  for (int isv = 0; isv < 2; isv++) {
-    const OpRows &o = isv ? v : k;
-    const float x = ok ? kv4_value(rec, c.hd, isv, (int)(p & 31), dim) : NAN;
-    ((T *)o.p)[s * o.seq + t * o.tok + head * o.head + dim] = store_value<TYPE>(x);
+  for (int i = threadIdx.x; i < 32 * 4 * NB; i += 256) {
+    const int t = blockIdx.x * 32 + i / (4 * NB), d8 = i % (4 * NB);
+    if (t >= n) continue;
+    const long pos = (long)b.pos[s] + t;
+    const bool ok = slot >= 0 && slot < c.nslot && pos >= 0 && pos < c.cap;
+    const int p = (int)(pos & 31);
+    const uint8_t *rec = ok ? record_of(c, slot, head, pos >> 5) : nullptr;
+    #pragma unroll
+    for (int isv = 0; isv < 2; isv++) {
+      const OpRows &o = isv ? v : k;
+      T *out = (T *)o.p + s * o.seq + t * o.tok + head * o.head + 8 * d8;
+      T y[8];
+      #pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = store_value<TYPE>(NAN);
+      if (ok) {
+        const uint32_t *w = (const uint32_t *)(rec + isv * 16 * HD);
+        const float d = h2f(((const uint16_t *)(rec + (32 + 2 * isv) * HD))[kv4_scale(p, d8 >> 2, NB)]);
+        const uint32_t kword = isv ? 0 : w[kv4_word((p >> 4) * NB + (d8 >> 2), (p & 15) + 16 * (d8 & 3))];
+        #pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int dim = 8 * d8 + e;
+          const uint32_t x = isv ? w[kv4_word(dim >> 4, (dim & 15) + 16 * ((p >> 2) & 3))] : kword;
+          y[e] = store_value<TYPE>(d * (float)((int)((x >> (4 * kv4_nibble(isv ? 4 * (p >> 4) + (p & 3) : e))) & 15) - 8));
+        }
+      }
+      if constexpr (VEC) {
+        #pragma unroll
+        for (int j = 0; j < 8 / W; j++) {
+          vec u;
+          #pragma unroll
+          for (int e = 0; e < W; e++) u[e] = y[j * W + e];
+          ((vec *)out)[j] = u;
+        }
+      } else {
+        #pragma unroll
+        for (int e = 0; e < 8; e++) out[e] = y[e];
+      }
+    }
   }
+}
+
+// Whether every head of the rows starts on a 16-byte boundary.
+static bool whole_pieces(const OpRows &r, int type) {
+  const int w = 16 / value_bytes(type);
+  return (uintptr_t)r.p % 16 == 0 && r.seq % w == 0 && r.tok % w == 0 && r.head % w == 0;
+}
+template <int NB, int TYPE, bool VEC>
+static void launch_kv(bool read, const Kv4View &c, const OpBatch &b, const OpRows &k, const OpRows &v, hipStream_t st) {
+  // (a window of n positions touches at most (n + 30) / 32 + 1 records)
+  if (read) hipLaunchKernelGGL((k_kv4_read<NB, TYPE, VEC>), dim3((b.ntok - 1) / 32 + 1, c.nkv, b.nseq), dim3(256), 0, st, c, b, k, v);
+  else hipLaunchKernelGGL((k_kv4_append<NB, TYPE, VEC>), dim3((unsigned)(((long)b.ntok + 30) / KV4_GROUP + 1), c.nkv, b.nseq), dim3(256), 0, st, c, b, k, v);
+  ZL_HIP(hipGetLastError());
+}
+template <int NB, int TYPE>
+static void launch_kv_v(bool read, const Kv4View &c, const OpBatch &b, const OpRows &k, const OpRows &v, hipStream_t st) {
+  if (whole_pieces(k, TYPE) && whole_pieces(v, TYPE)) launch_kv<NB, TYPE, true>(read, c, b, k, v, st);
+  else launch_kv<NB, TYPE, false>(read, c, b, k, v, st);
+}
+template <int NB>
+static void launch_kv_t(bool read, const Kv4View &c, const OpBatch &b, int type, const OpRows &k, const OpRows &v, hipStream_t st) {
+  if (type == T_F32) launch_kv_v<NB, T_F32>(read, c, b, k, v, st);
+  else if (type == T_F16) launch_kv_v<NB, T_F16>(read, c, b, k, v, st);
+  else launch_kv_v<NB, T_BF16>(read, c, b, k, v, st);
+}
+static void launch_kv_nb(bool read, const Kv4View &c, const OpBatch &b, int type, const OpRows &k, const OpRows &v, hipStream_t st) {
+  if (c.hd == 64) launch_kv_t<2>(read, c, b, type, k, v, st);
+  else if (c.hd == 128) launch_kv_t<4>(read, c, b, type, k, v, st);
+  else launch_kv_t<8>(read, c, b, type, k, v, st);
+}
+void launch_kv4_append(const Kv4View &c, const OpBatch &b, int type, const OpRows &k, const OpRows &v, hipStream_t st) {
+  launch_kv_nb(false, c, b, type, k, v, st);
+}
+void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows &k, const OpRows &v, hipStream_t st) {
+  launch_kv_nb(true, c, b, type, k, v, st);
 }
 
 // ---------------------------------------------------------------------------------------------- attention
@@ -803,19 +901,4 @@ void launch_kv4_attention(const Kv4Attn &a, int type, hipStream_t st) {
   else launch_attention_t<8>(a, type, st);
 }
 
-#define ZL_BY_TYPE(type, K, ...)                                             \
-  do {                                                                       \
-    if ((type) == T_F32) hipLaunchKernelGGL((K<T_F32>), __VA_ARGS__);        \
-    else if ((type) == T_F16) hipLaunchKernelGGL((K<T_F16>), __VA_ARGS__);   \
-    else hipLaunchKernelGGL((K<T_BF16>), __VA_ARGS__);                       \
-    ZL_HIP(hipGetLastError());                                               \
-  } while (0)
-
-void launch_kv4_append(const Kv4View &c, const OpBatch &b, int type, const OpRows &k, const OpRows &v, hipStream_t st) {
-  const dim3 grid((b.ntok + 30) / KV4_GROUP + 1, c.nkv, b.nseq);  // (a window of n positions touches at most this many records)
-  ZL_BY_TYPE(type, k_kv4_append, grid, dim3(256), 32 * c.hd, st, c, b, k, v);
-}
-void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows &k, const OpRows &v, hipStream_t st) {
-  ZL_BY_TYPE(type, k_kv4_read, dim3(b.ntok, c.nkv, b.nseq), dim3(c.hd), 0, st, c, b, k, v);
-}
 }  // namespace zl
