@@ -243,11 +243,20 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// The eight codes of a word less 8, as f16: pair r of (word >> 4 r) under the exponent of 1024, less 1032. k: 0x64006400 in a
-// vector register, so that and and or are one instruction (which takes a single scalar operand). Codes as they lie are f16
-// denormals, which the matrix cores take as well and which cost no and-or and no subtraction; but sums that start at -8 sum q
-// to make up for it lose five bits (outputs 7e-6 off float64's, against 2e-7), and the time is the same.
+// The eight codes of a word as f16 operands: pair r of (word >> 4 r).
+// TINY: as they lie, f16 denormals of code 2^-24, which the matrix cores take (16 cycles of a SIMD a word); the 2^24 and the
+// 8 to be taken off follow the sums. Sums of codes are larger than sums of codes less 8, and they lose bits: 7e-6 of an output
+// against 2e-7, so this is for 16-bit rows, whose own rounding is 30 times that.
+// Else: less 8, under the exponent of 1024 and less 1032 (40 cycles a word). k: 0x64006400 in a vector register, so that and
+// and or are one instruction (which takes a single scalar operand).
+template <bool TINY>
 __device__ __forceinline__ h8 unpack8(uint32_t w, uint32_t k) {
+  if constexpr (TINY) {
+    u4 x;
+    #pragma unroll
+    for (int r = 0; r < 4; r++) x[r] = (w >> (4 * r)) & 0x000f000fu;
+    return __builtin_bit_cast(h8, x);
+  }
   h8 x;
   #pragma unroll
   for (int r = 0; r < 4; r++) {
@@ -257,6 +266,8 @@ __device__ __forceinline__ h8 unpack8(uint32_t w, uint32_t k) {
   }
   return x;
 }
+constexpr float TINY_ONE = 16777216.0f;  // 2^24: a code's unit
+constexpr h8 ONES = {1, 1, 1, 1, 1, 1, 1, 1};
 // Scale v (of four positions) of entry i (position tile and block) of a lane's loads: taken out of its register where it is
 // used, as an operand half.
 template <int N>
@@ -264,37 +275,19 @@ __device__ __forceinline__ float scale_at(const u4 (&s)[N], int i, int v) {
   const uint32_t w = s[i >> 1][2 * (i & 1) + (v >> 1)];  // (a value of its own: a cast of the element itself takes element 0)
   return (float)__builtin_bit_cast(h2, w)[v & 1];
 }
-// Weights p times the value scales of their positions (f16 pairs d), rounded to f16, and with LOW the rest, rounded to f16:
-// v_fma_mixlo / mixhi round the exact product once, a product in f32 and a conversion twice. The compiler takes either for the
-// same source, from one kernel (and one element) to the next; a row's bits must not depend on that, so the instructions are
-// written out. (Register halves are read again four instructions after they were written at the earliest.)
-template <bool LOW>
-__device__ __forceinline__ void weigh8(const float (&p)[8], const uint32_t (&d)[4], u4 &hi, u4 &lo) {
-  uint32_t h[4], r[4] = {0, 0, 0, 0};
-  #define ZL_MIX(W, A, B, C, SEL) "v_fma_mix" W "_f16 " A ", " B ", " C SEL "\n\t"
-  __asm__(ZL_MIX("lo", "%0", "%4", "%12, 0", " op_sel_hi:[0,1,0]") ZL_MIX("lo", "%1", "%6", "%13, 0", " op_sel_hi:[0,1,0]")
-          ZL_MIX("lo", "%2", "%8", "%14, 0", " op_sel_hi:[0,1,0]") ZL_MIX("lo", "%3", "%10", "%15, 0", " op_sel_hi:[0,1,0]")
-          ZL_MIX("hi", "%0", "%5", "%12, 0", " op_sel:[0,1,0] op_sel_hi:[0,1,0]") ZL_MIX("hi", "%1", "%7", "%13, 0", " op_sel:[0,1,0] op_sel_hi:[0,1,0]")
-          ZL_MIX("hi", "%2", "%9", "%14, 0", " op_sel:[0,1,0] op_sel_hi:[0,1,0]") ZL_MIX("hi", "%3", "%11", "%15, 0", " op_sel:[0,1,0] op_sel_hi:[0,1,0]")
-          "s_nop 1"
-          : "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3])
-          : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "v"(d[0]), "v"(d[1]), "v"(d[2]), "v"(d[3]));
-  if (LOW)
-    __asm__(ZL_MIX("lo", "%0", "%4", "%12, -%16", " op_sel_hi:[0,1,1]") ZL_MIX("lo", "%1", "%6", "%13, -%17", " op_sel_hi:[0,1,1]")
-            ZL_MIX("lo", "%2", "%8", "%14, -%18", " op_sel_hi:[0,1,1]") ZL_MIX("lo", "%3", "%10", "%15, -%19", " op_sel_hi:[0,1,1]")
-            ZL_MIX("hi", "%0", "%5", "%12, -%16", " op_sel:[0,1,1] op_sel_hi:[0,1,1]") ZL_MIX("hi", "%1", "%7", "%13, -%17", " op_sel:[0,1,1] op_sel_hi:[0,1,1]")
-            ZL_MIX("hi", "%2", "%9", "%14, -%18", " op_sel:[0,1,1] op_sel_hi:[0,1,1]") ZL_MIX("hi", "%3", "%11", "%15, -%19", " op_sel:[0,1,1] op_sel_hi:[0,1,1]")
-            "s_nop 1"
-            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
-            : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "v"(d[0]), "v"(d[1]), "v"(d[2]), "v"(d[3]),
-              "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]));
-  #undef ZL_MIX
-  hi = u4{h[0], h[1], h[2], h[3]};
-  lo = u4{r[0], r[1], r[2], r[3]};
-}
 __device__ __forceinline__ int wave_max(int v) { return group_reduce(v, 64, [](int x, int y) { return max(x, y); }); }
-__device__ __forceinline__ float sum4(float x) { x += swizzle_xor16(x); return x + __shfl_xor(x, 32, 64); }
-__device__ __forceinline__ float max4(float x) { x = fmaxf(x, swizzle_xor16(x)); return fmaxf(x, __shfl_xor(x, 32, 64)); }
+// Over the four lanes l % 16 + 0, 16, 32, 48: rows of 16 lanes are swapped pairwise (16, then 32 apart), no trip through LDS.
+template <class Op>
+__device__ __forceinline__ float over4(float x, Op op) {
+  const uint32_t a = __float_as_uint(x);
+  const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const float y = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  const uint32_t b = __float_as_uint(y);
+  const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return op(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float sum4(float x) { return over4(x, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ float max4(float x) { return over4(x, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A softmax sum in progress; O holds N of the row's dimensions.
@@ -318,23 +311,61 @@ struct Sum {
   }
 };
 
+// K pieces at once, the first `n` of them: what folding them one by one gives, with the factors formed side by side.
+template <int K, int N>
+__device__ __forceinline__ void fold_all(Sum<N> &f, const float2 (&ml)[K], const float (&o)[K][N], int n) {
+  float M = f.m, a[K], b[K];
+  bool every = n >= K;  // all of them, none empty: no selects
+  #pragma unroll
+  for (int k = 0; k < K; k++) every = every && ml[k].x > -INFINITY;
+  if (every) {
+    #pragma unroll
+    for (int k = 0; k < K; k++) {
+      const float to = fmaxf(M, ml[k].x);
+      a[k] = exp2_(M - to);
+      b[k] = exp2_(ml[k].x - to);
+      M = to;
+    }
+    f.m = M;
+    #pragma unroll
+    for (int k = 0; k < K; k++) {
+      f.l = fmaf(f.l, a[k], ml[k].y * b[k]);
+      #pragma unroll
+      for (int i = 0; i < N; i++) f.o[i] = fmaf(f.o[i], a[k], o[k][i] * b[k]);
+    }
+    return;
+  }
+  for (int k = 0; k < K; k++) {
+    __asm__ volatile("");
+    if (k >= n) break;
+    Sum<N> p;
+    p.m = ml[k].x;
+    p.l = ml[k].y;
+    #pragma unroll
+    for (int i = 0; i < N; i++) p.o[i] = o[k][i];
+    f.fold(p);
+  }
+}
+
 // The queries of a tile of 16 rows as right operands: lane l has row l % 16, dimensions 32 b + 8 (l / 16) + e; and the factor
 // from the products (code units, scaled queries) to scores in powers of two.
-template <int NB>
+template <int NB, bool TINY>
 struct Queries {
   h8 hi[NB], lo[NB];
+  f4 z[NB];  // TINY: -8 2^-24 times the sum of block b of the lane's row, where the scores' sums start; else 0
   float c;
 };
 template <int NB, int TYPE>
-__device__ __forceinline__ void load_queries(Queries<NB> &q, const typename ValueOf<TYPE>::t *row, float scale, int lane) {
-  typedef typename ValueOf<TYPE>::t T;
-  float v[NB][8], am = 0.0f;
-  bool bad = false;
-  const T *p = row + 8 * (lane >> 4);
+__device__ __forceinline__ void fetch_queries(float (&v)[NB][8], const typename ValueOf<TYPE>::t *row, int lane) {
   #pragma unroll
   for (int b = 0; b < NB; b++)
     #pragma unroll
-    for (int e = 0; e < 8; e++) v[b][e] = load_value<TYPE>(p[32 * b + e]);
+    for (int e = 0; e < 8; e++) v[b][e] = load_value<TYPE>(row[32 * b + 8 * (lane >> 4) + e]);
+}
+template <int NB, bool TINY>
+__device__ __forceinline__ void set_queries(Queries<NB, TINY> &q, const float (&v)[NB][8], float scale) {
+  float am = 0.0f;
+  bool bad = false;
   #pragma unroll
   for (int b = 0; b < NB; b++)
     #pragma unroll
@@ -349,14 +380,18 @@ __device__ __forceinline__ void load_queries(Queries<NB> &q, const typename Valu
   const bool fine = am < INFINITY;  // (a row with a value that is not finite is NaN)
   #pragma unroll
   for (int b = 0; b < NB; b++) {
+    float sum = 0.0f;
     #pragma unroll
     for (int e = 0; e < 8; e++) {
       const float x = fine ? ldexpf(v[b][e], ex) : NAN;
       q.hi[b][e] = (_Float16)x;
       q.lo[b][e] = (_Float16)(x - (float)q.hi[b][e]);
+      sum += (float)q.hi[b][e];
     }
+    sum = TINY ? sum4(sum) * (-8.0f / TINY_ONE) : 0.0f;
+    q.z[b] = f4{sum, sum, sum, sum};
   }
-  q.c = fmaxf((float)ldexp((double)scale * 1.4426950408889634, -ex), 1.17549435e-38f);  // (not 0: it multiplies -inf)
+  q.c = fmaxf((float)ldexp((double)scale * 1.4426950408889634, TINY ? 24 - ex : -ex), 1.17549435e-38f);  // (not 0: it multiplies -inf)
 }
 
 // A lane's share of a span (two records): code words and scales, loaded with every lane's 16-byte loads side by side.
@@ -386,12 +421,12 @@ struct SpanWords {
 
 // Scores of 16 positions (tile t of a record) in code units, from the tile's operands k(b) and key scales.
 template <int NB, bool LOQ, class K>
-__device__ __forceinline__ f4 tile_scores(const K &k, const u4 (&ks)[NB], int t, const Queries<NB> &q) {
+__device__ __forceinline__ f4 tile_scores(const K &k, const u4 (&ks)[NB], int t, const Queries<NB, !LOQ> &q) {
   f4 s = f4{0.0f, 0.0f, 0.0f, 0.0f};
   #pragma unroll
   for (int b = 0; b < NB; b++) {
     const h8 x = k(b);
-    f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[b], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+    f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[b], q.z[b], 0, 0, 0);
     if (LOQ) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.lo[b], acc, 0, 0, 0);
     #pragma unroll
     for (int v = 0; v < 4; v++) s[v] = fmaf(acc[v], scale_at(ks, t * NB + b, v), s[v]);
@@ -399,8 +434,10 @@ __device__ __forceinline__ f4 tile_scores(const K &k, const u4 (&ks)[NB], int t,
   return s;
 }
 
-// Positions that the lane's row does not see (those behind lim of the span): no weight, ...
+// Positions that the lane's row does not see (those behind lim of the span): no weight, ... (in spans at the rows' ends only:
+// the empty asm keeps the compiler from making selects of it that every span would pay for)
 __device__ __forceinline__ void mask_scores(f4 (&s)[2][2], int lim, int g) {
+  __asm__ volatile("");
   #pragma unroll
   for (int i = 0; i < 2; i++)
     #pragma unroll
@@ -408,18 +445,31 @@ __device__ __forceinline__ void mask_scores(f4 (&s)[2][2], int lim, int g) {
       #pragma unroll
       for (int v = 0; v < 4; v++) s[i][t][v] = 32 * i + 16 * t + 4 * g + v > lim ? -INFINITY : s[i][t][v];
 }
-// ... and a scale of 0 (a stale one may be NaN): d, the pairs of block b in record i.
-__device__ __forceinline__ void mask_scales(uint32_t (&d)[4], int i, int lim, int g) {
+// ... and a scale of 0 (a stale one may be NaN): record i's value scales.
+template <int NB>
+__device__ __forceinline__ void mask_scales(u4 (&vs)[NB], int i, int lim, int g) {
+  __asm__ volatile("");
   #pragma unroll
   for (int t = 0; t < 2; t++) {
     const int n = lim - 32 * i - 16 * t - 4 * g;  // the last of the lane's four positions that is seen
-    d[2 * t] &= n >= 1 ? 0xffffffffu : n >= 0 ? 0xffffu : 0u;
-    d[2 * t + 1] &= n >= 3 ? 0xffffffffu : n >= 2 ? 0xffffu : 0u;
+    const uint32_t m0 = n >= 1 ? 0xffffffffu : n >= 0 ? 0xffffu : 0u, m1 = n >= 3 ? 0xffffffffu : n >= 2 ? 0xffffu : 0u;
+    #pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const int e = t * NB + b;
+      vs[e >> 1][2 * (e & 1)] &= m0;
+      vs[e >> 1][2 * (e & 1) + 1] &= m1;
+    }
   }
 }
 
-// Scores to weights, in place; the span's reference and the sum of its weights.
-__device__ __forceinline__ void span_softmax(f4 (&s)[2][2], float c, float &m, float &l) {
+// Weights of a lane's positions (four neighbouring ones of each tile of both records) in two f16 parts.
+template <bool LOW>
+struct Weights {
+  h2 hi[2][2][2], lo[2][2][2];  // [record][tile][pair]
+};
+// Scores to weights; the span's reference and the sum of its weights.
+template <bool LOW>
+__device__ __forceinline__ void span_softmax(const f4 (&s)[2][2], float c, Weights<LOW> &w, float &m, float &l) {
   float x = -INFINITY;
   #pragma unroll
   for (int i = 0; i < 2; i++)
@@ -435,24 +485,35 @@ __device__ __forceinline__ void span_softmax(f4 (&s)[2][2], float c, float &m, f
     #pragma unroll
     for (int t = 0; t < 2; t++)
       #pragma unroll
-      for (int v = 0; v < 4; v++) {
-        s[i][t][v] = exp2_(fmaf(s[i][t][v] - ref, c, 3.0f));
-        l += s[i][t][v];
+      for (int v = 0; v < 4; v += 2) {
+        const float p0 = exp2_(fmaf(s[i][t][v] - ref, c, 3.0f)), p1 = exp2_(fmaf(s[i][t][v + 1] - ref, c, 3.0f));
+        l += p0;
+        l += p1;
+        const h2 h = {(_Float16)p0, (_Float16)p1};
+        w.hi[i][t][v >> 1] = h;
+        // (the differences are exact, so that they are rounded once in whatever instructions they are formed)
+        if (LOW) w.lo[i][t][v >> 1] = (h2){(_Float16)fmaf(-1.0f, (float)h[0], p0), (_Float16)fmaf(-1.0f, (float)h[1], p1)};
       }
   m = x * c - 3.0f;
   l = sum4(l);
 }
 
-// Weights of record i times the value scales of block b, as right operands.
+// Weights of record i times the value scales d of block b, as right operands, in packed f16: hi = f16(ph d), and with LOW the
+// rest lo = f16(f16(ph d - hi) + pl d), the inner difference exact. Every step rounds once, in whichever kernel it is.
 template <int NB, bool LOW>
-__device__ __forceinline__ void weigh(const f4 (&s)[2][2], const u4 (&vs)[NB], int i, int b, bool masked, int lim, int g, h8 &hi, h8 &lo) {
-  const float p[8] = {s[i][0][0], s[i][0][1], s[i][0][2], s[i][0][3], s[i][1][0], s[i][1][1], s[i][1][2], s[i][1][3]};
-  uint32_t d[4] = {vs[b >> 1][2 * (b & 1)], vs[b >> 1][2 * (b & 1) + 1], vs[(NB + b) >> 1][2 * (b & 1)], vs[(NB + b) >> 1][2 * (b & 1) + 1]};
-  if (masked) mask_scales(d, i, lim, g);
-  u4 hu, lu;
-  weigh8<LOW>(p, d, hu, lu);
-  hi = __builtin_bit_cast(h8, hu);
-  lo = __builtin_bit_cast(h8, lu);
+__device__ __forceinline__ void weigh(const Weights<LOW> &w, const u4 (&vs)[NB], int i, int b, h8 &hi, h8 &lo) {
+  const uint32_t d[4] = {vs[b >> 1][2 * (b & 1)], vs[b >> 1][2 * (b & 1) + 1], vs[(NB + b) >> 1][2 * (b & 1)], vs[(NB + b) >> 1][2 * (b & 1) + 1]};
+  #pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const h2 e = __builtin_bit_cast(h2, d[k]), p = w.hi[i][k >> 1][k & 1], h = p * e;
+    hi[2 * k] = h[0];
+    hi[2 * k + 1] = h[1];
+    if (LOW) {
+      const h2 r = __builtin_elementwise_fma(w.lo[i][k >> 1][k & 1], e, __builtin_elementwise_fma(p, e, -h));
+      lo[2 * k] = r[0];
+      lo[2 * k + 1] = r[1];
+    }
+  }
 }
 
 // The rows of a block: tile t of KV head kvh of sequence s. A row's last position; below 0 it sees nothing.
@@ -489,6 +550,57 @@ __device__ __forceinline__ void emit(const Kv4Attn &a, int s, int tok, int head,
   ((T *)a.out.p)[s * a.out.seq + tok * a.out.tok + head * a.out.head + dim] = store_value<TYPE>(o);
 }
 
+// A span's two products of block b and record: values times weights, and with TINY the weights' sums.
+template <bool LOW, bool TINY>
+__device__ __forceinline__ void weighted_sums(f4 &o0, f4 &o1, f4 &wsum, h8 x0, h8 x1, h8 hi, h8 lo) {
+  o0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, hi, o0, 0, 0, 0);
+  o1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, hi, o1, 0, 0, 0);
+  if (TINY) wsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ONES, hi, wsum, 0, 0, 0);
+  if (LOW) {
+    o0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, lo, o0, 0, 0, 0);
+    o1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, lo, o1, 0, 0, 0);
+    if (TINY) wsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ONES, lo, wsum, 0, 0, 0);
+  }
+}
+// TINY: sums of codes to sums of codes less 8.
+template <int NB>
+__device__ __forceinline__ void take_off(f4 (&o)[2 * NB], const f4 (&wsum)[NB]) {
+  #pragma unroll
+  for (int j = 0; j < 2 * NB; j++)
+    #pragma unroll
+    for (int v = 0; v < 4; v++) o[j][v] = fmaf(o[j][v], TINY_ONE, -8.0f * wsum[j >> 1][v]);
+}
+
+// Row r of a block's tile: its spans of chunk c, in LDS ([span][row], span strides so and 16), to the row's output or the chunk's
+// record. The lane's dimensions are x, x + 32, ..., N of them.
+template <int NB, int TYPE, int N>
+__device__ __forceinline__ void fold_row(const Kv4Attn &a, const Tile &tl, int r, int c, int ns, int x, const float *o, int so, const float2 *ml) {
+  int tok, head;
+  const int last = tl.last(a, r, &tok, &head);
+  if (last < c * CHUNK) return;
+  float2 pml[SPANS];
+  float po[SPANS][N];
+  #pragma unroll
+  for (int w = 0; w < SPANS; w++) {
+    pml[w] = ml[w * 16];
+    #pragma unroll
+    for (int i = 0; i < N; i++) po[w][i] = o[w * so + 32 * i];
+  }
+  Sum<N> f;
+  f.clear();
+  fold_all<SPANS, N>(f, pml, po, ns);
+  if (last < CHUNK) {
+    #pragma unroll
+    for (int i = 0; i < N; i++) emit<TYPE>(a, tl.s, tok, head, x + 32 * i, f.o[i] / f.l);
+  } else {
+    const long row = row_index(a, tl.s, tok, head);
+    float *d = record_o(a, row, c);
+    #pragma unroll
+    for (int i = 0; i < N; i++) d[x + 32 * i] = f.o[i];
+    if (x == 0) *record_ml(a, row, c) = make_float2(f.m, f.l);
+  }
+}
+
 // Few rows: a block takes one tile of 16 rows and a chunk at a time (chunks x, x + X, ...), one span per wave, and folds the
 // spans in LDS. Rows that see a single chunk are finished here, the others leave the chunk's record. The next chunk's keys are
 // requested when the scores are done with this one's, its values after the weighted sums, so that the loads run under the
@@ -500,20 +612,21 @@ constexpr size_t chunk_lds(int nr) { return (size_t)chunk_buffers<NB>() * SPANS 
 template <int NB, int TYPE>
 __global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int tiles) {
   constexpr int HD = 32 * NB, LDO = HD + 4, NBUF = chunk_buffers<NB>();
-  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16;
+  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ;
   extern __shared__ __align__(16) float lds_all[];  // per buffer: [spans][rows][LDO], then (m, l) [spans][16]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   const Tile tl(a, blockIdx.z, blockIdx.y / tiles, blockIdx.y % tiles * 16);
   const int nr = min(16, a.b.ntok * tl.group - tl.base);
   int tok, head;
   const int last = tl.last(a, n, &tok, &head);
   const int most = wave_max(last);
-  // the fold's rows: 32 lanes each
-  const int fr = tid >> 5, fl = tid & 31;
-  int ft, fh;
-  const int flast = fr < nr ? tl.last(a, fr, &ft, &fh) : ROW_ABSENT;
-  if (blockIdx.x == 0 && (flast == ROW_NONE || flast == ROW_BAD))
-    for (int i = 0; i < NB; i++) emit<TYPE>(a, tl.s, ft, fh, 32 * i + fl, flast == ROW_NONE ? 0.0f : NAN);
+  const int fr = tid >> 5, fl = tid & 31;  // the fold: 32 lanes a row
+  if (blockIdx.x == 0 && fr < nr) {
+    int ft, fh;
+    const int flast = tl.last(a, fr, &ft, &fh);
+    if (flast == ROW_NONE || flast == ROW_BAD)
+      for (int i = 0; i < NB; i++) emit<TYPE>(a, tl.s, ft, fh, 32 * i + fl, flast == ROW_NONE ? 0.0f : NAN);
+  }
   if (most < 0 || (int)blockIdx.x * CHUNK > most) return;
   typedef typename ValueOf<TYPE>::t T;
   uint32_t k1024 = 0x64006400u;
@@ -524,11 +637,15 @@ __global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int 
     const int p0 = c * CHUNK + wave * SPAN;
     return head0 + (long)((p0 <= most ? p0 : min(c * CHUNK, most)) / SPAN) * (2 * kv4_record(HD));
   };
+  // (loads complete in order: the queries, which take a while to prepare, are requested first)
   SpanWords<NB> w;
+  Queries<NB, TINY> q;
+  float qv[NB][8];
+  fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), lane);
   w.load_keys(record_at(blockIdx.x), lane);
   if (NB <= 4) w.load_values(record_at(blockIdx.x), lane);
-  Queries<NB> q;
-  load_queries<NB, TYPE>(q, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.scale, lane);
+  __builtin_amdgcn_sched_barrier(0);
+  set_queries<NB, TINY>(q, qv, a.scale);
   int buf = 0;
   for (int c = blockIdx.x; c * CHUNK <= most; c += gridDim.x) {
     float *lds = lds_all + buf * SPANS * (nr * LDO + 32);
@@ -541,32 +658,36 @@ __global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int 
     for (int i = 0; i < 2; i++)
       #pragma unroll
       for (int t = 0; t < 2; t++) {
-        s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], k1024); }, w.ks[i], t, q);
+        s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], k1024); }, w.ks[i], t, q);
         __builtin_amdgcn_sched_barrier(0);
       }
     if (NB <= 4) w.load_keys(next, lane);
     else w.load_values(record_at(c), lane);  // (heads of 256 leave no registers for loads ahead)
     __builtin_amdgcn_sched_barrier(0);
-    if (masked) mask_scores(s, lim, g);
+    if (masked) {
+      mask_scores(s, lim, g);
+      mask_scales<NB>(w.vs[0], 0, lim, g);
+      mask_scales<NB>(w.vs[1], 1, lim, g);
+    }
     float m, l;
-    span_softmax(s, q.c, m, l);
-    f4 o[2 * NB];
+    Weights<LOW> pw;
+    span_softmax<LOW>(s, q.c, pw, m, l);
+    f4 o[2 * NB], wsum[NB];
     #pragma unroll
     for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    #pragma unroll
+    for (int b = 0; b < NB; b++) wsum[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     #pragma unroll
     for (int i = 0; i < 2; i++)
       #pragma unroll
       for (int b = 0; b < NB; b++) {
         h8 hi, lo;
-        weigh<NB, LOW>(s, w.vs[i], i, b, masked, lim, g, hi, lo);
-        #pragma unroll
-        for (int j = 2 * b; j < 2 * b + 2; j++) {
-          const h8 x = unpack8(w.vw[i][j >> 2][j & 3], k1024);
-          o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, o[j], 0, 0, 0);
-          if (LOW) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, o[j], 0, 0, 0);
-        }
+        weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
+        const h8 x0 = unpack8<TINY>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], k1024), x1 = unpack8<TINY>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], k1024);
+        weighted_sums<LOW, TINY>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
         __builtin_amdgcn_sched_barrier(0);
       }
+    if (TINY) take_off<NB>(o, wsum);
     if (NB <= 4) w.load_values(next, lane);
     else w.load_keys(next, lane);
     __builtin_amdgcn_sched_barrier(0);
@@ -577,28 +698,13 @@ __global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int 
       if (g == 0) ml[wave * 16 + n] = make_float2(m, l);
     }
     __syncthreads();
-    if (flast >= c * CHUNK) {
-      const int ns = min(SPANS, (most - c * CHUNK) / SPAN + 1);
-      Sum<NB> f, p;
-      f.clear();
-      for (int w = 0; w < ns; w++) {
-        const float2 v = ml[w * 16 + fr];
-        p.m = v.x;
-        p.l = v.y;
-        #pragma unroll
-        for (int i = 0; i < NB; i++) p.o[i] = lds[(w * nr + fr) * LDO + 32 * i + fl];
-        f.fold(p);
-      }
-      if (flast < CHUNK) {
-        #pragma unroll
-        for (int i = 0; i < NB; i++) emit<TYPE>(a, tl.s, ft, fh, 32 * i + fl, f.o[i] / f.l);
-      } else {
-        const long row = row_index(a, tl.s, ft, fh);
-        float *o = record_o(a, row, c);
-        #pragma unroll
-        for (int i = 0; i < NB; i++) o[32 * i + fl] = f.o[i];
-        if (fl == 0) *record_ml(a, row, c) = make_float2(f.m, f.l);
-      }
+    // the fold: 32 lanes a row with all its dimensions, or where there are at most four rows one block of 32 each
+    const int ns = min(SPANS, (most - c * CHUNK) / SPAN + 1);
+    if (nr <= 16 / NB) {
+      const int r = fr / NB, i = fr % NB, x = 32 * i + fl;
+      if (r < nr) fold_row<NB, TYPE, 1>(a, tl, r, c, ns, x, lds + r * LDO + x, nr * LDO, ml + r);
+    } else if (fr < nr) {
+      fold_row<NB, TYPE, NB>(a, tl, fr, c, ns, fl, lds + fr * LDO + fl, nr * LDO, ml + fr);
     }
     if (NBUF == 2) buf ^= 1;
     else __syncthreads();
@@ -652,12 +758,15 @@ __global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a) {
     }
     __syncthreads();
     if (grp == 0)
-      for (int i = 0; i < min(JOIN_PARTS, np - b0); i++) {
-        Sum<1> p;
-        p.m = pml[i].x;
-        p.l = pml[i].y;
-        p.o[0] = po[i][fl];
-        f.fold(p);
+      for (int i0 = 0; i0 < min(JOIN_PARTS, np - b0); i0 += 8) {
+        float2 m8[8];
+        float o8[8][1];
+        #pragma unroll
+        for (int i = 0; i < 8; i++) {
+          m8[i] = pml[i0 + i];
+          o8[i][0] = po[i0 + i][fl];
+        }
+        fold_all<8, 1>(f, m8, o8, min(JOIN_PARTS, np - b0) - i0);
       }
     __syncthreads();
   }
@@ -676,10 +785,10 @@ struct SpanOperands {
 template <int NB, int TYPE, int RT>
 __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) {
   constexpr int HD = 32 * NB, REC = 36 * HD, NW = 2 * NB / 4;  // NW: 16-byte loads of a lane per wave (of 8 per record pair and NB / 2)
-  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16;
+  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ;
   extern __shared__ __align__(16) uint8_t lds_raw[];
   SpanOperands<NB> *buf = (SpanOperands<NB> *)lds_raw;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4, part = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4, part = blockIdx.x;
   const int row0 = blockIdx.y % blocks * (64 * RT) + wave * (16 * RT);
   int last[RT], tok[RT], head[RT], most = ROW_ABSENT, blockmost;
   const Tile tl(a, blockIdx.z, blockIdx.y / blocks, 0);
@@ -722,16 +831,19 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) 
     for (int x = 0; x < NW; x++) {
       const int idx = wave * NW + x, i = idx / NB, kv = idx / (NB / 2) & 1, j = idx % (NB / 2);
       #pragma unroll
-      for (int y = 0; y < 4; y++) (kv ? d.v : d.k)[i][4 * j + y][lane] = unpack8(words[x][y], k1024);
+      for (int y = 0; y < 4; y++) (kv ? d.v : d.k)[i][4 * j + y][lane] = unpack8<TINY>(words[x][y], k1024);
     }
     const int e = tid, i = e / (8 * NB), r = e % (8 * NB);
     if (e < 16 * NB) (r < 4 * NB ? d.ks : d.vs)[i][r % (4 * NB)] = scales;
   };
   load(0);
-  Queries<NB> q[RT];
+  Queries<NB, TINY> q[RT];
   #pragma unroll
-  for (int r = 0; r < RT; r++)
-    load_queries<NB, TYPE>(q[r], (const T *)a.q.p + tl.s * a.q.seq + (last[r] >= 0 ? tok[r] * a.q.tok + head[r] * a.q.head : 0), a.scale, lane);
+  for (int r = 0; r < RT; r++) {
+    float qv[NB][8];
+    fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last[r] >= 0 ? tok[r] * a.q.tok + head[r] * a.q.head : 0), lane);
+    set_queries<NB, TINY>(q[r], qv, a.scale);
+  }
   Sum<8 * NB> f[RT], u[RT];
   #pragma unroll
   for (int r = 0; r < RT; r++) f[r].clear(), u[r].clear();
@@ -759,37 +871,43 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) 
       }
       Sum<8 * NB> z[RT];
       bool masked[RT];
+      Weights<LOW> pw[RT];
       #pragma unroll
       for (int r = 0; r < RT; r++) {
         masked[r] = __ballot(last[r] - p0 < SPAN - 1) != 0;
         if (masked[r]) mask_scores(s[r], last[r] - p0, g);
-        span_softmax(s[r], q[r].c, z[r].m, z[r].l);
+        span_softmax<LOW>(s[r], q[r].c, pw[r], z[r].m, z[r].l);
       }
-      f4 o[RT][2 * NB];
+      f4 o[RT][2 * NB], wsum[RT][NB];
       #pragma unroll
       for (int r = 0; r < RT; r++)
         #pragma unroll
-        for (int j = 0; j < 2 * NB; j++) o[r][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < 2 * NB; j++) o[r][j] = f4{0.0f, 0.0f, 0.0f, 0.0f}, wsum[r][j >> 1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
       #pragma unroll
       for (int i = 0; i < 2; i++) {
-        u4 vs[NB];
+        u4 vs[RT][NB];
         #pragma unroll
-        for (int j = 0; j < NB; j++) vs[j] = d.vs[i][g * NB + j];
+        for (int j = 0; j < NB; j++) vs[0][j] = d.vs[i][g * NB + j];
+        #pragma unroll
+        for (int r = RT - 1; r >= 0; r--) {
+          #pragma unroll
+          for (int j = 0; j < NB; j++) vs[r][j] = vs[0][j];
+          if (masked[r]) mask_scales<NB>(vs[r], i, last[r] - p0, g);
+        }
         #pragma unroll
         for (int b = 0; b < NB; b++) {
           const h8 x0 = d.v[i][2 * b][lane], x1 = d.v[i][2 * b + 1][lane];
           #pragma unroll
           for (int r = 0; r < RT; r++) {
             h8 hi, lo;
-            weigh<NB, LOW>(s[r], vs, i, b, masked[r], last[r] - p0, g, hi, lo);
-            o[r][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, hi, o[r][2 * b], 0, 0, 0);
-            o[r][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, hi, o[r][2 * b + 1], 0, 0, 0);
-            if (LOW) {
-              o[r][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, lo, o[r][2 * b], 0, 0, 0);
-              o[r][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, lo, o[r][2 * b + 1], 0, 0, 0);
-            }
+            weigh<NB, LOW>(pw[r], vs[r], i, b, hi, lo);
+            weighted_sums<LOW, TINY>(o[r][2 * b], o[r][2 * b + 1], wsum[r][b], x0, x1, hi, lo);
           }
         }
+      }
+      if (TINY) {
+        #pragma unroll
+        for (int r = 0; r < RT; r++) take_off<NB>(o[r], wsum[r]);
       }
       #pragma unroll
       for (int r = 0; r < RT; r++) {
