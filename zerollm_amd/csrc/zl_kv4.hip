@@ -222,7 +222,7 @@ void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows 
 
 // ---------------------------------------------------------------------------------------------- attention
 // softmax(scale q K) V of a row (a token's query head) over positions 0 .. last, in f32 with the exponentials to base 2. The
-// positions are cut, by their index alone, into spans of 64, chunks of 512 (8 spans) and parts of 2048 (4 chunks). A span has
+// positions are cut, by their index alone, into spans of 64, chunks of 256 (4 spans) and parts of 2048 (8 chunks). A span has
 // a softmax of its own: its reference m (the largest score less 3, so that weights reach 8), l = sum of weights and
 // o = sum of weights times values. Spans are folded into their chunk in order, chunks into their part, parts into the row:
 //   M' = max(M, m), L = L 2^(M - M') + l 2^(m - M'), O = O 2^(M - M') + o 2^(m - M').
@@ -235,8 +235,8 @@ void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows 
 // below 2^14 and split into two f16 parts (22 bits, or all the bits of 16-bit queries); a weight times its value's scale
 // likewise where the output is f32 or f16 (a single f16 part would add an error as large as the rounding of an f16
 // output). Scores are scaled by their key's scale in f32, block by block.
-constexpr int SPAN = 64, CHUNK = 512, PART = 2048;
-constexpr int SPANS = CHUNK / SPAN, CHUNKS = PART / CHUNK;
+constexpr int SPAN = 64, CHUNK = 256, PART = 2048;
+constexpr int CHUNKS = PART / CHUNK;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -356,38 +356,48 @@ struct Queries {
   float c;
 };
 template <int NB, int TYPE>
-__device__ __forceinline__ void fetch_queries(float (&v)[NB][8], const typename ValueOf<TYPE>::t *row, int lane) {
-  #pragma unroll
-  for (int b = 0; b < NB; b++)
+__device__ __forceinline__ void fetch_queries(float (&v)[NB][8], const typename ValueOf<TYPE>::t *row, bool vec, int lane) {
+  const typename ValueOf<TYPE>::t *p = row + 8 * (lane >> 4);
+  if (vec) {
     #pragma unroll
-    for (int e = 0; e < 8; e++) v[b][e] = load_value<TYPE>(row[32 * b + 8 * (lane >> 4) + e]);
+    for (int b = 0; b < NB; b++) load8<TYPE, true>(p + 32 * b, v[b]);
+  } else {
+    #pragma unroll
+    for (int b = 0; b < NB; b++) load8<TYPE, false>(p + 32 * b, v[b]);
+  }
 }
 template <int NB, bool TINY>
 __device__ __forceinline__ void set_queries(Queries<NB, TINY> &q, const float (&v)[NB][8], float scale) {
-  float am = 0.0f;
-  bool bad = false;
+  float am = 0.0f, any = 0.0f;
   #pragma unroll
   for (int b = 0; b < NB; b++)
     #pragma unroll
     for (int e = 0; e < 8; e++) {
       am = fmaxf(am, fabsf(v[b][e]));
-      bad |= !(fabsf(v[b][e]) < INFINITY);
+      any = fmaf(v[b][e], 0.0f, any);  // 0, or NaN where a value is not finite: the row is NaN then
     }
-  am = max4(bad ? INFINITY : am);
+  am = max4(am);
+  any = sum4(any);
+  // a power of two that takes the largest value to [2^13, 2^14); rows below 2^-112 stay smaller: their scores are 0 all the same
   int ex = 0;
-  if (am > 0.0f && am < INFINITY) frexpf(am, &ex);
-  ex = 14 - ex;  // am 2^ex is in [2^13, 2^14)
-  const bool fine = am < INFINITY;  // (a row with a value that is not finite is NaN)
+  if (am > 0.0f) frexpf(am, &ex);
+  ex = min(126, 14 - ex);
+  const float up = __uint_as_float((uint32_t)(127 + ex) << 23) + any;
   #pragma unroll
   for (int b = 0; b < NB; b++) {
     float sum = 0.0f;
+    u4 hi, lo;
     #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float x = fine ? ldexpf(v[b][e], ex) : NAN;
-      q.hi[b][e] = (_Float16)x;
-      q.lo[b][e] = (_Float16)(x - (float)q.hi[b][e]);
-      sum += (float)q.hi[b][e];
+    for (int e = 0; e < 4; e++) {
+      const float x0 = v[b][2 * e] * up, x1 = v[b][2 * e + 1] * up;
+      const h2 h = {(_Float16)x0, (_Float16)x1};
+      const h2 r = {(_Float16)fmaf(-1.0f, (float)h[0], x0), (_Float16)fmaf(-1.0f, (float)h[1], x1)};
+      hi[e] = __builtin_bit_cast(uint32_t, h);
+      lo[e] = __builtin_bit_cast(uint32_t, r);
+      if (TINY) sum += (float)h[0] + (float)h[1];
     }
+    q.hi[b] = __builtin_bit_cast(h8, hi);
+    q.lo[b] = __builtin_bit_cast(h8, lo);
     sum = TINY ? sum4(sum) * (-8.0f / TINY_ONE) : 0.0f;
     q.z[b] = f4{sum, sum, sum, sum};
   }
@@ -571,190 +581,163 @@ __device__ __forceinline__ void take_off(f4 (&o)[2 * NB], const f4 (&wsum)[NB]) 
     for (int v = 0; v < 4; v++) o[j][v] = fmaf(o[j][v], TINY_ONE, -8.0f * wsum[j >> 1][v]);
 }
 
-// Row r of a block's tile: its spans of chunk c, in LDS ([span][row], span strides so and 16), to the row's output or the chunk's
-// record. The lane's dimensions are x, x + 32, ..., N of them.
-template <int NB, int TYPE, int N>
-__device__ __forceinline__ void fold_row(const Kv4Attn &a, const Tile &tl, int r, int c, int ns, int x, const float *o, int so, const float2 *ml) {
-  int tok, head;
-  const int last = tl.last(a, r, &tok, &head);
-  if (last < c * CHUNK) return;
-  float2 pml[SPANS];
-  float po[SPANS][N];
+// A tile's finished sums: the rows' outputs where a call has one record per row, else record `rec` of the rows that see it. Lane
+// l has row l % 16, dimensions 16 j + 4 (l / 16) + v.
+template <int NB, int TYPE>
+__device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last, int tok, int head, int rec, int first, const Sum<8 * NB> &f, int g) {
+  if (a.nrec == 1) {
+    if (last == ROW_ABSENT) return;
+    #pragma unroll
+    for (int j = 0; j < 2 * NB; j++)
+      #pragma unroll
+      for (int v = 0; v < 4; v++)
+        emit<TYPE>(a, tl.s, tok, head, 16 * j + 4 * g + v, last >= 0 ? f.o[4 * j + v] / f.l : last == ROW_NONE ? 0.0f : NAN);
+    return;
+  }
+  if (last < first) return;
+  const long row = row_index(a, tl.s, tok, head);
+  float *o = record_o(a, row, rec) + 4 * g;
   #pragma unroll
-  for (int w = 0; w < SPANS; w++) {
-    pml[w] = ml[w * 16];
-    #pragma unroll
-    for (int i = 0; i < N; i++) po[w][i] = o[w * so + 32 * i];
-  }
-  Sum<N> f;
-  f.clear();
-  fold_all<SPANS, N>(f, pml, po, ns);
-  if (last < CHUNK) {
-    #pragma unroll
-    for (int i = 0; i < N; i++) emit<TYPE>(a, tl.s, tok, head, x + 32 * i, f.o[i] / f.l);
-  } else {
-    const long row = row_index(a, tl.s, tok, head);
-    float *d = record_o(a, row, c);
-    #pragma unroll
-    for (int i = 0; i < N; i++) d[x + 32 * i] = f.o[i];
-    if (x == 0) *record_ml(a, row, c) = make_float2(f.m, f.l);
-  }
+  for (int j = 0; j < 2 * NB; j++) *(f4 *)(o + 16 * j) = f4{f.o[4 * j], f.o[4 * j + 1], f.o[4 * j + 2], f.o[4 * j + 3]};
+  if (g == 0) *record_ml(a, row, rec) = make_float2(f.m, f.l);
 }
 
-// Few rows: a block takes one tile of 16 rows and a chunk at a time (chunks x, x + X, ...), one span per wave, and folds the
-// spans in LDS. Rows that see a single chunk are finished here, the others leave the chunk's record. The next chunk's keys are
-// requested when the scores are done with this one's, its values after the weighted sums, so that the loads run under the
-// rest; two buffers in LDS, so that a block meets once per chunk.
-template <int NB>
-constexpr int chunk_buffers() { return NB <= 4 ? 2 : 1; }  // (heads of 256: 133 KB each)
-template <int NB>
-constexpr size_t chunk_lds(int nr) { return (size_t)chunk_buffers<NB>() * SPANS * (nr * (32 * NB + 4) + 32) * 4; }
+// Few rows: a wave takes one tile of 16 rows and a chunk at a time, span by span, and leaves the chunk's record; no wave waits
+// for another. The next span's keys are requested when the scores are done with this one's, its values after the weighted
+// sums, so that the loads run under the rest. (A chunk of 512 per block, one span per wave, folded in LDS behind a barrier:
+// decode_131k 47 us against 27, the waves waiting for each other and for the fold.)
 template <int NB, int TYPE>
-__global__ __launch_bounds__(64 * SPANS) void k_kv4_chunks(const Kv4Attn a, int tiles) {
-  constexpr int HD = 32 * NB, LDO = HD + 4, NBUF = chunk_buffers<NB>();
-  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ;
-  extern __shared__ __align__(16) float lds_all[];  // per buffer: [spans][rows][LDO], then (m, l) [spans][16]
+__global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4Attn a, int tiles) {
+  constexpr int HD = 32 * NB;
+  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   const Tile tl(a, blockIdx.z, blockIdx.y / tiles, blockIdx.y % tiles * 16);
-  const int nr = min(16, a.b.ntok * tl.group - tl.base);
   int tok, head;
   const int last = tl.last(a, n, &tok, &head);
-  const int most = wave_max(last);
-  const int fr = tid >> 5, fl = tid & 31;  // the fold: 32 lanes a row
-  if (blockIdx.x == 0 && fr < nr) {
-    int ft, fh;
-    const int flast = tl.last(a, fr, &ft, &fh);
-    if (flast == ROW_NONE || flast == ROW_BAD)
-      for (int i = 0; i < NB; i++) emit<TYPE>(a, tl.s, ft, fh, 32 * i + fl, flast == ROW_NONE ? 0.0f : NAN);
+  const int most = __builtin_amdgcn_readfirstlane(wave_max(last)), c0 = blockIdx.x * 4 + wave, step = gridDim.x * 4;
+  Sum<8 * NB> u;
+  u.clear();
+  if (most < c0 * CHUNK) {
+    if (a.nrec == 1 && c0 == 0) leave<NB, TYPE>(a, tl, last, tok, head, 0, 0, u, g);
+    return;
   }
-  if (most < 0 || (int)blockIdx.x * CHUNK > most) return;
   typedef typename ValueOf<TYPE>::t T;
   uint32_t k1024 = 0x64006400u;
   __asm__("" : "+v"(k1024));
-  // (a wave whose span lies behind the last position reads its chunk's first record, for nothing)
-  const uint8_t *head0 = record_of(a.c, tl.slot, tl.kvh, 0);
-  auto record_at = [&](int c) {
-    const int p0 = c * CHUNK + wave * SPAN;
-    return head0 + (long)((p0 <= most ? p0 : min(c * CHUNK, most)) / SPAN) * (2 * kv4_record(HD));
-  };
   // (loads complete in order: the queries, which take a while to prepare, are requested first)
   SpanWords<NB> w;
   Queries<NB, TINY> q;
-  float qv[NB][8];
-  fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), lane);
-  w.load_keys(record_at(blockIdx.x), lane);
-  if (NB <= 4) w.load_values(record_at(blockIdx.x), lane);
-  __builtin_amdgcn_sched_barrier(0);
-  set_queries<NB, TINY>(q, qv, a.scale);
-  int buf = 0;
-  for (int c = blockIdx.x; c * CHUNK <= most; c += gridDim.x) {
-    float *lds = lds_all + buf * SPANS * (nr * LDO + 32);
-    float2 *ml = (float2 *)(lds + SPANS * nr * LDO);
-    const int p0 = c * CHUNK + wave * SPAN, lim = last - p0;
-    const uint8_t *next = record_at(c + gridDim.x);
-    const bool masked = __ballot(lim < SPAN - 1) != 0;
-    f4 s[2][2];
-    #pragma unroll
-    for (int i = 0; i < 2; i++)
-      #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], k1024); }, w.ks[i], t, q);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    if (NB <= 4) w.load_keys(next, lane);
-    else w.load_values(record_at(c), lane);  // (heads of 256 leave no registers for loads ahead)
+  {
+    float qv[NB][8];
+    fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.qvec, lane);
+    const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, (long)c0 * (CHUNK / KV4_GROUP));
+    w.load_keys(rec, lane);
+    if (AHEAD) w.load_values(rec, lane);
     __builtin_amdgcn_sched_barrier(0);
-    if (masked) {
-      mask_scores(s, lim, g);
-      mask_scales<NB>(w.vs[0], 0, lim, g);
-      mask_scales<NB>(w.vs[1], 1, lim, g);
-    }
-    float m, l;
-    Weights<LOW> pw;
-    span_softmax<LOW>(s, q.c, pw, m, l);
-    f4 o[2 * NB], wsum[NB];
-    #pragma unroll
-    for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    #pragma unroll
-    for (int b = 0; b < NB; b++) wsum[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    #pragma unroll
-    for (int i = 0; i < 2; i++)
+    set_queries<NB, TINY>(q, qv, a.scale);
+  }
+  for (int c = c0; c * CHUNK <= most; c += step) {
+    const int ns = min(CHUNK / SPAN, (most - c * CHUNK) / SPAN + 1);
+    u.clear();
+    for (int sp = 0; sp < ns; sp++) {
+      const int p0 = c * CHUNK + sp * SPAN, lim = last - p0;
+      const int pn = sp + 1 < ns ? p0 + SPAN : (c + step) * CHUNK <= most ? (c + step) * CHUNK : p0;  // (the last one is read again, for nothing)
+      const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, p0 / KV4_GROUP), *next = record_of(a.c, tl.slot, tl.kvh, pn / KV4_GROUP);
+      const bool masked = __ballot(lim < SPAN - 1) != 0;
+      f4 s[2][2];
       #pragma unroll
-      for (int b = 0; b < NB; b++) {
-        h8 hi, lo;
-        weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
-        const h8 x0 = unpack8<TINY>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], k1024), x1 = unpack8<TINY>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], k1024);
-        weighted_sums<LOW, TINY>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < 2; i++)
+        #pragma unroll
+        for (int t = 0; t < 2; t++) {
+          s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], k1024); }, w.ks[i], t, q);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      if (AHEAD) w.load_keys(next, lane);
+      else w.load_values(rec, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      if (masked) {
+        mask_scores(s, lim, g);
+        mask_scales<NB>(w.vs[0], 0, lim, g);
+        mask_scales<NB>(w.vs[1], 1, lim, g);
       }
-    if (TINY) take_off<NB>(o, wsum);
-    if (NB <= 4) w.load_values(next, lane);
-    else w.load_keys(next, lane);
-    __builtin_amdgcn_sched_barrier(0);
-    if (p0 <= most && n < nr) {
-      float *d = lds + (wave * nr + n) * LDO + 4 * g;
+      Sum<8 * NB> r;
+      Weights<LOW> pw;
+      span_softmax<LOW>(s, q.c, pw, r.m, r.l);
+      f4 o[2 * NB], wsum[NB];
       #pragma unroll
-      for (int j = 0; j < 2 * NB; j++) *(f4 *)(d + 16 * j) = o[j];
-      if (g == 0) ml[wave * 16 + n] = make_float2(m, l);
+      for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      #pragma unroll
+      for (int b = 0; b < NB; b++) wsum[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      #pragma unroll
+      for (int i = 0; i < 2; i++)
+        #pragma unroll
+        for (int b = 0; b < NB; b++) {
+          h8 hi, lo;
+          weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
+          const h8 x0 = unpack8<TINY>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], k1024), x1 = unpack8<TINY>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], k1024);
+          weighted_sums<LOW, TINY>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      if (AHEAD) w.load_values(next, lane);
+      else w.load_keys(next, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      if (TINY) take_off<NB>(o, wsum);
+      #pragma unroll
+      for (int j = 0; j < 2 * NB; j++)
+        #pragma unroll
+        for (int v = 0; v < 4; v++) r.o[4 * j + v] = o[j][v];
+      u.fold(r);
     }
-    __syncthreads();
-    // the fold: 32 lanes a row with all its dimensions, or where there are at most four rows one block of 32 each
-    const int ns = min(SPANS, (most - c * CHUNK) / SPAN + 1);
-    if (nr <= 16 / NB) {
-      const int r = fr / NB, i = fr % NB, x = 32 * i + fl;
-      if (r < nr) fold_row<NB, TYPE, 1>(a, tl, r, c, ns, x, lds + r * LDO + x, nr * LDO, ml + r);
-    } else if (fr < nr) {
-      fold_row<NB, TYPE, NB>(a, tl, fr, c, ns, fl, lds + fr * LDO + fl, nr * LDO, ml + fr);
-    }
-    if (NBUF == 2) buf ^= 1;
-    else __syncthreads();
+    leave<NB, TYPE>(a, tl, last, tok, head, c, c * CHUNK, u, g);
   }
 }
 
-// Rows of several records: a block per (row, 32 dimensions), a dimension per lane. Eight groups of 32 lanes fold the records
-// of JOIN_PARTS parts side by side (a group's loads issued together), then one folds the parts into the row, in order.
+// A row of a call, its last position (as Tile::last) and whether it is the call's to write.
+__device__ __forceinline__ int row_of(const Kv4Attn &a, long row, int *s, int *tok, int *head) {
+  *head = (int)(row % a.nhead);
+  *tok = (int)(row / a.nhead % a.b.ntok);
+  *s = (int)(row / a.nhead / a.b.ntok);
+  if (*tok >= count_of(a.b, *s)) return ROW_ABSENT;
+  const int slot = slot_of(a.b, *s);
+  const long p = (long)a.b.pos[*s] + *tok;
+  return slot < 0 || slot >= a.c.nslot || p >= a.c.cap ? ROW_BAD : p < 0 ? ROW_NONE : (int)p;
+}
+
+// Rows of chunk records, few of them: a block per (row, 32 dimensions), a dimension per lane. Eight groups of 32 lanes fold the
+// chunks of a part each side by side (a group's loads issued together), then one folds the parts into the row, in order.
 constexpr int JOIN_PARTS = 32;
-template <int PER, int TYPE>
-__global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a) {
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_kv4_join_chunks(const Kv4Attn a) {
   __shared__ float po[JOIN_PARTS][32];
   __shared__ float2 pml[JOIN_PARTS];
-  constexpr int LEN = PART / PER;  // positions per record
-  const long row = blockIdx.x;
   const int fl = threadIdx.x & 31, grp = threadIdx.x >> 5, dim = blockIdx.y * 32 + fl;
-  const int head = (int)(row % a.nhead), tok = (int)(row / a.nhead % a.b.ntok), s = (int)(row / a.nhead / a.b.ntok);
-  const Tile tl(a, s, 0, 0);
-  const long last = (long)a.b.pos[s] + tok;
-  if (!tl.ok || tok >= tl.ntok || last < LEN || last >= a.c.cap) return;
-  const int nrec = (int)(last / LEN) + 1, np = (nrec + PER - 1) / PER;
-  const float *o = record_o(a, row, 0) + dim;
-  const float2 *ml = record_ml(a, row, 0);
+  int s, tok, head;
+  const int last = row_of(a, blockIdx.x, &s, &tok, &head);
+  if (last == ROW_ABSENT) return;
+  if (last < 0) {
+    if (grp == 0) emit<TYPE>(a, s, tok, head, dim, last == ROW_NONE ? 0.0f : NAN);
+    return;
+  }
+  const int nrec = last / CHUNK + 1, np = (nrec + CHUNKS - 1) / CHUNKS;
+  const float *o = record_o(a, blockIdx.x, 0) + dim;
+  const float2 *ml = record_ml(a, blockIdx.x, 0);
   Sum<1> f;
   f.clear();
   for (int b0 = 0; b0 < np; b0 += JOIN_PARTS) {
-    constexpr int R = JOIN_PARTS / 8;  // parts per group: grp, grp + 8, ...
-    float x[R][PER];
-    float2 v[R][PER];
-    #pragma unroll
-    for (int r = 0; r < R; r++)
+    for (int p = b0 + grp; p < min(b0 + JOIN_PARTS, np); p += 8) {
+      float x[CHUNKS][1];
+      float2 v[CHUNKS];
       #pragma unroll
-      for (int k = 0; k < PER; k++) {
-        const int c = min((b0 + grp + 8 * r) * PER + k, nrec - 1);
-        x[r][k] = o[(long)c * a.c.hd];
-        v[r][k] = ml[c];
+      for (int k = 0; k < CHUNKS; k++) {
+        const int c = min(p * CHUNKS + k, nrec - 1);
+        x[k][0] = o[(long)c * a.c.hd];
+        v[k] = ml[c];
       }
-    #pragma unroll
-    for (int r = 0; r < R; r++) {
-      Sum<1> u, p;
+      Sum<1> u;
       u.clear();
-      #pragma unroll
-      for (int k = 0; k < PER; k++) {
-        p.m = v[r][k].x;
-        p.l = v[r][k].y;
-        p.o[0] = x[r][k];
-        if ((b0 + grp + 8 * r) * PER + k < nrec) u.fold(p);
-      }
-      po[grp + 8 * r][fl] = u.o[0];
-      if (fl == 0) pml[grp + 8 * r] = make_float2(u.m, u.l);
+      fold_all<CHUNKS, 1>(u, v, x, nrec - p * CHUNKS);
+      po[p - b0][fl] = u.o[0];
+      if (fl == 0) pml[p - b0] = make_float2(u.m, u.l);
     }
     __syncthreads();
     if (grp == 0)
@@ -771,6 +754,36 @@ __global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a) {
     __syncthreads();
   }
   if (grp == 0) emit<TYPE>(a, s, tok, head, dim, f.o[0] / f.l);
+}
+
+// Rows of part records, many of them: 32 lanes per row.
+template <int NB, int TYPE>
+__global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a) {
+  const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int fl = threadIdx.x & 31;
+  if (row >= (long)a.b.nseq * a.b.ntok * a.nhead) return;
+  int s, tok, head;
+  const int last = row_of(a, row, &s, &tok, &head);
+  if (last == ROW_ABSENT) return;
+  Sum<NB> f;
+  f.clear();
+  const int nrec = last < 0 ? 0 : last / PART + 1;
+  const float *o = record_o(a, row, 0) + fl;
+  const float2 *ml = record_ml(a, row, 0);
+  for (int c0 = 0; c0 < nrec; c0 += 4) {
+    float2 v[4];
+    float x[4][NB];
+    #pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int c = min(c0 + k, nrec - 1);
+      v[k] = ml[c];
+      #pragma unroll
+      for (int i = 0; i < NB; i++) x[k][i] = o[(long)c * a.c.hd + 32 * i];
+    }
+    fold_all<4, NB>(f, v, x, nrec - c0);
+  }
+  #pragma unroll
+  for (int i = 0; i < NB; i++) emit<TYPE>(a, s, tok, head, 32 * i + fl, last >= 0 ? f.o[i] / f.l : last == ROW_NONE ? 0.0f : NAN);
 }
 
 // Many rows: a block takes four waves of RT tiles of 16 rows each through the spans of one part. The waves unpack a span's
@@ -796,9 +809,6 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) 
   for (int r = 0; r < RT; r++) {
     last[r] = tl.last(a, row0 + 16 * r + n, &tok[r], &head[r]);
     most = max(most, wave_max(last[r]));
-    if (part == 0 && (last[r] == ROW_NONE || last[r] == ROW_BAD))
-      for (int j = 0; j < 2 * NB; j++)
-        for (int v = 0; v < 4; v++) emit<TYPE>(a, tl.s, tok[r], head[r], 16 * j + 4 * g + v, last[r] == ROW_NONE ? 0.0f : NAN);
   }
   {
     int *red = (int *)lds_raw;
@@ -807,7 +817,14 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) 
     blockmost = max(max(red[0], red[1]), max(red[2], red[3]));
     __syncthreads();
   }
-  if (blockmost < part * PART) return;
+  Sum<8 * NB> f[RT], u[RT];
+  #pragma unroll
+  for (int r = 0; r < RT; r++) f[r].clear(), u[r].clear();
+  if (blockmost < part * PART) {
+    if (a.nrec == 1)
+      for (int r = 0; r < RT; r++) leave<NB, TYPE>(a, tl, last[r], tok[r], head[r], 0, 0, f[r], g);
+    return;
+  }
   typedef typename ValueOf<TYPE>::t T;
   uint32_t k1024 = 0x64006400u;
   __asm__("" : "+v"(k1024));
@@ -841,12 +858,9 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) 
   #pragma unroll
   for (int r = 0; r < RT; r++) {
     float qv[NB][8];
-    fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last[r] >= 0 ? tok[r] * a.q.tok + head[r] * a.q.head : 0), lane);
+    fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last[r] >= 0 ? tok[r] * a.q.tok + head[r] * a.q.head : 0), a.qvec, lane);
     set_queries<NB, TINY>(q[r], qv, a.scale);
   }
-  Sum<8 * NB> f[RT], u[RT];
-  #pragma unroll
-  for (int r = 0; r < RT; r++) f[r].clear(), u[r].clear();
   stage(buf[0]);
   load(min(1, nspan - 1));
   __syncthreads();
@@ -918,7 +932,7 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) 
         u[r].fold(z[r]);
       }
     }
-    if ((sp & (SPANS - 1)) == SPANS - 1 || sp == nspan - 1) {
+    if ((sp & (CHUNK / SPAN - 1)) == CHUNK / SPAN - 1 || sp == nspan - 1) {
       #pragma unroll
       for (int r = 0; r < RT; r++) {
         f[r].fold(u[r]);
@@ -932,21 +946,7 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) 
     __syncthreads();
   }
   #pragma unroll
-  for (int r = 0; r < RT; r++) {
-    if (last[r] < part * PART) continue;
-    if (last[r] < PART) {
-      #pragma unroll
-      for (int j = 0; j < 2 * NB; j++)
-        #pragma unroll
-        for (int v = 0; v < 4; v++) emit<TYPE>(a, tl.s, tok[r], head[r], 16 * j + 4 * g + v, f[r].o[4 * j + v] / f[r].l);
-    } else {
-      const long row = row_index(a, tl.s, tok[r], head[r]);
-      float *o = record_o(a, row, part);
-      #pragma unroll
-      for (int j = 0; j < 2 * NB; j++) *(float4 *)(o + 16 * j + 4 * g) = make_float4(f[r].o[4 * j], f[r].o[4 * j + 1], f[r].o[4 * j + 2], f[r].o[4 * j + 3]);
-      if (g == 0) *record_ml(a, row, part) = make_float2(f[r].m, f[r].l);
-    }
-  }
+  for (int r = 0; r < RT; r++) leave<NB, TYPE>(a, tl, last[r], tok[r], head[r], part, part * PART, f[r], g);
 }
 
 // Whether a call's rows fill the GPU with a wave per (tile, part).
@@ -968,23 +968,24 @@ static void launch_attention_k(Kv4Attn a, hipStream_t st) {
   const bool many = many_rows(a.c, a.b.nseq, a.b.ntok, a.nhead);
   const int group = a.nhead / a.c.nkv;
   a.nrec = record_count(a.c, many);
+  a.qvec = whole_pieces(a.q, TYPE);
   const long rows = (long)a.b.ntok * group;
   if (many) {
     constexpr int RT = parts_tiles(NB);
     const long nb = (rows + 64 * RT - 1) / (64 * RT);
     hipLaunchKernelGGL((k_kv4_parts<NB, TYPE, RT>), dim3(a.nrec, (unsigned)(nb * a.c.nkv), a.b.nseq), dim3(256), 2 * sizeof(SpanOperands<NB>), st, a, (int)nb);
   } else {
-    // as many blocks as stay resident (one per CU, two of heads of 64), each with an even share of the chunks
-    const int tiles = (int)((rows + 15) / 16), slots = NB <= 2 ? 512 : 256;
-    const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (a.nrec * y + slots - 1) / slots;
-    const int gx = (int)((a.nrec + rounds - 1) / rounds);
-    hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3(gx, tiles * a.c.nkv, a.b.nseq), dim3(64 * SPANS), chunk_lds<NB>((int)std::min(16L, rows)), st, a, tiles);
+    // waves of chunks up to two a SIMD, each with an even share of the chunks beyond
+    const int tiles = (int)((rows + 15) / 16);
+    const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (a.nrec * y + 2047) / 2048;
+    const int gx = (int)((a.nrec + 4 * rounds - 1) / (4 * rounds));
+    hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3(gx, tiles * a.c.nkv, a.b.nseq), dim3(256), 0, st, a, tiles);
   }
   ZL_HIP(hipGetLastError());
   if (a.nrec > 1) {
-    const dim3 grid((unsigned)(rows * a.c.nkv * a.b.nseq), NB);
-    if (many) hipLaunchKernelGGL((k_kv4_join<1, TYPE>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_kv4_join<CHUNKS, TYPE>), grid, dim3(256), 0, st, a);
+    const long n = rows * a.c.nkv * a.b.nseq;
+    if (many) hipLaunchKernelGGL((k_kv4_join_parts<NB, TYPE>), dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_kv4_join_chunks<TYPE>), dim3((unsigned)n, NB), dim3(256), 0, st, a);
     ZL_HIP(hipGetLastError());
   }
 }
@@ -992,7 +993,6 @@ static void launch_attention_k(Kv4Attn a, hipStream_t st) {
 // Dynamic LDS above 64 KB is requested per kernel, once per GPU, when a cache is created: no launch changes an attribute.
 template <int NB, int TYPE>
 static void prepare_k() {
-  ZL_HIP(hipFuncSetAttribute((const void *)k_kv4_chunks<NB, TYPE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_lds<NB>(16)));
   ZL_HIP(hipFuncSetAttribute((const void *)k_kv4_parts<NB, TYPE, parts_tiles(NB)>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * sizeof(SpanOperands<NB>))));
 }
 template <int NB>

@@ -67,7 +67,8 @@ struct Kv4Attn {
   int nhead;
   float scale;
   void *work;
-  int nrec;        // records per row in work (set by the launcher)
+  int nrec;        // records per row in work, and whether the queries are whole 16-byte pieces (set by the launcher)
+  bool qvec;
 };
 void kv4_prepare(int hd);  // once before launches of this head size
 long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead);
