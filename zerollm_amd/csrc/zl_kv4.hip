@@ -445,9 +445,9 @@ __device__ __forceinline__ f4 tile_scores(const K &k, const u4 (&ks)[NB], int t,
 }
 
 // Positions that the lane's row does not see (those behind lim of the span): no weight, ... (in spans at the rows' ends only:
-// the empty asm keeps the compiler from making selects of it that every span would pay for)
+// the empty asm, which lim depends on, keeps the compiler from making selects of it that every span would pay for)
 __device__ __forceinline__ void mask_scores(f4 (&s)[2][2], int lim, int g) {
-  __asm__ volatile("");
+  __asm__ volatile("" : "+v"(lim));
   #pragma unroll
   for (int i = 0; i < 2; i++)
     #pragma unroll
@@ -458,7 +458,7 @@ __device__ __forceinline__ void mask_scores(f4 (&s)[2][2], int lim, int g) {
 // ... and a scale of 0 (a stale one may be NaN): record i's value scales.
 template <int NB>
 __device__ __forceinline__ void mask_scales(u4 (&vs)[NB], int i, int lim, int g) {
-  __asm__ volatile("");
+  __asm__ volatile("" : "+v"(lim));
   #pragma unroll
   for (int t = 0; t < 2; t++) {
     const int n = lim - 32 * i - 16 * t - 4 * g;  // the last of the lane's four positions that is seen
@@ -581,6 +581,12 @@ __device__ __forceinline__ void take_off(f4 (&o)[2 * NB], const f4 (&wsum)[NB]) 
     for (int v = 0; v < 4; v++) o[j][v] = fmaf(o[j][v], TINY_ONE, -8.0f * wsum[j >> 1][v]);
 }
 
+// Positions per record of a sequence's rows (of k_kv4_chunks): by the sequence's last position, so that all its rows agree.
+__device__ __forceinline__ int record_len(const Kv4Attn &a, int s) {
+  const long last = min((long)a.b.pos[s] + count_of(a.b, s), a.c.cap) - 1;
+  return last < (long)a.spanmax * SPAN ? SPAN : CHUNK;
+}
+
 // A tile's finished sums: the rows' outputs where a call has one record per row, else record `rec` of the rows that see it. Lane
 // l has row l % 16, dimensions 16 j + 4 (l / 16) + v.
 template <int NB, int TYPE>
@@ -603,7 +609,8 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 }
 
 // Few rows: a wave takes one tile of 16 rows and a chunk at a time, span by span, and leaves the chunk's record; no wave waits
-// for another. The next span's keys are requested when the scores are done with this one's, its values after the weighted
+// for another. Sequences of so few spans that a wave for each does not overfill the GPU (a.spanmax, by the call's tiles) leave
+// a record per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 9). The next span's keys are requested when the scores are done with this one's, its values after the weighted
 // sums, so that the loads run under the rest. (A chunk of 512 per block, one span per wave, folded in LDS behind a barrier:
 // decode_131k 47 us against 27, the waves waiting for each other and for the fold.)
 template <int NB, int TYPE>
@@ -615,9 +622,10 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
   int tok, head;
   const int last = tl.last(a, n, &tok, &head);
   const int most = __builtin_amdgcn_readfirstlane(wave_max(last)), c0 = blockIdx.x * 4 + wave, step = gridDim.x * 4;
+  const int unit = record_len(a, tl.s);
   Sum<8 * NB> u;
   u.clear();
-  if (most < c0 * CHUNK) {
+  if (most < (long)c0 * unit) {
     if (a.nrec == 1 && c0 == 0) leave<NB, TYPE>(a, tl, last, tok, head, 0, 0, u, g);
     return;
   }
@@ -630,18 +638,18 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
   {
     float qv[NB][8];
     fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.qvec, lane);
-    const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, (long)c0 * (CHUNK / KV4_GROUP));
+    const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, (long)c0 * (unit / KV4_GROUP));
     w.load_keys(rec, lane);
     if (AHEAD) w.load_values(rec, lane);
     __builtin_amdgcn_sched_barrier(0);
     set_queries<NB, TINY>(q, qv, a.scale);
   }
-  for (int c = c0; c * CHUNK <= most; c += step) {
-    const int ns = min(CHUNK / SPAN, (most - c * CHUNK) / SPAN + 1);
+  for (int c = c0; (long)c * unit <= most; c += step) {
+    const int ns = min(unit / SPAN, (most - c * unit) / SPAN + 1);
     u.clear();
     for (int sp = 0; sp < ns; sp++) {
-      const int p0 = c * CHUNK + sp * SPAN, lim = last - p0;
-      const int pn = sp + 1 < ns ? p0 + SPAN : (c + step) * CHUNK <= most ? (c + step) * CHUNK : p0;  // (the last one is read again, for nothing)
+      const int p0 = c * unit + sp * SPAN, lim = last - p0;
+      const int pn = sp + 1 < ns ? p0 + SPAN : (long)(c + step) * unit <= most ? (c + step) * unit : p0;  // (the last one is read again, for nothing)
       const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, p0 / KV4_GROUP), *next = record_of(a.c, tl.slot, tl.kvh, pn / KV4_GROUP);
       const bool masked = __ballot(lim < SPAN - 1) != 0;
       f4 s[2][2];
@@ -688,7 +696,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
         for (int v = 0; v < 4; v++) r.o[4 * j + v] = o[j][v];
       u.fold(r);
     }
-    leave<NB, TYPE>(a, tl, last, tok, head, c, c * CHUNK, u, g);
+    leave<NB, TYPE>(a, tl, last, tok, head, c, c * unit, u, g);
   }
 }
 
@@ -703,11 +711,11 @@ __device__ __forceinline__ int row_of(const Kv4Attn &a, long row, int *s, int *t
   return slot < 0 || slot >= a.c.nslot || p >= a.c.cap ? ROW_BAD : p < 0 ? ROW_NONE : (int)p;
 }
 
-// Rows of chunk records, few of them: a block per (row, 32 dimensions), a dimension per lane. Eight groups of 32 lanes fold the
-// chunks of a part each side by side (a group's loads issued together), then one folds the parts into the row, in order.
+// Rows of chunk or span records, few of them: a block per (row, 32 dimensions), a dimension per lane. Its groups of 32 lanes fold
+// the chunks of a part each side by side (a group's loads issued together), then one folds the parts into the row, in order.
 constexpr int JOIN_PARTS = 32;
-template <int TYPE>
-__global__ __launch_bounds__(256) void k_kv4_join_chunks(const Kv4Attn a) {
+template <int TYPE, int GROUPS>
+__global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a) {
   __shared__ float po[JOIN_PARTS][32];
   __shared__ float2 pml[JOIN_PARTS];
   const int fl = threadIdx.x & 31, grp = threadIdx.x >> 5, dim = blockIdx.y * 32 + fl;
@@ -718,24 +726,48 @@ __global__ __launch_bounds__(256) void k_kv4_join_chunks(const Kv4Attn a) {
     if (grp == 0) emit<TYPE>(a, s, tok, head, dim, last == ROW_NONE ? 0.0f : NAN);
     return;
   }
-  const int nrec = last / CHUNK + 1, np = (nrec + CHUNKS - 1) / CHUNKS;
+  const int len = record_len(a, s), nrec = last / len + 1, per = len == SPAN ? CHUNK / SPAN : 1;  // records per chunk
+  const int np = last / PART + 1;
   const float *o = record_o(a, blockIdx.x, 0) + dim;
   const float2 *ml = record_ml(a, blockIdx.x, 0);
   Sum<1> f;
   f.clear();
   for (int b0 = 0; b0 < np; b0 += JOIN_PARTS) {
-    for (int p = b0 + grp; p < min(b0 + JOIN_PARTS, np); p += 8) {
-      float x[CHUNKS][1];
-      float2 v[CHUNKS];
-      #pragma unroll
-      for (int k = 0; k < CHUNKS; k++) {
-        const int c = min(p * CHUNKS + k, nrec - 1);
-        x[k][0] = o[(long)c * a.c.hd];
-        v[k] = ml[c];
-      }
+    for (int p = b0 + grp; p < min(b0 + JOIN_PARTS, np); p += GROUPS) {
       Sum<1> u;
       u.clear();
-      fold_all<CHUNKS, 1>(u, v, x, nrec - p * CHUNKS);
+      for (int j = 0; j < per; j++) {  // chunk records: all eight of a part; span records: two chunks' at a time
+        float x[CHUNKS][1];
+        float2 v[CHUNKS];
+        const int r0 = (p * per + j) * CHUNKS;
+        if (r0 >= nrec) break;
+        #pragma unroll
+        for (int k = 0; k < CHUNKS; k++) {
+          const int c = min(r0 + k, nrec - 1);
+          x[k][0] = o[(long)c * a.c.hd];
+          v[k] = ml[c];
+        }
+        if (per == 1) {
+          fold_all<CHUNKS, 1>(u, v, x, nrec - r0);
+        } else {
+          #pragma unroll
+          for (int h = 0; h < CHUNKS; h += CHUNK / SPAN) {
+            float y[CHUNK / SPAN][1];
+            float2 w[CHUNK / SPAN];
+            #pragma unroll
+            for (int k = 0; k < CHUNK / SPAN; k++) {
+              y[k][0] = x[h + k][0];
+              w[k] = v[h + k];
+            }
+            Sum<1> c;
+            c.clear();
+            if (r0 + h < nrec) {
+              fold_all<CHUNK / SPAN, 1>(c, w, y, nrec - r0 - h);
+              u.fold(c);
+            }
+          }
+        }
+      }
       po[p - b0][fl] = u.o[0];
       if (fl == 0) pml[p - b0] = make_float2(u.m, u.l);
     }
@@ -796,7 +828,7 @@ struct SpanOperands {
   u4 ks[2][4 * NB], vs[2][4 * NB];        // the records' scales as they are
 };
 template <int NB, int TYPE, int RT>
-__global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) {
+__global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_parts(const Kv4Attn a, int blocks) {
   constexpr int HD = 32 * NB, REC = 36 * HD, NW = 2 * NB / 4;  // NW: 16-byte loads of a lane per wave (of 8 per record pair and NB / 2)
   constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ;
   extern __shared__ __align__(16) uint8_t lds_raw[];
@@ -949,25 +981,30 @@ __global__ __launch_bounds__(256) void k_kv4_parts(const Kv4Attn a, int blocks) 
   for (int r = 0; r < RT; r++) leave<NB, TYPE>(a, tl, last[r], tok[r], head[r], part, part * PART, f[r], g);
 }
 
+// Tiles of 16 rows times KV heads times sequences.
+static long tile_count(const Kv4View &c, int nseq, int ntok, int nhead) { return ((long)ntok * (nhead / c.nkv) + 15) / 16 * c.nkv * nseq; }
 // Whether a call's rows fill the GPU with a wave per (tile, part).
-static bool many_rows(const Kv4View &c, int nseq, int ntok, int nhead) {
-  const long tiles = ((long)ntok * (nhead / c.nkv) + 15) / 16 * c.nkv * nseq;
-  return tiles >= 128;
+static bool many_rows(const Kv4View &c, int nseq, int ntok, int nhead) { return tile_count(c, nseq, ntok, nhead) >= 128; }
+// Spans of a sequence up to which its rows have a record per span: as many as give about two waves a SIMD.
+static int span_max(const Kv4View &c, long tiles) { return (int)std::min((c.cap + SPAN - 1) / SPAN, 2048 / tiles); }
+static int record_count(const Kv4View &c, int nseq, int ntok, int nhead) {
+  if (many_rows(c, nseq, ntok, nhead)) return (int)((c.cap + PART - 1) / PART);
+  return (int)std::max((c.cap + CHUNK - 1) / CHUNK, (long)span_max(c, tile_count(c, nseq, ntok, nhead)));
 }
-static int record_count(const Kv4View &c, bool many) { return (int)((c.cap + (many ? PART : CHUNK) - 1) / (many ? PART : CHUNK)); }
 
 long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead) {
-  const long rows = (long)nseq * ntok * nhead, rec = record_count(c, many_rows(c, nseq, ntok, nhead));
-  return std::max(16L, rows * rec * (c.hd + 2) * 4);
+  if (nseq == 0 || ntok == 0) return 16;
+  return std::max(16L, (long)nseq * ntok * nhead * record_count(c, nseq, ntok, nhead) * (c.hd + 2) * 4);
 }
 
-constexpr int parts_tiles(int nb) { return nb <= 4 ? 2 : 1; }  // RT: row tiles per wave (heads of 256: registers for one)
+constexpr int parts_tiles(int nb) { return 1; }
 
 template <int NB, int TYPE>
 static void launch_attention_k(Kv4Attn a, hipStream_t st) {
   const bool many = many_rows(a.c, a.b.nseq, a.b.ntok, a.nhead);
   const int group = a.nhead / a.c.nkv;
-  a.nrec = record_count(a.c, many);
+  a.nrec = record_count(a.c, a.b.nseq, a.b.ntok, a.nhead);
+  a.spanmax = many ? 0 : span_max(a.c, tile_count(a.c, a.b.nseq, a.b.ntok, a.nhead));
   a.qvec = whole_pieces(a.q, TYPE);
   const long rows = (long)a.b.ntok * group;
   if (many) {
@@ -975,17 +1012,18 @@ static void launch_attention_k(Kv4Attn a, hipStream_t st) {
     const long nb = (rows + 64 * RT - 1) / (64 * RT);
     hipLaunchKernelGGL((k_kv4_parts<NB, TYPE, RT>), dim3(a.nrec, (unsigned)(nb * a.c.nkv), a.b.nseq), dim3(256), 2 * sizeof(SpanOperands<NB>), st, a, (int)nb);
   } else {
-    // waves of chunks up to two a SIMD, each with an even share of the chunks beyond
-    const int tiles = (int)((rows + 15) / 16);
-    const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (a.nrec * y + 2047) / 2048;
-    const int gx = (int)((a.nrec + 4 * rounds - 1) / (4 * rounds));
+    // waves of chunks up to two a SIMD, each with an even share of the chunks beyond; or of spans
+    const int tiles = (int)((rows + 15) / 16), nch = (int)((a.c.cap + CHUNK - 1) / CHUNK);
+    const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (nch * y + 2047) / 2048;
+    const int gx = std::max((int)((nch + 4 * rounds - 1) / (4 * rounds)), (a.spanmax + 3) / 4);
     hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3(gx, tiles * a.c.nkv, a.b.nseq), dim3(256), 0, st, a, tiles);
   }
   ZL_HIP(hipGetLastError());
   if (a.nrec > 1) {
     const long n = rows * a.c.nkv * a.b.nseq;
     if (many) hipLaunchKernelGGL((k_kv4_join_parts<NB, TYPE>), dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_kv4_join_chunks<TYPE>), dim3((unsigned)n, NB), dim3(256), 0, st, a);
+    else if (a.c.cap > 16 * PART) hipLaunchKernelGGL((k_kv4_join_chunks<TYPE, 32>), dim3((unsigned)n, NB), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((k_kv4_join_chunks<TYPE, 8>), dim3((unsigned)n, NB), dim3(256), 0, st, a);
     ZL_HIP(hipGetLastError());
   }
 }

@@ -67,7 +67,9 @@ struct Kv4Attn {
   int nhead;
   float scale;
   void *work;
-  int nrec;        // records per row in work, and whether the queries are whole 16-byte pieces (set by the launcher)
+  // set by the launcher: records per row in work, spans of a sequence up to which they are spans', whether the queries are whole
+  // 16-byte pieces
+  int nrec, spanmax;
   bool qvec;
 };
 void kv4_prepare(int hd);  // once before launches of this head size
