@@ -232,9 +232,9 @@ void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows 
 // Products run on the matrix cores (v_mfma_f32_16x16x32_f16) for 16 rows at a time: keys times queries first, which leaves
 // lane l with the scores of row l % 16 at four neighbouring positions, then values (as the left operand) times weights,
 // which takes those positions as they lie. Codes less 8 are exact in f16. Queries are scaled per row by a power of two to
-// below 2^14 and split into two f16 parts (22 bits, or all the bits of 16-bit queries); a weight times its value's scale
-// likewise where the output is f32 or f16 (a single f16 part would add an error as large as the rounding of an f16
-// output). Scores are scaled by their key's scale in f32, block by block.
+// below 2^14 and split into two f16 parts (22 bits; 16-bit queries need one); a weight times its value's scale likewise where
+// the output is f32 or f16: rounded to one f16 part, and the product again, it would be off by 2^-11 twice, more than the
+// rounding of an f16 output (3.4e-4 of the output together, against 2.0e-4). bf16 outputs are rounded by 2^-8, and have one. Scores are scaled by their key's scale in f32, block by block.
 constexpr int SPAN = 64, CHUNK = 256, PART = 2048;
 constexpr int CHUNKS = PART / CHUNK;
 
@@ -300,9 +300,8 @@ struct Sum {
     #pragma unroll
     for (int i = 0; i < N; i++) o[i] = 0.0f;
   }
-  // (a piece that saw nothing leaves the sum as it is; one of NaN has l NaN)
+  // (a piece that saw nothing has m = -inf and l = o = 0, and adds 0; one of NaN has l NaN)
   __device__ __forceinline__ void fold(const Sum &p) {
-    if (p.m == -INFINITY && p.l == 0.0f) return;
     const float M = fmaxf(m, p.m), r = M == -INFINITY ? 0.0f : M, a = exp2_(m - r), b = exp2_(p.m - r);
     m = M;
     l = fmaf(l, a, p.l * b);
@@ -315,35 +314,20 @@ struct Sum {
 template <int K, int N>
 __device__ __forceinline__ void fold_all(Sum<N> &f, const float2 (&ml)[K], const float (&o)[K][N], int n) {
   float M = f.m, a[K], b[K];
-  bool every = n >= K;  // all of them, none empty: no selects
   #pragma unroll
-  for (int k = 0; k < K; k++) every = every && ml[k].x > -INFINITY;
-  if (every) {
-    #pragma unroll
-    for (int k = 0; k < K; k++) {
-      const float to = fmaxf(M, ml[k].x);
-      a[k] = exp2_(M - to);
-      b[k] = exp2_(ml[k].x - to);
-      M = to;
-    }
-    f.m = M;
-    #pragma unroll
-    for (int k = 0; k < K; k++) {
-      f.l = fmaf(f.l, a[k], ml[k].y * b[k]);
-      #pragma unroll
-      for (int i = 0; i < N; i++) f.o[i] = fmaf(f.o[i], a[k], o[k][i] * b[k]);
-    }
-    return;
-  }
   for (int k = 0; k < K; k++) {
-    __asm__ volatile("");
+    const float to = fmaxf(M, k < n ? ml[k].x : -INFINITY), r = to == -INFINITY ? 0.0f : to;
+    a[k] = exp2_(M - r);
+    b[k] = exp2_(ml[k].x - r);
+    M = to;
+  }
+  f.m = M;
+  #pragma unroll
+  for (int k = 0; k < K; k++) {
     if (k >= n) break;
-    Sum<N> p;
-    p.m = ml[k].x;
-    p.l = ml[k].y;
+    f.l = fmaf(f.l, a[k], ml[k].y * b[k]);
     #pragma unroll
-    for (int i = 0; i < N; i++) p.o[i] = o[k][i];
-    f.fold(p);
+    for (int i = 0; i < N; i++) f.o[i] = fmaf(f.o[i], a[k], o[k][i] * b[k]);
   }
 }
 
@@ -557,7 +541,8 @@ __device__ __forceinline__ float2 *record_ml(const Kv4Attn &a, long row, int rec
 template <int TYPE>
 __device__ __forceinline__ void emit(const Kv4Attn &a, int s, int tok, int head, int dim, float o) {
   typedef typename ValueOf<TYPE>::t T;
-  ((T *)a.out.p)[s * a.out.seq + tok * a.out.tok + head * a.out.head + dim] = store_value<TYPE>(o);
+  // (+ 0: a sum of -0 comes out the same whether it was folded with empty pieces or not)
+  ((T *)a.out.p)[s * a.out.seq + tok * a.out.tok + head * a.out.head + dim] = store_value<TYPE>(o + 0.0f);
 }
 
 // A span's two products of block b and record: values times weights, and with TINY the weights' sums.
@@ -578,7 +563,7 @@ __device__ __forceinline__ void take_off(f4 (&o)[2 * NB], const f4 (&wsum)[NB]) 
   #pragma unroll
   for (int j = 0; j < 2 * NB; j++)
     #pragma unroll
-    for (int v = 0; v < 4; v++) o[j][v] = fmaf(o[j][v], TINY_ONE, -8.0f * wsum[j >> 1][v]);
+    for (int v = 0; v < 4; v++) o[j][v] = fmaf(o[j][v], TINY_ONE, -8.0f * wsum[j >> 1][0]);  // (all rows of wsum are the same)
 }
 
 // Positions per record of a sequence's rows (of k_kv4_chunks): by the sequence's last position, so that all its rows agree.
@@ -818,8 +803,8 @@ __global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a) {
   for (int i = 0; i < NB; i++) emit<TYPE>(a, s, tok, head, 32 * i + fl, last >= 0 ? f.o[i] / f.l : last == ROW_NONE ? 0.0f : NAN);
 }
 
-// Many rows: a block takes four waves of RT tiles of 16 rows each through the spans of one part. The waves unpack a span's
-// codes to f16 operands in LDS, a quarter each, and read all of them, so that a span is unpacked once for 64 RT rows; the
+// Many rows: a block takes PW waves of a tile of 16 rows each through the spans of one part. The waves unpack a span's
+// codes to f16 operands in LDS, a share each, and read all of them, so that a span is unpacked once for 16 PW rows; the
 // next span's words are on their way meanwhile, and two buffers let the block meet once per span. A wave folds its rows'
 // spans, chunks and part in registers; the parts' records are joined.
 template <int NB>
@@ -827,14 +812,15 @@ struct SpanOperands {
   h8 k[2][2 * NB][64], v[2][2 * NB][64];  // [record][word][lane]
   u4 ks[2][4 * NB], vs[2][4 * NB];        // the records' scales as they are
 };
-template <int NB, int TYPE, int RT>
-__global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_parts(const Kv4Attn a, int blocks) {
-  constexpr int HD = 32 * NB, REC = 36 * HD, NW = 2 * NB / 4;  // NW: 16-byte loads of a lane per wave (of 8 per record pair and NB / 2)
+constexpr int part_waves(int nb) { return nb <= 4 ? 8 : 4; }  // (heads of 256: registers for one wave a SIMD)
+template <int NB, int TYPE>
+__global__ __launch_bounds__(64 * part_waves(NB)) void k_kv4_parts(const Kv4Attn a, int blocks) {
+  constexpr int HD = 32 * NB, REC = 36 * HD, RT = 1, PW = part_waves(NB), NW = 2 * NB / PW > 0 ? 2 * NB / PW : 1;  // NW: a lane's 16-byte loads of words
   constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ;
   extern __shared__ __align__(16) uint8_t lds_raw[];
   SpanOperands<NB> *buf = (SpanOperands<NB> *)lds_raw;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4, part = blockIdx.x;
-  const int row0 = blockIdx.y % blocks * (64 * RT) + wave * (16 * RT);
+  const int row0 = blockIdx.y % blocks * (16 * PW) + wave * (16 * RT);
   int last[RT], tok[RT], head[RT], most = ROW_ABSENT, blockmost;
   const Tile tl(a, blockIdx.z, blockIdx.y / blocks, 0);
   #pragma unroll
@@ -846,7 +832,8 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_parts(const Kv4Att
     int *red = (int *)lds_raw;
     if (lane == 0) red[wave] = most;
     __syncthreads();
-    blockmost = max(max(red[0], red[1]), max(red[2], red[3]));
+    blockmost = red[0];
+    for (int w = 1; w < PW; w++) blockmost = max(blockmost, red[w]);
     __syncthreads();
   }
   Sum<8 * NB> f[RT], u[RT];
@@ -860,7 +847,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_parts(const Kv4Att
   typedef typename ValueOf<TYPE>::t T;
   uint32_t k1024 = 0x64006400u;
   __asm__("" : "+v"(k1024));
-  // the wave's quarter of a span: records' key words then value words, NW 16-byte loads (of NB / 2 per record and kind)
+  // the wave's share of a span: records' key words then value words, NW 16-byte loads (of NB / 2 per record and kind)
   const int npos = min(blockmost + 1, (part + 1) * PART), nspan = (npos - part * PART + SPAN - 1) / SPAN;
   const uint8_t *base = record_of(a.c, tl.slot, tl.kvh, (long)part * (PART / KV4_GROUP));
   u4 words[NW], scales;
@@ -869,6 +856,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_parts(const Kv4Att
     #pragma unroll
     for (int x = 0; x < NW; x++) {
       const int idx = wave * NW + x, i = idx / NB, kv = idx / (NB / 2) & 1, j = idx % (NB / 2);
+      if (idx >= 2 * NB) break;
       words[x] = ((const u4 *)(rec + i * REC + kv * 16 * HD))[j * 64 + lane];
     }
     // 16 NB pieces of scales: [record][keys | values][4 NB]
@@ -879,6 +867,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_parts(const Kv4Att
     #pragma unroll
     for (int x = 0; x < NW; x++) {
       const int idx = wave * NW + x, i = idx / NB, kv = idx / (NB / 2) & 1, j = idx % (NB / 2);
+      if (idx >= 2 * NB) break;
       #pragma unroll
       for (int y = 0; y < 4; y++) (kv ? d.v : d.k)[i][4 * j + y][lane] = unpack8<TINY>(words[x][y], k1024);
     }
@@ -997,8 +986,6 @@ long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead) {
   return std::max(16L, (long)nseq * ntok * nhead * record_count(c, nseq, ntok, nhead) * (c.hd + 2) * 4);
 }
 
-constexpr int parts_tiles(int nb) { return 1; }
-
 template <int NB, int TYPE>
 static void launch_attention_k(Kv4Attn a, hipStream_t st) {
   const bool many = many_rows(a.c, a.b.nseq, a.b.ntok, a.nhead);
@@ -1008,9 +995,9 @@ static void launch_attention_k(Kv4Attn a, hipStream_t st) {
   a.qvec = whole_pieces(a.q, TYPE);
   const long rows = (long)a.b.ntok * group;
   if (many) {
-    constexpr int RT = parts_tiles(NB);
-    const long nb = (rows + 64 * RT - 1) / (64 * RT);
-    hipLaunchKernelGGL((k_kv4_parts<NB, TYPE, RT>), dim3(a.nrec, (unsigned)(nb * a.c.nkv), a.b.nseq), dim3(256), 2 * sizeof(SpanOperands<NB>), st, a, (int)nb);
+    constexpr int PW = part_waves(NB);
+    const long nb = (rows + 16 * PW - 1) / (16 * PW);
+    hipLaunchKernelGGL((k_kv4_parts<NB, TYPE>), dim3(a.nrec, (unsigned)(nb * a.c.nkv), a.b.nseq), dim3(64 * PW), 2 * sizeof(SpanOperands<NB>), st, a, (int)nb);
   } else {
     // waves of chunks up to two a SIMD, each with an even share of the chunks beyond; or of spans
     const int tiles = (int)((rows + 15) / 16), nch = (int)((a.c.cap + CHUNK - 1) / CHUNK);
@@ -1031,7 +1018,7 @@ static void launch_attention_k(Kv4Attn a, hipStream_t st) {
 // Dynamic LDS above 64 KB is requested per kernel, once per GPU, when a cache is created: no launch changes an attribute.
 template <int NB, int TYPE>
 static void prepare_k() {
-  ZL_HIP(hipFuncSetAttribute((const void *)k_kv4_parts<NB, TYPE, parts_tiles(NB)>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * sizeof(SpanOperands<NB>))));
+  ZL_HIP(hipFuncSetAttribute((const void *)k_kv4_parts<NB, TYPE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * sizeof(SpanOperands<NB>))));
 }
 template <int NB>
 static void prepare_nb() {
