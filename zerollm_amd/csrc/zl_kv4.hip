@@ -222,10 +222,11 @@ void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows 
 
 // ---------------------------------------------------------------------------------------------- attention
 // softmax(scale q K) V of a row (a token's query head) over positions 0 .. last, in f32 with the exponentials to base 2. The
-// positions are cut, by their index alone, into spans of 64, chunks of 256 (4 spans) and parts of 2048 (8 chunks). A span has
+// positions are cut, by their index alone, into spans of 64, chunks of 256 (4 spans) and parts of 1024 (4 chunks). A span has
 // a softmax of its own: its reference m (the largest score less 3, so that weights reach 8), l = sum of weights and
-// o = sum of weights times values. Spans are folded into their chunk in order, chunks into their part, parts into the row:
+// o = sum of weights times values. Spans are folded into their chunk in order, chunks into their part:
 //   M' = max(M, m), L = L 2^(M - M') + l 2^(m - M'), O = O 2^(M - M') + o 2^(m - M').
+// Parts are joined into the row (JOIN_PARTS).
 // Whichever block or kernel forms a piece, it does these operations, so a row has the same bits in a batch of any size and
 // in a cache of any capacity.
 //
@@ -235,7 +236,7 @@ void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows 
 // below 2^14 and split into two f16 parts (22 bits; 16-bit queries need one); a weight times its value's scale likewise where
 // the output is f32 or f16: rounded to one f16 part, and the product again, it would be off by 2^-11 twice, more than the
 // rounding of an f16 output (3.4e-4 of the output together, against 2.0e-4). bf16 outputs are rounded by 2^-8, and have one. Scores are scaled by their key's scale in f32, block by block.
-constexpr int SPAN = 64, CHUNK = 256, PART = 2048;
+constexpr int SPAN = 64, CHUNK = 256, PART = 1024;
 constexpr int CHUNKS = PART / CHUNK;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -247,20 +248,25 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 // TINY: as they lie, f16 denormals of code 2^-24, which the matrix cores take (16 cycles of a SIMD a word); the 2^24 and the
 // 8 to be taken off follow the sums. Sums of codes are larger than sums of codes less 8, and they lose bits: 7e-6 of an output
 // against 2e-7, so this is for 16-bit rows, whose own rounding is 30 times that.
-// Else: less 8, under the exponent of 1024 and less 1032 (40 cycles a word). k: 0x64006400 in a vector register, so that and
-// and or are one instruction (which takes a single scalar operand).
+// Else: less 8, under the exponent of 1024 and less 1032 (40 cycles a word).
+// The constants are in vector registers: a 32-bit operation takes 2 cycles of a SIMD from two waves' vector operands and 4 with a
+// scalar one, and and-or takes a single scalar one.
+struct Unpack {
+  uint32_t mask = 0x000f000fu, k1024 = 0x64006400u;
+  __device__ __forceinline__ Unpack() { __asm__("" : "+v"(mask), "+v"(k1024)); }
+};
 template <bool TINY>
-__device__ __forceinline__ h8 unpack8(uint32_t w, uint32_t k) {
+__device__ __forceinline__ h8 unpack8(uint32_t w, const Unpack &k) {
   if constexpr (TINY) {
     u4 x;
     #pragma unroll
-    for (int r = 0; r < 4; r++) x[r] = (w >> (4 * r)) & 0x000f000fu;
+    for (int r = 0; r < 4; r++) x[r] = (w >> (4 * r)) & k.mask;
     return __builtin_bit_cast(h8, x);
   }
   h8 x;
   #pragma unroll
   for (int r = 0; r < 4; r++) {
-    const h2 p = __builtin_bit_cast(h2, ((w >> (4 * r)) & 0x000f000fu) | k) - (h2){1032, 1032};
+    const h2 p = __builtin_bit_cast(h2, ((w >> (4 * r)) & k.mask) | k.k1024) - (h2){1032, 1032};
     x[2 * r] = p[0];
     x[2 * r + 1] = p[1];
   }
@@ -510,6 +516,16 @@ __device__ __forceinline__ void weigh(const Weights<LOW> &w, const u4 (&vs)[NB],
   }
 }
 
+// Blocks of a one-dimensional grid, which the GPU deals to its 8 XCDs in turn: `groups` of n blocks that read the same records, each
+// on one XCD, whose L2 then holds them.
+__host__ __device__ inline long deal_blocks(long groups, int n) { return (groups + 7) / 8 * 8 * n; }
+__device__ __forceinline__ bool dealt(long groups, int n, long *group, int *i) {
+  const long j = blockIdx.x >> 3;
+  *i = (int)(j % n);
+  *group = j / n * 8 + (blockIdx.x & 7);
+  return *group < groups;
+}
+
 // The rows of a block: tile t of KV head kvh of sequence s. A row's last position; below 0 it sees nothing.
 constexpr int ROW_NONE = -1, ROW_BAD = -2, ROW_ABSENT = -3;
 struct Tile {
@@ -595,18 +611,24 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 
 // Few rows: a wave takes one tile of 16 rows and a chunk at a time, span by span, and leaves the chunk's record; no wave waits
 // for another. Sequences of so few spans that a wave for each does not overfill the GPU (a.spanmax, by the call's tiles) leave
-// a record per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 9). The next span's keys are requested when the scores are done with this one's, its values after the weighted
-// sums, so that the loads run under the rest. (A chunk of 512 per block, one span per wave, folded in LDS behind a barrier:
-// decode_131k 47 us against 27, the waves waiting for each other and for the fold.)
+// a record per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 8.5). The next
+// span's keys are requested when the scores are done with this one's, its values after the weighted sums, so that the loads run
+// under the rest. (A chunk of 512 per block, one span per wave, folded in LDS behind a barrier: 9 tokens of 32 heads after 16384
+// positions took 48 us against 41, the waves waiting for each other and for the fold.) A token
+// of 32 heads of 128 over 8 KV heads after 131000 positions: 44 us, 151 MB at 3.4 TB/s, near a read's own rate (4.1). 9 tokens after
+// 16384: 27 us, bound by the vector units and by the waves' start and end.
 template <int NB, int TYPE>
-__global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4Attn a, int tiles) {
+__global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
   constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
-  const Tile tl(a, blockIdx.z, blockIdx.y / tiles, blockIdx.y % tiles * 16);
+  long group;  // [sequence][KV head][block of chunks]
+  int tile;
+  if (!dealt((long)gx * a.c.nkv * a.b.nseq, tiles, &group, &tile)) return;
+  const Tile tl(a, (int)(group / gx / a.c.nkv), (int)(group / gx % a.c.nkv), tile * 16);
   int tok, head;
   const int last = tl.last(a, n, &tok, &head);
-  const int most = __builtin_amdgcn_readfirstlane(wave_max(last)), c0 = blockIdx.x * 4 + wave, step = gridDim.x * 4;
+  const int most = __builtin_amdgcn_readfirstlane(wave_max(last)), c0 = (int)(group % gx) * 4 + wave, step = gx * 4;
   const int unit = record_len(a, tl.s);
   Sum<8 * NB> u;
   u.clear();
@@ -615,8 +637,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
     return;
   }
   typedef typename ValueOf<TYPE>::t T;
-  uint32_t k1024 = 0x64006400u;
-  __asm__("" : "+v"(k1024));
+  const Unpack uk;
   // (loads complete in order: the queries, which take a while to prepare, are requested first)
   SpanWords<NB> w;
   Queries<NB, TINY> q;
@@ -642,7 +663,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
       for (int i = 0; i < 2; i++)
         #pragma unroll
         for (int t = 0; t < 2; t++) {
-          s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], k1024); }, w.ks[i], t, q);
+          s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], uk); }, w.ks[i], t, q);
           __builtin_amdgcn_sched_barrier(0);
         }
       if (AHEAD) w.load_keys(next, lane);
@@ -667,7 +688,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
         for (int b = 0; b < NB; b++) {
           h8 hi, lo;
           weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
-          const h8 x0 = unpack8<TINY>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], k1024), x1 = unpack8<TINY>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], k1024);
+          const h8 x0 = unpack8<TINY>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<TINY>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
           weighted_sums<LOW, TINY>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -696,13 +717,19 @@ __device__ __forceinline__ int row_of(const Kv4Attn &a, long row, int *s, int *t
   return slot < 0 || slot >= a.c.nslot || p >= a.c.cap ? ROW_BAD : p < 0 ? ROW_NONE : (int)p;
 }
 
-// Rows of chunk or span records, few of them: a block per (row, 32 dimensions), a dimension per lane. Its groups of 32 lanes fold
-// the chunks of a part each side by side (a group's loads issued together), then one folds the parts into the row, in order.
-constexpr int JOIN_PARTS = 32;
+// Parts to a row: up to 128 of them (131072 positions) side by side, weighted by 2^(m - M) of their largest M and summed into eight
+// sums by their index, which are added in order; such sums are folded one after the other.
+constexpr int JOIN_PARTS = 128, JOIN_SUMS = 8;
+
+// Rows of chunk or span records, few of them: a block per (row, 32 dimensions), a dimension per lane. Its groups of 32 lanes fold the
+// chunks of a part each, the loads of AT parts issued together, and eight of them sum the parts up. Rows of up to 32 parts have 8
+// groups, longer ones 32.
 template <int TYPE, int GROUPS>
 __global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a) {
-  __shared__ float po[JOIN_PARTS][32];
-  __shared__ float2 pml[JOIN_PARTS];
+  constexpr int AT = GROUPS == 8 ? 2 : 4, MOST = GROUPS == 8 ? 32 : JOIN_PARTS;
+  __shared__ float po[MOST][32], so[JOIN_SUMS][32];
+  __shared__ float2 pml[MOST];
+  __shared__ float sl[JOIN_SUMS];
   const int fl = threadIdx.x & 31, grp = threadIdx.x >> 5, dim = blockIdx.y * 32 + fl;
   int s, tok, head;
   const int last = row_of(a, blockIdx.x, &s, &tok, &head);
@@ -711,64 +738,91 @@ __global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a
     if (grp == 0) emit<TYPE>(a, s, tok, head, dim, last == ROW_NONE ? 0.0f : NAN);
     return;
   }
-  const int len = record_len(a, s), nrec = last / len + 1, per = len == SPAN ? CHUNK / SPAN : 1;  // records per chunk
+  const int len = record_len(a, s), nrec = last / len + 1;
   const int np = last / PART + 1;
   const float *o = record_o(a, blockIdx.x, 0) + dim;
   const float2 *ml = record_ml(a, blockIdx.x, 0);
   Sum<1> f;
   f.clear();
-  for (int b0 = 0; b0 < np; b0 += JOIN_PARTS) {
-    for (int p = b0 + grp; p < min(b0 + JOIN_PARTS, np); p += GROUPS) {
-      Sum<1> u;
-      u.clear();
-      for (int j = 0; j < per; j++) {  // chunk records: all eight of a part; span records: two chunks' at a time
-        float x[CHUNKS][1];
-        float2 v[CHUNKS];
-        const int r0 = (p * per + j) * CHUNKS;
-        if (r0 >= nrec) break;
+  for (int b0 = 0; b0 < np; b0 += MOST) {
+    const int n = min(MOST, np - b0);
+    if (len == CHUNK) {
+      for (int i0 = grp; i0 < n; i0 += AT * GROUPS) {
+        float x[AT][CHUNKS][1];
+        float2 v[AT][CHUNKS];
         #pragma unroll
-        for (int k = 0; k < CHUNKS; k++) {
-          const int c = min(r0 + k, nrec - 1);
-          x[k][0] = o[(long)c * a.c.hd];
-          v[k] = ml[c];
-        }
-        if (per == 1) {
-          fold_all<CHUNKS, 1>(u, v, x, nrec - r0);
-        } else {
+        for (int i = 0; i < AT; i++)
           #pragma unroll
-          for (int h = 0; h < CHUNKS; h += CHUNK / SPAN) {
-            float y[CHUNK / SPAN][1];
-            float2 w[CHUNK / SPAN];
+          for (int k = 0; k < CHUNKS; k++) {
+            const int c = min((b0 + i0 + i * GROUPS) * CHUNKS + k, nrec - 1);
+            x[i][k][0] = o[(long)c * a.c.hd];
+            v[i][k] = ml[c];
+          }
+        #pragma unroll
+        for (int i = 0; i < AT; i++) {
+          const int p = i0 + i * GROUPS;
+          if (p >= n) break;
+          Sum<1> u;
+          u.clear();
+          fold_all<CHUNKS, 1>(u, v[i], x[i], nrec - (b0 + p) * CHUNKS);
+          po[p][fl] = u.o[0];
+          if (fl == 0) pml[p] = make_float2(u.m, u.l);
+        }
+      }
+    } else {
+      static_assert(CHUNK / SPAN == CHUNKS, "records folded at a time");
+      for (int p = grp; p < n; p += GROUPS) {
+        Sum<1> u;
+        u.clear();
+        for (int j0 = (b0 + p) * CHUNKS; j0 < (b0 + p + 1) * CHUNKS && j0 * CHUNKS < nrec; j0 += 2) {  // two chunks' loads together
+          float x[2][CHUNKS][1];
+          float2 v[2][CHUNKS];
+          #pragma unroll
+          for (int j = 0; j < 2; j++)
             #pragma unroll
-            for (int k = 0; k < CHUNK / SPAN; k++) {
-              y[k][0] = x[h + k][0];
-              w[k] = v[h + k];
+            for (int k = 0; k < CHUNKS; k++) {
+              const int c = min((j0 + j) * CHUNKS + k, nrec - 1);
+              x[j][k][0] = o[(long)c * a.c.hd];
+              v[j][k] = ml[c];
             }
+          #pragma unroll
+          for (int j = 0; j < 2; j++) {
+            if ((j0 + j) * CHUNKS >= nrec) break;
             Sum<1> c;
             c.clear();
-            if (r0 + h < nrec) {
-              fold_all<CHUNK / SPAN, 1>(c, w, y, nrec - r0 - h);
-              u.fold(c);
-            }
+            fold_all<CHUNKS, 1>(c, v[j], x[j], nrec - (j0 + j) * CHUNKS);
+            u.fold(c);
           }
         }
+        po[p][fl] = u.o[0];
+        if (fl == 0) pml[p] = make_float2(u.m, u.l);
       }
-      po[p - b0][fl] = u.o[0];
-      if (fl == 0) pml[p - b0] = make_float2(u.m, u.l);
     }
     __syncthreads();
-    if (grp == 0)
-      for (int i0 = 0; i0 < min(JOIN_PARTS, np - b0); i0 += 8) {
-        float2 m8[8];
-        float o8[8][1];
-        #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          m8[i] = pml[i0 + i];
-          o8[i][0] = po[i0 + i][fl];
-        }
-        fold_all<8, 1>(f, m8, o8, min(JOIN_PARTS, np - b0) - i0);
+    float M = -INFINITY;
+    if (grp < JOIN_SUMS) {
+      for (int p = fl; p < n; p += 32) M = fmaxf(M, pml[p].x);
+      M = group_reduce(M, 32, [](float x, float y) { return fmaxf(x, y); });
+      const float r = M == -INFINITY ? 0.0f : M;
+      float l = 0.0f, x = 0.0f;
+      for (int p = grp; p < n; p += JOIN_SUMS) {
+        const float w = exp2_(pml[p].x - r);
+        l = fmaf(pml[p].y, w, l);
+        x = fmaf(po[p][fl], w, x);
       }
+      so[grp][fl] = x;
+      if (fl == 0) sl[grp] = l;
+    }
     __syncthreads();
+    if (grp == 0) {
+      Sum<1> u;
+      u.m = M;
+      u.l = sl[0];
+      u.o[0] = so[0][fl];
+      #pragma unroll
+      for (int i = 1; i < JOIN_SUMS; i++) u.l += sl[i], u.o[0] += so[i][fl];
+      f.fold(u);
+    }
   }
   if (grp == 0) emit<TYPE>(a, s, tok, head, dim, f.o[0] / f.l);
 }
@@ -784,20 +838,39 @@ __global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a) {
   if (last == ROW_ABSENT) return;
   Sum<NB> f;
   f.clear();
-  const int nrec = last < 0 ? 0 : last / PART + 1;
+  const int np = last < 0 ? 0 : last / PART + 1;
   const float *o = record_o(a, row, 0) + fl;
   const float2 *ml = record_ml(a, row, 0);
-  for (int c0 = 0; c0 < nrec; c0 += 4) {
-    float2 v[4];
-    float x[4][NB];
+  for (int b0 = 0; b0 < np; b0 += JOIN_PARTS) {
+    const int n = min(JOIN_PARTS, np - b0);
+    Sum<NB> u[JOIN_SUMS];
+    float M = -INFINITY;
+    for (int p = fl; p < n; p += 32) M = fmaxf(M, ml[b0 + p].x);
+    M = group_reduce(M, 32, [](float x, float y) { return fmaxf(x, y); });
+    const float r = M == -INFINITY ? 0.0f : M;
     #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int c = min(c0 + k, nrec - 1);
-      v[k] = ml[c];
+    for (int k = 0; k < JOIN_SUMS; k++) u[k].clear();
+    for (int p0 = 0; p0 < n; p0 += JOIN_SUMS) {
       #pragma unroll
-      for (int i = 0; i < NB; i++) x[k][i] = o[(long)c * a.c.hd + 32 * i];
+      for (int k = 0; k < JOIN_SUMS; k++) {
+        const int p = b0 + min(p0 + k, n - 1);
+        const float2 v = ml[p];
+        const float w = p0 + k < n ? exp2_(v.x - r) : 0.0f;
+        if (p0 + k < n) {
+          u[k].l = fmaf(v.y, w, u[k].l);
+          #pragma unroll
+          for (int i = 0; i < NB; i++) u[k].o[i] = fmaf(o[(long)p * a.c.hd + 32 * i], w, u[k].o[i]);
+        }
+      }
     }
-    fold_all<4, NB>(f, v, x, nrec - c0);
+    #pragma unroll
+    for (int k = 1; k < JOIN_SUMS; k++) {
+      u[0].l += u[k].l;
+      #pragma unroll
+      for (int i = 0; i < NB; i++) u[0].o[i] += u[k].o[i];
+    }
+    u[0].m = M;
+    f.fold(u[0]);
   }
   #pragma unroll
   for (int i = 0; i < NB; i++) emit<TYPE>(a, s, tok, head, 32 * i + fl, last >= 0 ? f.o[i] / f.l : last == ROW_NONE ? 0.0f : NAN);
@@ -819,10 +892,13 @@ __global__ __launch_bounds__(64 * part_waves(NB)) void k_kv4_parts(const Kv4Attn
   constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ;
   extern __shared__ __align__(16) uint8_t lds_raw[];
   SpanOperands<NB> *buf = (SpanOperands<NB> *)lds_raw;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4, part = blockIdx.x;
-  const int row0 = blockIdx.y % blocks * (16 * PW) + wave * (16 * RT);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
+  long group;  // [sequence][KV head][part]
+  int block;
+  if (!dealt((long)a.nrec * a.c.nkv * a.b.nseq, blocks, &group, &block)) return;
+  const int part = (int)(group % a.nrec), row0 = block * (16 * PW) + wave * (16 * RT);
   int last[RT], tok[RT], head[RT], most = ROW_ABSENT, blockmost;
-  const Tile tl(a, blockIdx.z, blockIdx.y / blocks, 0);
+  const Tile tl(a, (int)(group / a.nrec / a.c.nkv), (int)(group / a.nrec % a.c.nkv), 0);
   #pragma unroll
   for (int r = 0; r < RT; r++) {
     last[r] = tl.last(a, row0 + 16 * r + n, &tok[r], &head[r]);
@@ -845,8 +921,7 @@ __global__ __launch_bounds__(64 * part_waves(NB)) void k_kv4_parts(const Kv4Attn
     return;
   }
   typedef typename ValueOf<TYPE>::t T;
-  uint32_t k1024 = 0x64006400u;
-  __asm__("" : "+v"(k1024));
+  const Unpack uk;
   // the wave's share of a span: records' key words then value words, NW 16-byte loads (of NB / 2 per record and kind)
   const int npos = min(blockmost + 1, (part + 1) * PART), nspan = (npos - part * PART + SPAN - 1) / SPAN;
   const uint8_t *base = record_of(a.c, tl.slot, tl.kvh, (long)part * (PART / KV4_GROUP));
@@ -869,7 +944,7 @@ __global__ __launch_bounds__(64 * part_waves(NB)) void k_kv4_parts(const Kv4Attn
       const int idx = wave * NW + x, i = idx / NB, kv = idx / (NB / 2) & 1, j = idx % (NB / 2);
       if (idx >= 2 * NB) break;
       #pragma unroll
-      for (int y = 0; y < 4; y++) (kv ? d.v : d.k)[i][4 * j + y][lane] = unpack8<TINY>(words[x][y], k1024);
+      for (int y = 0; y < 4; y++) (kv ? d.v : d.k)[i][4 * j + y][lane] = unpack8<TINY>(words[x][y], uk);
     }
     const int e = tid, i = e / (8 * NB), r = e % (8 * NB);
     if (e < 16 * NB) (r < 4 * NB ? d.ks : d.vs)[i][r % (4 * NB)] = scales;
@@ -997,19 +1072,19 @@ static void launch_attention_k(Kv4Attn a, hipStream_t st) {
   if (many) {
     constexpr int PW = part_waves(NB);
     const long nb = (rows + 16 * PW - 1) / (16 * PW);
-    hipLaunchKernelGGL((k_kv4_parts<NB, TYPE>), dim3(a.nrec, (unsigned)(nb * a.c.nkv), a.b.nseq), dim3(64 * PW), 2 * sizeof(SpanOperands<NB>), st, a, (int)nb);
+    hipLaunchKernelGGL((k_kv4_parts<NB, TYPE>), dim3((unsigned)deal_blocks((long)a.nrec * a.c.nkv * a.b.nseq, (int)nb)), dim3(64 * PW), 2 * sizeof(SpanOperands<NB>), st, a, (int)nb);
   } else {
     // waves of chunks up to two a SIMD, each with an even share of the chunks beyond; or of spans
     const int tiles = (int)((rows + 15) / 16), nch = (int)((a.c.cap + CHUNK - 1) / CHUNK);
     const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (nch * y + 2047) / 2048;
     const int gx = std::max((int)((nch + 4 * rounds - 1) / (4 * rounds)), (a.spanmax + 3) / 4);
-    hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3(gx, tiles * a.c.nkv, a.b.nseq), dim3(256), 0, st, a, tiles);
+    hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3((unsigned)deal_blocks((long)gx * a.c.nkv * a.b.nseq, tiles)), dim3(256), 0, st, a, tiles, gx);
   }
   ZL_HIP(hipGetLastError());
   if (a.nrec > 1) {
     const long n = rows * a.c.nkv * a.b.nseq;
     if (many) hipLaunchKernelGGL((k_kv4_join_parts<NB, TYPE>), dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, a);
-    else if (a.c.cap > 16 * PART) hipLaunchKernelGGL((k_kv4_join_chunks<TYPE, 32>), dim3((unsigned)n, NB), dim3(1024), 0, st, a);
+    else if (a.c.cap > 32 * PART) hipLaunchKernelGGL((k_kv4_join_chunks<TYPE, 32>), dim3((unsigned)n, NB), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((k_kv4_join_chunks<TYPE, 8>), dim3((unsigned)n, NB), dim3(256), 0, st, a);
     ZL_HIP(hipGetLastError());
   }
