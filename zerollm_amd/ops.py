@@ -20,19 +20,22 @@ from . import _lib
 from ._lib import call
 
 _TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
+_type_of = {}  # by torch's type objects, filled as they come: a call on few rows is as long as its checks
 
 
 def _place(x, name):
-    d = getattr(x, "device", None)
-    if getattr(d, "type", None) != "cuda" or (d.index or 0) != _lib.DEVICE:
-        raise ValueError(f"{name} must be a tensor on GPU {_lib.DEVICE} (got {d})")
+    if not getattr(x, "is_cuda", False) or x.get_device() != _lib.DEVICE:
+        raise ValueError(f"{name} must be a tensor on GPU {_lib.DEVICE} (got {getattr(x, 'device', None)})")
 
 
 def _type(x, name):
     _place(x, name)
-    t = _TYPES.get(str(x.dtype))
+    t = _type_of.get(x.dtype)
     if t is None:
-        raise ValueError(f"{name} must be float32, float16 or bfloat16 (got {x.dtype})")
+        t = _TYPES.get(str(x.dtype))
+        if t is None:
+            raise ValueError(f"{name} must be float32, float16 or bfloat16 (got {x.dtype})")
+        _type_of[x.dtype] = t
     return t
 
 
@@ -40,7 +43,7 @@ def _ints(x, n, name):
     if x is None:
         return None
     _place(x, name)
-    if str(x.dtype) != "torch.int32" or tuple(x.shape) != (n,) or not x.is_contiguous():
+    if x.dtype != _torch().int32 or x.shape != (n,) or not x.is_contiguous():
         raise ValueError(f"{name} must be {n} contiguous int32 values (got {x.dtype} {tuple(x.shape)})")
     return x.data_ptr()
 
@@ -59,7 +62,7 @@ def _rows(x, name, shape=None, type_=None, written=False):
         raise ValueError(f"{name} must be {shape} (got {s})")
     if type_ is not None and t != type_:
         raise ValueError(f"{name} must have the type of the other rows (got {x.dtype})")
-    if written and any(n > 1 and d == 0 for n, d in zip(s, st)):
+    if written and 0 in st and any(n > 1 and d == 0 for n, d in zip(s, st)):
         raise ValueError(f"{name} is written, so its rows must not share memory")
     return _lib.zl_rows(x.data_ptr(), st[0], st[1], st[2]), t, s
 
@@ -100,6 +103,7 @@ class KVCacheQ4:
         call("zl_kv4_create", int(n_slot), int(n_head_kv), int(head_dim), int(capacity), C.byref(self._h))
         self.n_slot, self.n_head_kv, self.head_dim, self.capacity = int(n_slot), int(n_head_kv), int(head_dim), int(capacity)
         self.closed = False
+        self._sized = None, 0  # the last queries' shape and its work space
 
     @property
     def nbytes(self) -> int:
@@ -148,10 +152,10 @@ class KVCacheQ4:
         if out is None:
             out = _torch().empty(tuple(q.shape), dtype=q.dtype, device=q.device)
         o = _rows(out, "out", s, t, True)[0]
-        n = C.c_int64()
-        call("zl_kv4_attention_work", self._handle(), s[0], s[1], s[2], C.byref(n))
-        w = _work(work, n.value, q)
-        call("zl_kv4_attention", self._h, b, t, qr, s[2], scale or 0.0, o, w.data_ptr(), w.numel() * w.element_size(), _stream())
+        if s != self._sized[0]:
+            self._sized = s, self.work_bytes(s[0], s[1], s[2])
+        w = _work(work, self._sized[1], q)
+        call("zl_kv4_attention", self._handle(), b, t, qr, s[2], scale or 0.0, o, w.data_ptr(), w.numel() * w.element_size(), _stream())
         return out
 
     def close(self):
