@@ -8,7 +8,7 @@
 // Scores live in a [token][head][ctx] f32 buffer between the two. The weighted sum of a chunk keeps the reference's f32
 // rounding after every position, so rows of up to 2048 positions are the reference's bits (a random-weight network turns a
 // 1e-7 change there into a visible logit difference); the chunks of longer rows are joined in f64.
-#include "zl_kernels.h"
+#include "zl_ops.h"
 #include "zl_exp.h"
 #include <algorithm>
 #include <climits>
@@ -299,6 +299,73 @@ __global__ __launch_bounds__(64) void k_attn_prep(const AttnArgs a) {
   }
 }
 
+// The same for a cache in 4 bits (zl_ops.h): keys and values are quantised as zl_kv4_append does. A value word holds the codes of 8
+// positions, and other blocks of the pass may write their own ones, so each code goes in by two atomic operations on its four bits
+// alone: their order does not matter. A launch of its own for the append costs 5 us a layer, this one none.
+template <int HD>
+__global__ __launch_bounds__(64) void k_attn_prep_q4(const AttnArgs a, const Kv4View c) {
+  constexpr int NB = HD / 32;
+  __shared__ float v[2][HD];
+  const int b = blockIdx.x, hy = blockIdx.y, lane = threadIdx.x;
+  const Step *st = a.step;
+  if (b >= st->B) return;
+  const int pos = st->pos0 + b;
+  const bool isq = hy < a.nHead;
+  const int h = isq ? hy : hy - a.nHead;
+  const float *src = isq ? a.q + (long)b * a.ldq + (long)h * a.qhs : a.k + (long)b * a.ldkv + (long)h * HD;
+  for (int i = lane; i < HD; i += 64) {
+    v[0][i] = src[i];
+    if (!isq) v[1][i] = a.v[(long)b * a.ldkv + (long)h * HD + i];
+  }
+  __syncthreads();
+  norm_rope<HD>(v[0], isq ? a.qNorm : a.kNorm, a.eps, a.nRot, a.neox, a.cosT, a.sinT, pos, lane);
+  __syncthreads();
+  if (isq) {
+    for (int i = lane; i < HD; i += 64) a.qr[((long)b * a.nHead + h) * HD + i] = v[0][i];
+    return;
+  }
+  if (lane >= 2 * HD / 8 || pos < 0 || pos >= c.cap) return;
+  const int isv = lane / (HD / 8), d8 = lane % (HD / 8), p = pos & 31;
+  float y[8];
+  #pragma unroll
+  for (int e = 0; e < 8; e++) y[e] = v[isv][8 * d8 + e];
+  int code[8];
+  const uint16_t scale = kv4_quant(y, lane, code);
+  uint8_t *rec = c.base + ((long)h * c.ngroup + (pos >> 5)) * kv4_record(HD);
+  if ((lane & 3) == 0) ((uint16_t *)(rec + (isv ? 34 : 32) * HD))[kv4_scale(p, d8 >> 2, NB)] = scale;
+  uint32_t *words = (uint32_t *)(rec + isv * 16 * HD);
+  if (!isv) {
+    words[kv4_word((p >> 4) * NB + (d8 >> 2), (p & 15) + 16 * (d8 & 3))] = kv4_pack(code);
+    return;
+  }
+  const int sh = 4 * kv4_nibble(4 * (p >> 4) + (p & 3));
+  #pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const int dim = 8 * d8 + e;
+    uint32_t *w = words + kv4_word(dim >> 4, (dim & 15) + 16 * ((p >> 2) & 3));
+    atomicAnd(w, ~(15u << sh));
+    atomicOr(w, (uint32_t)code[e] << sh);
+  }
+}
+
+// The attention over a cache in 4 bits (c: the layer's, one slot), work for its records.
+void launch_attention_q4(const AttnArgs &a, const Kv4View &c, void *work, int B, hipStream_t st) {
+  ZL_REQUIRE(a.qhs >= a.hd && a.ldq >= a.nHead * a.qhs && c.hd == a.hd && c.nkv == a.nHeadKv, ZL_ERR_ARG, "attention: head sizes");
+  const dim3 gp(B, a.nHead + a.nHeadKv);
+  if (a.hd == 64) hipLaunchKernelGGL(k_attn_prep_q4<64>, gp, dim3(64), 0, st, a, c);
+  else if (a.hd == 128) hipLaunchKernelGGL(k_attn_prep_q4<128>, gp, dim3(64), 0, st, a, c);
+  else hipLaunchKernelGGL(k_attn_prep_q4<256>, gp, dim3(64), 0, st, a, c);
+  ZL_HIP(hipGetLastError());
+  Kv4Attn k{};
+  k.c = c;
+  k.b = OpBatch{1, B, &a.step->pos0, &a.step->B, nullptr};
+  k.q = OpRows{a.qr, 0, (long)a.nHead * a.hd, a.hd};
+  k.nhead = a.nHead;
+  k.scale = (float)a.scale;
+  k.work = work;
+  launch_kv4_attention_model(k, HeadOut{a.gate, a.ldq, a.qhs, a.hd, a.out, a.ldo, a.act}, st);
+}
+
 // Block (every X-th 64-position tile of the pass, KV head, group of NWV row tiles); wave w computes row tile NWV z + w: 16
 // rows r = b G + g (token b, query head kvh G + g) against every position of its tiles, 16 positions at a time. Lane l
 // supplies A = the row l mod 16's dimension 32 j + 4 m + l / 16 (its query values, f64, held for the whole block) and B = key value
@@ -503,18 +570,6 @@ __device__ __forceinline__ void chunk_join(const double *r, long lds, int n, int
   }
   #pragma unroll
   for (int i = 0; i < NS; i++) out[i] = (float)(O[i] / L);
-}
-
-// The head output of 32 dimensions on 32 consecutive lanes: the output gate when there is one
-// (src/model/forward-qwen35.js:103: o * sigmoid(gate), f64, stored f32), the f32 row, its quantisation.
-__device__ __forceinline__ void attn_emit(const AttnArgs &a, int b, int h, int dim, float o) {
-  const int col = h * a.hd + dim;
-  if (a.gate) {
-    const double g = (double)a.gate[(long)b * a.ldq + (long)h * a.qhs + dim];
-    o = (float)((double)o * (1.0 / (1.0 + exp(-g))));
-  }
-  if (a.out) a.out[(long)b * a.ldo + col] = o;
-  if (a.act.q) quant_block32(o, col, a.act, b);  // (unset: the output GEMV quantises the f32 rows itself)
 }
 
 // One block per (32-dim slice, query head, token, chunk). The slice's V rows (dimension-major in the cache) are staged

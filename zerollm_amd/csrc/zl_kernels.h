@@ -144,6 +144,14 @@ struct AttnArgs {
   int mmMinB, mmAvMinB;  // ... and at least mmAvMinB tokens the matrix-core weighted sums (k_attn_av_mm)
   float *qr;
 };
+// The fields of AttnArgs that say where head outputs go.
+struct HeadOut {
+  const float *gate;
+  int ldq, qhs, hd;
+  float *out;
+  int ldo;
+  Act act;
+};
 // Positions per chunk of a row. Rows of up to this many positions are the reference's f32 chain over the whole row; the
 // chunks of longer ones run side by side.
 constexpr int ATTN_CHUNK = 2048;
@@ -309,6 +317,19 @@ __device__ inline void quant_block32(float v, int i, const Act &a, int row) {
     a.rb[k] = RecB{d, 32 * b.s16a, 32 * b.s16b};
     a.rc[k] = RecC{d, 8 * b.s32, 16 * b.s32};
   }
+}
+
+// The head output of 32 dimensions on 32 consecutive lanes: the output gate when there is one
+// (src/model/forward-qwen35.js:103: o * sigmoid(gate), f64, stored f32), the f32 row, its quantisation.
+template <class A>  // AttnArgs or HeadOut
+__device__ __forceinline__ void attn_emit(const A &a, int b, int h, int dim, float o) {
+  const int col = h * a.hd + dim;
+  if (a.gate) {
+    const double g = (double)a.gate[(long)b * a.ldq + (long)h * a.qhs + dim];
+    o = (float)((double)o * (1.0 / (1.0 + exp(-g))));
+  }
+  if (a.out) a.out[(long)b * a.ldo + col] = o;
+  if (a.act.q) quant_block32(o, col, a.act, b);  // (unset: the output GEMV quantises the f32 rows itself)
 }
 
 // RMSNorm scale of one row (src/compute/ref-kernels.js:305-310): 1/sqrt(mean(x^2) + eps), the sum of squares taken by

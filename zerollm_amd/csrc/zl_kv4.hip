@@ -12,9 +12,7 @@ __device__ __forceinline__ int slot_of(const OpBatch &b, int s) { return b.slot 
 
 // ---------------------------------------------------------------------------------------------- append
 // One block per (32-position record that a sequence may touch, KV head, sequence). A lane takes 8 values, four lanes a block
-// of 32: the value of largest magnitude (the lowest index among equals) gives d = mx / -8, and code = clamp(trunc(x / d + 8.5),
-// 0, 15) with 1/d, the product and the sum each rounded in f64, as the library's Q4_0 quantiser. The codes go to LDS and from
-// there in whole words: a key word is one lane's 8 values; a value word holds 8 positions, and those that are not appended
+// of 32 (kv4_quant). The codes go to LDS and from there in whole words: a key word is one lane's 8 values; a value word holds 8 positions, and those that are not appended
 // keep their codes. The block of the first sequence that touches a record of a slot takes all of them, in order.
 // Bound by the loads' latency: all of a record's are requested together (2048 tokens of 8 heads of 128, bf16: 37 us with a
 // value per lane and a load at a time).
@@ -80,37 +78,14 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4View c, const OpBat
       for (int u = 0; u < UNITS; u++) {
         const int i = u * 256 + tid, t = i / (4 * NB), d8 = i % (4 * NB), p = q0 + t;
         if (t >= n) continue;  // (four lanes of a block of 32 go together)
-        const float (&y)[8] = x[isv][u];
-        float am = 0.0f;
-        uint32_t neg = 0;
-        bool bad = false;
-        #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float m = fabsf(y[e]);
-          bad |= !(m <= 65504.0f);
-          if (m > am) { am = m; neg = __float_as_uint(y[e]) >> 31; }
-        }
-        const float all = fmaxf(fmaxf(am, dpp_move<0xB1>(am)), dpp_move<0x4E>(fmaxf(am, dpp_move<0xB1>(am))));
-        // the first lane that reached it, and its sign, as one number; bad blocks
-        uint32_t first = am == all ? 2 * (tid & 3) + neg : 8;
-        first = min(first, dpp_move<0xB1>(first));
-        first = min(first, dpp_move<0x4E>(first));
-        uint32_t nan = bad;
-        nan |= dpp_move<0xB1>(nan);
-        nan |= dpp_move<0x4E>(nan);
-        const float mx = first & 1 ? -all : all;
-        const double d = (double)mx / -8.0, inv = d != 0.0 ? 1.0 / d : 0.0;
-        uint32_t w = 0;
+        int code[8];
+        const uint16_t scale = kv4_quant(x[isv][u], tid, code);
+        if ((tid & 3) == 0) ((uint16_t *)(rec + (isv ? 34 : 32) * HD))[kv4_scale(p, d8 >> 2, NB)] = scale;
         uint64_t bytes = 0;
         #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int code = nan ? 8 : min(15, max(0, (int)((double)y[e] * inv + 8.5)));
-          w |= (uint32_t)code << (4 * kv4_nibble(e));
-          bytes |= (uint64_t)code << (8 * e);
-        }
-        if ((tid & 3) == 0) ((uint16_t *)(rec + (isv ? 34 : 32) * HD))[kv4_scale(p, d8 >> 2, NB)] = nan ? (uint16_t)0x7e00 : f2h((float)d);
+        for (int e = 0; e < 8; e++) bytes |= (uint64_t)code[e] << (8 * e);
         if (isv) vn[p][d8] = bytes;
-        else kw[kv4_word((p >> 4) * NB + (d8 >> 2), (p & 15) + 16 * (d8 & 3))] = w;
+        else kw[kv4_word((p >> 4) * NB + (d8 >> 2), (p & 15) + 16 * (d8 & 3))] = kv4_pack(code);
       }
     __syncthreads();
     uint32_t *kd = (uint32_t *)rec, *vd = (uint32_t *)(rec + 16 * HD);
@@ -554,12 +529,19 @@ __device__ __forceinline__ float2 *record_ml(const Kv4Attn &a, long row, int rec
   const long rows = (long)a.b.nseq * a.b.ntok * a.nhead;
   return (float2 *)((float *)a.work + rows * a.nrec * a.c.hd) + row * a.nrec + rec;
 }
+// Where outputs go: rows of the caller's type, or a model's (32 dimensions on 32 lanes).
+// (+ 0: a sum of -0 comes out the same whether it was folded with empty pieces or not)
 template <int TYPE>
-__device__ __forceinline__ void emit(const Kv4Attn &a, int s, int tok, int head, int dim, float o) {
-  typedef typename ValueOf<TYPE>::t T;
-  // (+ 0: a sum of -0 comes out the same whether it was folded with empty pieces or not)
-  ((T *)a.out.p)[s * a.out.seq + tok * a.out.tok + head * a.out.head + dim] = store_value<TYPE>(o + 0.0f);
-}
+struct ToRows {
+  OpRows r;
+  __device__ __forceinline__ void emit(int s, int tok, int head, int dim, float o) const {
+    ((typename ValueOf<TYPE>::t *)r.p)[s * r.seq + tok * r.tok + head * r.head + dim] = store_value<TYPE>(o + 0.0f);
+  }
+};
+struct ToModel {
+  HeadOut h;
+  __device__ __forceinline__ void emit(int, int tok, int head, int dim, float o) const { attn_emit(h, tok, head, dim, o + 0.0f); }
+};
 
 // A span's two products of block b and record: values times weights, and with TINY the weights' sums.
 template <bool LOW, bool TINY>
@@ -592,13 +574,14 @@ __device__ __forceinline__ int record_len(const Kv4Attn &a, int s) {
 // l has row l % 16, dimensions 16 j + 4 (l / 16) + v.
 template <int NB, int TYPE>
 __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last, int tok, int head, int rec, int first, const Sum<8 * NB> &f, int g) {
-  if (a.nrec == 1) {
+  if (a.direct) {
     if (last == ROW_ABSENT) return;
+    const ToRows<TYPE> out{a.out};
     #pragma unroll
     for (int j = 0; j < 2 * NB; j++)
       #pragma unroll
       for (int v = 0; v < 4; v++)
-        emit<TYPE>(a, tl.s, tok, head, 16 * j + 4 * g + v, last >= 0 ? f.o[4 * j + v] / f.l : last == ROW_NONE ? 0.0f : NAN);
+        out.emit(tl.s, tok, head, 16 * j + 4 * g + v, last >= 0 ? f.o[4 * j + v] / f.l : last == ROW_NONE ? 0.0f : NAN);
     return;
   }
   if (last < first) return;
@@ -633,7 +616,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
   Sum<8 * NB> u;
   u.clear();
   if (most < (long)c0 * unit) {
-    if (a.nrec == 1 && c0 == 0) leave<NB, TYPE>(a, tl, last, tok, head, 0, 0, u, g);
+    if (a.direct && c0 == 0) leave<NB, TYPE>(a, tl, last, tok, head, 0, 0, u, g);
     return;
   }
   typedef typename ValueOf<TYPE>::t T;
@@ -724,8 +707,8 @@ constexpr int JOIN_PARTS = 128, JOIN_SUMS = 8;
 // Rows of chunk or span records, few of them: a block per (row, 32 dimensions), a dimension per lane. Its groups of 32 lanes fold the
 // chunks of a part each, the loads of AT parts issued together, and eight of them sum the parts up. Rows of up to 32 parts have 8
 // groups, longer ones 32.
-template <int TYPE, int GROUPS>
-__global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a) {
+template <int GROUPS, class OUT>
+__global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a, const OUT out) {
   constexpr int AT = GROUPS == 8 ? 2 : 4, MOST = GROUPS == 8 ? 32 : JOIN_PARTS;
   __shared__ float po[MOST][32], so[JOIN_SUMS][32];
   __shared__ float2 pml[MOST];
@@ -735,7 +718,7 @@ __global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a
   const int last = row_of(a, blockIdx.x, &s, &tok, &head);
   if (last == ROW_ABSENT) return;
   if (last < 0) {
-    if (grp == 0) emit<TYPE>(a, s, tok, head, dim, last == ROW_NONE ? 0.0f : NAN);
+    if (grp == 0) out.emit(s, tok, head, dim, last == ROW_NONE ? 0.0f : NAN);
     return;
   }
   const int len = record_len(a, s), nrec = last / len + 1;
@@ -824,12 +807,12 @@ __global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a
       f.fold(u);
     }
   }
-  if (grp == 0) emit<TYPE>(a, s, tok, head, dim, f.o[0] / f.l);
+  if (grp == 0) out.emit(s, tok, head, dim, f.o[0] / f.l);
 }
 
 // Rows of part records, many of them: 32 lanes per row.
-template <int NB, int TYPE>
-__global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a) {
+template <int NB, class OUT>
+__global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a, const OUT out) {
   const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int fl = threadIdx.x & 31;
   if (row >= (long)a.b.nseq * a.b.ntok * a.nhead) return;
@@ -873,7 +856,7 @@ __global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a) {
     f.fold(u[0]);
   }
   #pragma unroll
-  for (int i = 0; i < NB; i++) emit<TYPE>(a, s, tok, head, 32 * i + fl, last >= 0 ? f.o[i] / f.l : last == ROW_NONE ? 0.0f : NAN);
+  for (int i = 0; i < NB; i++) out.emit(s, tok, head, 32 * i + fl, last >= 0 ? f.o[i] / f.l : last == ROW_NONE ? 0.0f : NAN);
 }
 
 // Many rows: a block takes PW waves of a tile of 16 rows each through the spans of one part. The waves unpack a span's
@@ -916,7 +899,7 @@ __global__ __launch_bounds__(64 * part_waves(NB)) void k_kv4_parts(const Kv4Attn
   #pragma unroll
   for (int r = 0; r < RT; r++) f[r].clear(), u[r].clear();
   if (blockmost < part * PART) {
-    if (a.nrec == 1)
+    if (a.direct)
       for (int r = 0; r < RT; r++) leave<NB, TYPE>(a, tl, last[r], tok[r], head[r], 0, 0, f[r], g);
     return;
   }
@@ -1061,13 +1044,14 @@ long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead) {
   return std::max(16L, (long)nseq * ntok * nhead * record_count(c, nseq, ntok, nhead) * (c.hd + 2) * 4);
 }
 
-template <int NB, int TYPE>
-static void launch_attention_k(Kv4Attn a, hipStream_t st) {
+template <int NB, int TYPE, class OUT>
+static void launch_attention_k(Kv4Attn a, const OUT &out, bool direct, hipStream_t st) {
   const bool many = many_rows(a.c, a.b.nseq, a.b.ntok, a.nhead);
   const int group = a.nhead / a.c.nkv;
   a.nrec = record_count(a.c, a.b.nseq, a.b.ntok, a.nhead);
   a.spanmax = many ? 0 : span_max(a.c, tile_count(a.c, a.b.nseq, a.b.ntok, a.nhead));
   a.qvec = whole_pieces(a.q, TYPE);
+  a.direct = direct && a.nrec == 1;
   const long rows = (long)a.b.ntok * group;
   if (many) {
     constexpr int PW = part_waves(NB);
@@ -1081,11 +1065,11 @@ static void launch_attention_k(Kv4Attn a, hipStream_t st) {
     hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3((unsigned)deal_blocks((long)gx * a.c.nkv * a.b.nseq, tiles)), dim3(256), 0, st, a, tiles, gx);
   }
   ZL_HIP(hipGetLastError());
-  if (a.nrec > 1) {
+  if (!a.direct) {
     const long n = rows * a.c.nkv * a.b.nseq;
-    if (many) hipLaunchKernelGGL((k_kv4_join_parts<NB, TYPE>), dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, a);
-    else if (a.c.cap > 32 * PART) hipLaunchKernelGGL((k_kv4_join_chunks<TYPE, 32>), dim3((unsigned)n, NB), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((k_kv4_join_chunks<TYPE, 8>), dim3((unsigned)n, NB), dim3(256), 0, st, a);
+    if (many) hipLaunchKernelGGL((k_kv4_join_parts<NB, OUT>), dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, a, out);
+    else if (a.c.cap > 32 * PART) hipLaunchKernelGGL((k_kv4_join_chunks<32, OUT>), dim3((unsigned)n, NB), dim3(1024), 0, st, a, out);
+    else hipLaunchKernelGGL((k_kv4_join_chunks<8, OUT>), dim3((unsigned)n, NB), dim3(256), 0, st, a, out);
     ZL_HIP(hipGetLastError());
   }
 }
@@ -1109,14 +1093,19 @@ void kv4_prepare(int hd) {
 
 template <int NB>
 static void launch_attention_t(const Kv4Attn &a, int type, hipStream_t st) {
-  if (type == T_F32) launch_attention_k<NB, T_F32>(a, st);
-  else if (type == T_F16) launch_attention_k<NB, T_F16>(a, st);
-  else launch_attention_k<NB, T_BF16>(a, st);
+  if (type == T_F32) launch_attention_k<NB, T_F32>(a, ToRows<T_F32>{a.out}, true, st);
+  else if (type == T_F16) launch_attention_k<NB, T_F16>(a, ToRows<T_F16>{a.out}, true, st);
+  else launch_attention_k<NB, T_BF16>(a, ToRows<T_BF16>{a.out}, true, st);
 }
 void launch_kv4_attention(const Kv4Attn &a, int type, hipStream_t st) {
   if (a.c.hd == 64) launch_attention_t<2>(a, type, st);
   else if (a.c.hd == 128) launch_attention_t<4>(a, type, st);
   else launch_attention_t<8>(a, type, st);
+}
+void launch_kv4_attention_model(const Kv4Attn &a, const HeadOut &out, hipStream_t st) {
+  if (a.c.hd == 64) launch_attention_k<2, T_F32>(a, ToModel{out}, false, st);
+  else if (a.c.hd == 128) launch_attention_k<4, T_F32>(a, ToModel{out}, false, st);
+  else launch_attention_k<8, T_F32>(a, ToModel{out}, false, st);
 }
 
 }  // namespace zl

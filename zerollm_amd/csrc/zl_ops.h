@@ -43,6 +43,41 @@ __host__ __device__ constexpr int kv4_word(int w, int lane) { return ((w >> 2) *
 __host__ __device__ constexpr int kv4_nibble(int e) { return (e >> 1) + 4 * (e & 1); }
 __host__ __device__ constexpr int kv4_scale(int p, int b, int nb) { return ((((p >> 2) & 3) * 2 + ((p >> 4) & 1)) * nb + b) * 4 + (p & 3); }
 
+// Q4_0 of a block of 32 values, eight on each of four neighbouring lanes: the value of largest magnitude (the lowest index among
+// equals) gives d = mx / -8, and code = clamp(trunc(x / d + 8.5), 0, 15) with 1/d, the product and the sum each rounded in f64, as
+// the library's Q4_0 quantiser. Returns d in f16; NaN for a block with a value that is not finite or beyond f16.
+__device__ __forceinline__ uint16_t kv4_quant(const float (&y)[8], int lane, int (&code)[8]) {
+  float am = 0.0f;
+  uint32_t neg = 0;
+  bool bad = false;
+  #pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float m = fabsf(y[e]);
+    bad |= !(m <= 65504.0f);
+    if (m > am) { am = m; neg = __float_as_uint(y[e]) >> 31; }
+  }
+  const float two = fmaxf(am, dpp_move<0xB1>(am)), all = fmaxf(two, dpp_move<0x4E>(two));
+  // the first lane that reached it, and its sign, as one number; bad blocks
+  uint32_t first = am == all ? 2 * (lane & 3) + neg : 8;
+  first = min(first, dpp_move<0xB1>(first));
+  first = min(first, dpp_move<0x4E>(first));
+  uint32_t nan = bad;
+  nan |= dpp_move<0xB1>(nan);
+  nan |= dpp_move<0x4E>(nan);
+  const float mx = first & 1 ? -all : all;
+  const double d = (double)mx / -8.0, inv = d != 0.0 ? 1.0 / d : 0.0;
+  #pragma unroll
+  for (int e = 0; e < 8; e++) code[e] = nan ? 8 : min(15, max(0, (int)((double)y[e] * inv + 8.5)));
+  return nan ? (uint16_t)0x7e00 : f2h((float)d);
+}
+// A key word: the lane's eight codes.
+__device__ __forceinline__ uint32_t kv4_pack(const int (&code)[8]) {
+  uint32_t w = 0;
+  #pragma unroll
+  for (int e = 0; e < 8; e++) w |= (uint32_t)code[e] << (4 * kv4_nibble(e));
+  return w;
+}
+
 struct Kv4View {
   uint8_t *base;
   int nslot, nkv, hd;
@@ -70,11 +105,15 @@ struct Kv4Attn {
   // set by the launcher: records per row in work, spans of a sequence up to which they are spans', whether the queries are whole
   // 16-byte pieces
   int nrec, spanmax;
-  bool qvec;
+  bool qvec, direct;  // direct: no records, a row's only ones are its output
 };
 void kv4_prepare(int hd);  // once before launches of this head size
 long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead);
 void launch_kv4_attention(const Kv4Attn &a, int type, hipStream_t st);
+// f32 queries of one sequence, outputs to a model's rows (a.out is not used).
+void launch_kv4_attention_model(const Kv4Attn &a, const HeadOut &out, hipStream_t st);
+// A layer's attention of a model whose cache is in 4 bits (zl_attn.hip).
+void launch_attention_q4(const AttnArgs &a, const Kv4View &c, void *work, int B, hipStream_t st);
 
 // ---- rotary positions
 struct RopeArgs {

@@ -231,6 +231,10 @@ struct zl_model {
   float *cosT = nullptr, *sinT = nullptr;
   zl_rope_opts rope{};  // position scaling (rope.scaling 0: none)
   void *kcache = nullptr, *vcache = nullptr;
+  // the cache in 4 bits (kcache and vcache null): layer ai's slot of the view, and the attention's work space
+  bool kvQ4 = false;
+  zl::Kv4View kv4{};
+  void *kv4Work = nullptr;
   float *x = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *hb = nullptr, *logits = nullptr;
   float *scores = nullptr;  // attention scores [maxBatch][n_head][ctx]
   double *attnPart = nullptr;  // position-split weighted-sum partials (contexts beyond ZEROLLM_ATTN_EXACT_CTX), or null
@@ -452,14 +456,25 @@ static void finish_model(zl_model *m, const float *ropeFreqs) {
     L.ai = L.rec ? -1 : m->nAttn++;
     L.ri = L.rec ? m->nRec++ : -1;
   }
-  // K: [slot][kv head][pos][dim]; V: [slot][kv head][dim][vstride] (vstride = ctx rounded up to 16 positions)
-  m->vstride = (m->ctx + 15) / 16 * 16;
-  const size_t kElems = (size_t)std::max(m->nAttn, 1) * c.n_head_kv * m->ctx * c.head_dim;
-  const size_t vElems = (size_t)std::max(m->nAttn, 1) * c.n_head_kv * c.head_dim * m->vstride;
-  m->kcache = m->ar.alloc(kElems * (m->kvF16 ? 2 : 4));
-  m->vcache = m->ar.alloc(vElems * (m->kvF16 ? 2 : 4));
-  zero_now(m->kcache, kElems * (m->kvF16 ? 2 : 4));
-  zero_now(m->vcache, vElems * (m->kvF16 ? 2 : 4));
+  if (m->kvQ4) {
+    m->kv4 = Kv4View{nullptr, std::max(m->nAttn, 1), c.n_head_kv, c.head_dim, m->ctx, kv4_groups(m->ctx)};
+    const int64_t bytes = kv4_bytes(m->kv4.nslot, c.n_head_kv, c.head_dim, m->ctx);
+    m->kv4.base = (uint8_t *)m->ar.alloc(bytes);
+    zero_now(m->kv4.base, bytes);
+    kv4_prepare(c.head_dim);
+    long work = 0;  // (fewer rows split into more records: the most of any pass)
+    for (int b = 1; b <= m->maxBatch; b++) work = std::max(work, kv4_attention_work(m->kv4, 1, b, c.n_head));
+    m->kv4Work = m->ar.alloc(work);
+  } else {
+    // K: [slot][kv head][pos][dim]; V: [slot][kv head][dim][vstride] (vstride = ctx rounded up to 16 positions)
+    m->vstride = (m->ctx + 15) / 16 * 16;
+    const size_t kElems = (size_t)std::max(m->nAttn, 1) * c.n_head_kv * m->ctx * c.head_dim;
+    const size_t vElems = (size_t)std::max(m->nAttn, 1) * c.n_head_kv * c.head_dim * m->vstride;
+    m->kcache = m->ar.alloc(kElems * (m->kvF16 ? 2 : 4));
+    m->vcache = m->ar.alloc(vElems * (m->kvF16 ? 2 : 4));
+    zero_now(m->kcache, kElems * (m->kvF16 ? 2 : 4));
+    zero_now(m->vcache, vElems * (m->kvF16 ? 2 : 4));
+  }
   const int B = m->maxBatch;
   const int inner = m->hybrid ? c.ssm_d_inner : 0;
   if (m->hybrid) {
@@ -486,19 +501,21 @@ static void finish_model(zl_model *m, const float *ropeFreqs) {
   m->v = (float *)m->ar.alloc((size_t)B * kvdim(m) * 4);
   m->hb = (float *)m->ar.alloc((size_t)B * c.n_ff * 4);
   m->logits = (float *)m->ar.alloc((size_t)m->logitsBatch * c.vocab * 4);
-  m->scores = (float *)m->ar.alloc((size_t)B * c.n_head * m->ctx * 4);
   m->qr = (float *)m->ar.alloc((size_t)B * c.n_head * c.head_dim * 4);
-  m->attnChunks = (m->ctx + ATTN_CHUNK - 1) / ATTN_CHUNK;
-  const size_t rows = (size_t)B * c.n_head, ns = c.head_dim / 32;
-  m->attnMl = (double2 *)m->ar.alloc(rows * m->attnChunks * sizeof(double2));
-  if (m->attnChunks > 1) {
-    m->attnRec = (double *)m->ar.alloc(rows * ns * m->attnChunks * ATTN_REC_DOUBLES * 8);
-    m->attnCnt = (uint32_t *)m->ar.alloc(rows * ns * 4);
-    zero_now(m->attnCnt, rows * ns * 4);
-  }
-  if (split) {
-    m->attnNch = (m->ctx + ATTN_SPLIT_C - 1) / ATTN_SPLIT_C;
-    m->attnPart = (double *)m->ar.alloc((size_t)B * c.n_head * m->attnNch * (c.head_dim + 2) * 8);
+  if (!m->kvQ4) {
+    m->scores = (float *)m->ar.alloc((size_t)B * c.n_head * m->ctx * 4);
+    m->attnChunks = (m->ctx + ATTN_CHUNK - 1) / ATTN_CHUNK;
+    const size_t rows = (size_t)B * c.n_head, ns = c.head_dim / 32;
+    m->attnMl = (double2 *)m->ar.alloc(rows * m->attnChunks * sizeof(double2));
+    if (m->attnChunks > 1) {
+      m->attnRec = (double *)m->ar.alloc(rows * ns * m->attnChunks * ATTN_REC_DOUBLES * 8);
+      m->attnCnt = (uint32_t *)m->ar.alloc(rows * ns * 4);
+      zero_now(m->attnCnt, rows * ns * 4);
+    }
+    if (split) {
+      m->attnNch = (m->ctx + ATTN_SPLIT_C - 1) / ATTN_SPLIT_C;
+      m->attnPart = (double *)m->ar.alloc((size_t)B * c.n_head * m->attnNch * (c.head_dim + 2) * 8);
+    }
   }
   const int ld = pad64(std::max(std::max(c.n_embd, inner), std::max(qdim(m), c.n_ff)));
   m->act = alloc_act(m->ar, B, ld, true);
@@ -739,7 +756,14 @@ static void enqueue_forward(zl_model *m, int B, int want) {
       aa.mmMinB = m->attnMmMinB; aa.mmAvMinB = m->attnMmAvMinB; aa.qr = m->qr;
       // a single-token Q8_0 attn_output GEMV quantises the f32 head outputs itself: the attention writes them alone
       if (rg_path({&L.wo}, B)) aa.act.q = nullptr;
-      launch_attention(aa, B, m->st);
+      if (m->kvQ4) {
+        Kv4View slot = m->kv4;
+        slot.base += (int64_t)L.ai * kv4_bytes(1, c.n_head_kv, c.head_dim, m->ctx);
+        slot.nslot = 1;
+        launch_attention_q4(aa, slot, m->kv4Work, B, m->st);
+      } else {
+        launch_attention(aa, B, m->st);
+      }
       gemv_group(m, {{&L.wo, nullptr, 0, nullptr}}, B, EPI_RESID, m->act, m->act.f, m->act.ld);
     }
     ZL_REQUIRE(L.wgate.type == L.wup.type, ZL_ERR_UNSUPPORTED, "ffn_gate and ffn_up must share a type");
@@ -1081,6 +1105,7 @@ static zl_model *new_model(const zl_model_opts *o) {
 // The options of zl_model_ext; returns the context. Scaled positions reach factor times the trained context.
 static int take_ext(zl_model *m, const zl_model_ext *ext, int want_ctx) {
   double most = m->cfg.n_ctx_train;
+  m->kvQ4 = ext && ext->kv_q4;
   if (ext && ext->rope && ext->rope->scaling) {
     zl_rope_opts r = *ext->rope;
     r.n_rot = m->cfg.n_rot; r.base = (double)m->cfg.rope_base; r.freq_factors = nullptr;
@@ -1894,7 +1919,7 @@ int zl_model_config(const zl_model *m, zl_config *out) {
 int zl_model_info_get(const zl_model *m, zl_model_info *out) {
   ZL_API_BEGIN
   ZL_REQUIRE(m && out, ZL_ERR_ARG, "null argument");
-  out->ctx = m->ctx; out->max_batch = m->maxBatch; out->logits_batch = m->logitsBatch; out->kv_f16 = m->kvF16;
+  out->ctx = m->ctx; out->max_batch = m->maxBatch; out->logits_batch = m->logitsBatch; out->kv_f16 = m->kvQ4 ? 2 : m->kvF16;
   out->weight_bytes = m->weightBytes; out->device_bytes = m->ar.bytes;
   out->state_bytes = m->hybrid ? (int64_t)state_bytes(m) : 0;
   out->state_capture_slots = m->capture ? m->capSlots : 0;

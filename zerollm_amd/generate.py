@@ -82,3 +82,32 @@ def generate(model, prompt_ids, max_tokens=256, sample=None, stop_ids=(), signal
             model.forward_batch([tok], logits="last", copy=False)
     finally:
         stats["decodeMs"] = (time.perf_counter() - t1) * 1e3
+
+
+def score(model, ids, start=1, top=0):
+    """How likely the model finds ids[start:]: LogProbs over them (host arrays), each token given all before it, in passes of as
+    many tokens as return their logits. The model keeps ids[:-1] as its context, and starts from what it shares with it."""
+    import numpy as np
+
+    from .ops import LogProbs
+
+    ids = list(ids)
+    if not 1 <= start < len(ids):
+        raise ValueError(f"start must be 1 to {len(ids) - 1} (got {start})")
+    if len(ids) - 1 > model.ctx:
+        raise ValueError(f"{len(ids)} tokens do not fit the context window of {model.ctx}")
+    reuse = min(common_prefix(model.tokens, ids), start - 1)
+    model.truncate(reuse)
+    prefill_tokens(model, ids[:start - 1], start=reuse, want_logits=False, copy=False)
+    step = min(model.max_batch, model.logits_batch)
+    parts = []
+    for i in range(start - 1, len(ids) - 1, step):
+        end = min(len(ids) - 1, i + step)
+        model.forward_batch(ids[i:end], logits="all", copy=False)
+        parts.append(model.logprobs(end - i, tokens=ids[i + 1:end + 1], top=top))
+
+    def join(name):
+        v = [getattr(p, name) for p in parts]
+        return None if v[0] is None else np.concatenate(v)
+
+    return LogProbs(join("logprobs"), join("entropy"), join("top_ids"), join("top_logprobs"))

@@ -3,7 +3,7 @@
 Same members and semantics: forward / forward_batch with logits False|True|'none'|'last'|'all', truncate (positional
 KV bookkeeping; restore + replay for hybrid models), mark_rollback, reset, close (idempotent), and the fields tokens, pos,
 ctx, cfg, max_batch,
-logits_batch, kernels ('hip'), kv. Errors carry the reference's messages ("context full (N tokens)", "token id X out of
+logits_batch, kernels ('hip'), kv (also q4_0 here). Errors carry the reference's messages ("context full (N tokens)", "token id X out of
 range", "batch of B tokens (max M)", "model is closed"). Returned logits are a view over model-owned host memory that
 is valid until the next call, as the reference's are (src/compute/pool.js:133, 143).
 """
@@ -15,6 +15,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import ZLError, call, lib, ptr
+from .ops import LogProbs, rope_opts
 
 ARCH_NAMES = {0: "llama", 1: "qwen2", 2: "qwen3", 3: "qwen35"}
 
@@ -22,8 +23,8 @@ ARCH_NAMES = {0: "llama", 1: "qwen2", 2: "qwen3", 3: "qwen35"}
 def _opts(ctx, kv, max_batch, logits_batch, max_checkpoints=None, checkpoint_every=0, boundary_ids=()):
     """PoolModel.create options; the last three are the hybrid checkpoint policy (src/model/state-checkpoints.js:18-35):
     max_checkpoints None = the default 6, 0 = none."""
-    if kv not in ("f32", "f16"):
-        raise ValueError(f'kv must be f32 or f16 (got "{kv}")')
+    if kv not in ("f32", "f16", "q4_0"):
+        raise ValueError(f'kv must be f32, f16 or q4_0 (got "{kv}")')
     ids = (C.c_int32 * max(1, len(boundary_ids)))(*boundary_ids)
     o = _lib.zl_model_opts(ctx=int(ctx or 0), kv_f16=1 if kv == "f16" else 0, max_batch=int(max_batch or 16),
                            logits_batch=int(logits_batch or 0),
@@ -31,6 +32,17 @@ def _opts(ctx, kv, max_batch, logits_batch, max_checkpoints=None, checkpoint_eve
                            checkpoint_every=int(checkpoint_every or 0), boundary_ids=ids, n_boundary=len(boundary_ids))
     o._ids = ids  # kept alive with the struct
     return o
+
+
+def _ext(kv, rope):
+    """zl_model_ext of a cache in 4 bits or of scaled positions, None without either."""
+    if kv != "q4_0" and rope is None:
+        return None
+    e = _lib.zl_model_ext(kv_q4=1 if kv == "q4_0" else 0)
+    if rope is not None:
+        e._rope = rope_opts(**rope)
+        e.rope = C.pointer(e._rope)
+    return e
 
 
 class HipModel:
@@ -70,22 +82,30 @@ class HipModel:
 
     # ---- construction
     @classmethod
-    def load(cls, path: str, ctx=None, kv="f32", max_batch=16, logits_batch=None, **ck) -> "HipModel":
-        """PoolModel.create over a GGUF file (src/compute/pool.js:33-121). ck: max_checkpoints, checkpoint_every,
-        boundary_ids (hybrid models)."""
+    def load(cls, path: str, ctx=None, kv="f32", max_batch=16, logits_batch=None, rope=None, **ck) -> "HipModel":
+        """PoolModel.create over a GGUF file (src/compute/pool.js:33-121). kv "q4_0" holds keys and values as Q4_0 blocks.
+        rope: positions scaled beyond the trained context, a dict of ops.rope_opts' scaling, factor, orig_ctx, beta_fast,
+        beta_slow, attn_factor; the context may then reach factor times the trained one. ck: max_checkpoints,
+        checkpoint_every, boundary_ids (hybrid models)."""
         h = C.c_void_p()
-        o = _opts(ctx, kv, max_batch, logits_batch, **ck)
-        call("zl_model_load", path.encode(), C.byref(o), C.byref(h))
+        o, e = _opts(ctx, kv, max_batch, logits_batch, **ck), _ext(kv, rope)
+        if e is None:
+            call("zl_model_load", path.encode(), C.byref(o), C.byref(h))
+        else:
+            call("zl_model_load_ext", path.encode(), C.byref(o), C.byref(e), C.byref(h))
         return cls(h, kv)
 
     @classmethod
-    def from_synth(cls, cfg: "_lib.zl_config", tensors, ctx=None, kv="f32", max_batch=16, logits_batch=None,
+    def from_synth(cls, cfg: "_lib.zl_config", tensors, ctx=None, kv="f32", max_batch=16, logits_batch=None, rope=None,
                    **ck) -> "HipModel":
-        """A synthetic model generated in HBM (see zerollm_amd.synth)."""
+        """A synthetic model generated in HBM (see zerollm_amd.synth); kv and rope as load's."""
         h = C.c_void_p()
-        o = _opts(ctx, kv, max_batch, logits_batch, **ck)
+        o, e = _opts(ctx, kv, max_batch, logits_batch, **ck), _ext(kv, rope)
         arr = (_lib.zl_synth_tensor * len(tensors))(*tensors)
-        call("zl_model_synth", C.byref(cfg), arr, len(tensors), C.byref(o), C.byref(h))
+        if e is None:
+            call("zl_model_synth", C.byref(cfg), arr, len(tensors), C.byref(o), C.byref(h))
+        else:
+            call("zl_model_synth_ext", C.byref(cfg), arr, len(tensors), C.byref(o), C.byref(e), C.byref(h))
         return cls(h, kv)
 
     # ---- state
@@ -126,6 +146,28 @@ class HipModel:
         if want == 2:
             return self._logits[:B]
         return self._logits[0] if want else None
+
+    def logprobs(self, n: int = 1, row0: int = 0, tokens=None, top: int = 0) -> LogProbs:
+        """ops.logprobs of rows row0 .. row0 + n of the last pass's logits, as host arrays: of each row the log probability
+        of its entry of tokens (None without), the entropy, the `top` likeliest ids and their log probabilities."""
+        self._check_open()
+        n, top = int(n), int(top)
+        tok = None
+        if tokens is not None:
+            tok = np.ascontiguousarray(tokens, np.int32)
+            if tok.shape != (n,):
+                raise ValueError(f"tokens must be {n} ids (got {tok.shape})")
+        if n < 0 or not 0 <= top <= 64:
+            raise ValueError(f"n must not be negative, top 0 to 64 (got {n}, {top})")
+        out = LogProbs(np.empty(n, np.float32) if tok is not None else None, np.empty(n, np.float32),
+                       np.empty((n, top), np.int32) if top else None, np.empty((n, top), np.float32) if top else None)
+
+        def p(x, ctype):
+            return None if x is None else ptr(x, ctype)
+
+        call("zl_model_logprobs", self._h, int(row0), n, p(tok, C.c_int32), top, p(out.logprobs, C.c_float),
+             p(out.entropy, C.c_float), p(out.top_ids, C.c_int32), p(out.top_logprobs, C.c_float))
+        return out
 
     def truncate(self, n: int) -> int:
         """Roll back to n positions (src/compute/pool.js:278-294): positional KV is bookkeeping; a hybrid model restores
