@@ -207,14 +207,16 @@ __global__ __launch_bounds__(256) void k_logprobs(const LogprobArgs a, int parts
       const uint32_t tv = (uint32_t)(c.t >> 32);
       const float tf = tv ? keyf(tv) : NAN;  // (NaN: every logit is offered)
       if (__ballot(!(mx < tf))) {
+        // the lane's logits at the threshold, one of each lane at a time (read again: an index into registers would be 16 selections)
+        uint32_t mask = 0;
         #pragma unroll
-        for (int j = 0; j < NV; j++)
-          #pragma unroll
-          for (int e = 0; e < VE; e++) {
-            if (!__ballot(!(v[j * VE + e] < tf))) continue;
-            const int i = t0 + (j * 256 + tid) * VE + e;
-            c.offer(i >= off && i < i1, rank_key(v[j * VE + e], i - off), lane);
-          }
+        for (int e = 0; e < 16; e++) mask |= !(v[e] < tf) ? 1u << e : 0u;
+        while (__ballot(mask != 0)) {
+          const int e = __ffs((int)mask) - 1, i = t0 + ((e / VE) * 256 + tid) * VE + e % VE;
+          const bool have = mask && i >= off && i < i1;
+          c.offer(have, have ? rank_key(load_value<TYPE>(base[i]), i - off) : 0, lane);
+          mask &= mask - 1;
+        }
       }
     }
   }
