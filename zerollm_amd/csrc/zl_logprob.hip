@@ -5,10 +5,11 @@
 // along, so that nothing cancels. -inf counts for nothing; NaN and +inf make l NaN, and with it every float output.
 //
 // Alternatives are 64-bit numbers, the ordered value above the complement of the id, so that a larger one is a better one
-// and equal values go to the lowest id. Every wave keeps a list of candidates in LDS with a threshold that the n_top-th
-// best so far has reached: a lane whose 16 logits hold nothing at the threshold costs one comparison. The first threshold is
-// the n_top-th largest of the lanes' maxima. Full lists are cut to their n_top best (a search for the n_top-th largest
-// number, bit by bit with ballots).
+// and equal values go to the lowest id. The pass keeps each lane's largest logit; at least n_top logits are at or above the
+// n_top-th largest of a block's. The lanes whose largest reaches that threshold, n_top of 256 but for ties, have their pieces read
+// again (from the caches), and what reaches it is listed in LDS. Full lists are cut to their n_top best (a search for the
+// n_top-th largest number, bit by bit with ballots). (Lists filled during the pass, under a threshold of what came before: 2048 x
+// 32000 bf16, 5 alternatives, 46 us.)
 //
 // Bound by HBM (each logit is read once) for many rows, by the latency of two launches for few.
 #include "zl_ops.h"
@@ -57,16 +58,6 @@ struct Candidates {
   rank_t *buf;
   int n, k;
   rank_t t;
-  // The first threshold: the k-th largest of the lanes' largest values kx (0: a lane that has none).
-  __device__ __forceinline__ void start(uint32_t kx) {
-    uint32_t kth = 0;
-    for (int bit = 31; bit >= 0; bit--) {
-      const int cnt = __popcll(__ballot(kx >= (kth | (1u << bit))));
-      if (cnt >= k) kth |= 1u << bit;
-      if (cnt == k) break;
-    }
-    t = kth ? ((rank_t)kth << 32) - 1 : 0;
-  }
   // Cut to the k largest (n > k). Entries are distinct, none is 0.
   template <int N>
   __device__ __forceinline__ void cut_n(int lane) {
@@ -109,9 +100,33 @@ struct Candidates {
   }
 };
 
+// The k-th largest of the block's 256 numbers, in all lanes; keys: 1 KB of LDS, free again afterwards.
+__device__ __forceinline__ uint32_t block_threshold(uint32_t key, int k, uint32_t *keys, int lane, int wave) {
+  keys[64 * wave + lane] = key;
+  __syncthreads();
+  uint32_t x[4], v = 0;
+  if (wave == 0) {
+    #pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = keys[lane + 64 * i];
+    for (int bit = 31; bit >= 0; bit--) {
+      int cnt = 0;
+      #pragma unroll
+      for (int i = 0; i < 4; i++) cnt += __popcll(__ballot(x[i] >= (v | (1u << bit))));
+      if (cnt >= k) v |= 1u << bit;
+      if (cnt == k) break;
+    }
+  }
+  __syncthreads();
+  if (wave == 0 && lane == 0) keys[0] = v;
+  __syncthreads();
+  v = keys[0];
+  __syncthreads();
+  return v;
+}
+
 // The k best of the four waves' lists, in wave 0's list, by the whole block.
 __device__ __forceinline__ void merge_waves(Candidates &c, rank_t (*lists)[LP_CAP], int *counts, int lane, int wave) {
-  if (c.n > (wave == 0 ? c.k : 64)) c.cut(lane);  // (wave 0 for its threshold, the others to fit one offer)
+  if (c.n > 64) c.cut(lane);  // (to fit one offer)
   if (lane == 0) counts[wave] = c.n;
   __syncthreads();
   if (wave == 0) {
@@ -164,7 +179,7 @@ __global__ __launch_bounds__(256) void k_logprobs(const LogprobArgs a, int parts
   const int i0 = part * span, i1 = min(a.vocab + off, i0 + span);
   RowSum s;
   Candidates c{lists[wave], 0, a.ntop, 0};
-  bool first = true;
+  float lm = -INFINITY;  // the lane's largest logit
   for (int t0 = i0; t0 < i1; t0 += LP_TILE) {
     float v[16];
     #pragma unroll
@@ -190,33 +205,39 @@ __global__ __launch_bounds__(256) void k_logprobs(const LogprobArgs a, int parts
       s.l += p;
       s.e = fmaf(p, fmaxf(d, -3.0e38f), s.e);
     }
-    if (a.ntop) {
-      if (first) {
-        // at least ntop logits are at or above the ntop-th largest of the lanes' maxima (0: a lane with none but NaN)
-        uint32_t kx = 0;
-        #pragma unroll
-        for (int j = 0; j < NV; j++)
+    lm = fmaxf(lm, mx);
+  }
+  if (a.ntop) {
+    // no threshold where it is -inf: such lanes may hold nothing
+    const uint32_t none = fkey(-INFINITY), kth = block_threshold(fkey(lm), a.ntop, (uint32_t *)lists[3], lane, wave);
+    c.t = kth > none ? ((rank_t)kth << 32) - 1 : 0;
+    const float tf = c.t ? keyf(kth) : NAN;  // (NaN: every logit is offered)
+    // the lanes that have something at it: their pieces of every tile, a piece per lane
+    const bool in = !(lm < tf);
+    const unsigned long long who = __ballot(in);
+    const int rank = __popcll(who & ((1ull << lane) - 1)), held = __popcll(who);
+    const int list = __builtin_amdgcn_ds_permute(4 * (in ? rank : held + lane - rank), lane);  // the lanes in order, those first
+    const int tiles = (i1 - i0 + LP_TILE - 1) / LP_TILE;
+    for (int p0 = 0; p0 < held * tiles; p0 += 64) {
+      const int p = p0 + lane, t0 = i0 + p % tiles * LP_TILE, from = wave * 64 + __shfl(list, min(p / tiles, 63), 64);
+      const int end = p < held * tiles ? i1 : 0;
+      uint32_t mask = 0;
+      #pragma unroll
+      for (int j = 0; j < NV; j++) {
+        const int i = t0 + (j * 256 + from) * VE;
+        if (i >= off && i + VE <= end) {
+          const vec u = *(const vec *)(base + i);
           #pragma unroll
-          for (int e = 0; e < VE; e++) {
-            const int i = t0 + (j * 256 + tid) * VE + e;
-            if (i >= off && i < i1 && v[j * VE + e] == v[j * VE + e]) kx = max(kx, fkey(v[j * VE + e]));
-          }
-        c.start(kx);
-        first = false;
-      }
-      const uint32_t tv = (uint32_t)(c.t >> 32);
-      const float tf = tv ? keyf(tv) : NAN;  // (NaN: every logit is offered)
-      if (__ballot(!(mx < tf))) {
-        // the lane's logits at the threshold, one of each lane at a time (read again: an index into registers would be 16 selections)
-        uint32_t mask = 0;
-        #pragma unroll
-        for (int e = 0; e < 16; e++) mask |= !(v[e] < tf) ? 1u << e : 0u;
-        while (__ballot(mask != 0)) {
-          const int e = __ffs((int)mask) - 1, i = t0 + ((e / VE) * 256 + tid) * VE + e % VE;
-          const bool have = mask && i >= off && i < i1;
-          c.offer(have, have ? rank_key(load_value<TYPE>(base[i]), i - off) : 0, lane);
-          mask &= mask - 1;
+          for (int e = 0; e < VE; e++) mask |= !(load_value<TYPE>(u[e]) < tf) ? 1u << (j * VE + e) : 0u;
+        } else {
+          #pragma unroll
+          for (int e = 0; e < VE; e++) mask |= i + e >= off && i + e < end && !(load_value<TYPE>(base[i + e]) < tf) ? 1u << (j * VE + e) : 0u;
         }
+      }
+      while (__ballot(mask != 0)) {
+        const int e = __ffs((int)mask) - 1, i = t0 + ((e / VE) * 256 + from) * VE + e % VE;
+        c.offer(mask != 0, mask ? rank_key(load_value<TYPE>(base[i]), i - off) : 0, lane);
+        mask &= mask - 1;
       }
     }
   }
@@ -251,11 +272,14 @@ __global__ __launch_bounds__(256) void k_logprobs_join(const LogprobArgs a, int 
   if (a.ntop) {
     const rank_t *top = part_top(a, parts, row);
     const int total = parts * a.ntop;
+    rank_t best = 0;
+    for (int i = tid; i < total; i += 256) best = max(best, top[i]);
+    const uint32_t kth = block_threshold((uint32_t)(best >> 32), a.ntop, (uint32_t *)lists[3], lane, wave);
+    c.t = kth ? ((rank_t)kth << 32) - 1 : 0;
     for (int i0 = 0; i0 < total; i0 += 1024) {
       rank_t x[4];
       #pragma unroll
       for (int j = 0; j < 4; j++) x[j] = i0 + 256 * j + tid < total ? top[i0 + 256 * j + tid] : 0;
-      if (i0 == 0) c.start(max(max((uint32_t)(x[0] >> 32), (uint32_t)(x[1] >> 32)), max((uint32_t)(x[2] >> 32), (uint32_t)(x[3] >> 32))));
       #pragma unroll
       for (int j = 0; j < 4; j++) c.offer(x[j] != 0, x[j], lane);
     }
