@@ -211,9 +211,8 @@ __global__ __launch_bounds__(256) void k_logprobs(const LogprobArgs a, int parts
     // no threshold where it is -inf: such lanes may hold nothing
     const uint32_t none = fkey(-INFINITY), kth = block_threshold(fkey(lm), a.ntop, (uint32_t *)lists[3], lane, wave);
     c.t = kth > none ? ((rank_t)kth << 32) - 1 : 0;
-    const float tf = c.t ? keyf(kth) : NAN;  // (NaN: every logit is offered)
     // the lanes that have something at it: their pieces of every tile, a piece per lane
-    const bool in = !(lm < tf);
+    const bool in = !c.t || lm >= keyf(kth);
     const unsigned long long who = __ballot(in);
     const int rank = __popcll(who & ((1ull << lane) - 1)), held = __popcll(who);
     const int list = __builtin_amdgcn_ds_permute(4 * (in ? rank : held + lane - rank), lane);  // the lanes in order, those first
@@ -221,6 +220,11 @@ __global__ __launch_bounds__(256) void k_logprobs(const LogprobArgs a, int parts
     for (int p0 = 0; p0 < held * tiles; p0 += 64) {
       const int p = p0 + lane, t0 = i0 + p % tiles * LP_TILE, from = wave * 64 + __shfl(list, min(p / tiles, 63), 64);
       const int end = p < held * tiles ? i1 : 0;
+      // what is at the least number above the threshold, which cuts raise: its value or more, among its equals its id or before
+      const rank_t least = c.t + 1;
+      const uint32_t tv = (uint32_t)(least >> 32), ti = ~(uint32_t)least;
+      const float tf = tv ? keyf(tv) : NAN;  // (NaN: everything)
+      auto may = [&](float v, int i) { return !(v < tf) && !(v == tf && (uint32_t)(i - off) > ti); };
       uint32_t mask = 0;
       #pragma unroll
       for (int j = 0; j < NV; j++) {
@@ -228,10 +232,10 @@ __global__ __launch_bounds__(256) void k_logprobs(const LogprobArgs a, int parts
         if (i >= off && i + VE <= end) {
           const vec u = *(const vec *)(base + i);
           #pragma unroll
-          for (int e = 0; e < VE; e++) mask |= !(load_value<TYPE>(u[e]) < tf) ? 1u << (j * VE + e) : 0u;
+          for (int e = 0; e < VE; e++) mask |= may(load_value<TYPE>(u[e]), i + e) ? 1u << (j * VE + e) : 0u;
         } else {
           #pragma unroll
-          for (int e = 0; e < VE; e++) mask |= i + e >= off && i + e < end && !(load_value<TYPE>(base[i + e]) < tf) ? 1u << (j * VE + e) : 0u;
+          for (int e = 0; e < VE; e++) mask |= i + e >= off && i + e < end && may(load_value<TYPE>(base[i + e]), i + e) ? 1u << (j * VE + e) : 0u;
         }
       }
       while (__ballot(mask != 0)) {
