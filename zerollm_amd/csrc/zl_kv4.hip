@@ -600,19 +600,23 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 // positions took 48 us against 41, the waves waiting for each other and for the fold.) A token
 // of 32 heads of 128 over 8 KV heads after 131000 positions: 44 us, 151 MB at 3.4 TB/s, near a read's own rate (4.1). 9 tokens after
 // 16384: 27 us, bound by the vector units and by the waves' start and end.
-template <int NB, int TYPE>
-__global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4Attn a, int tiles, int gx) {
+template <int NB, int TYPE, bool MANY>
+__global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
   constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
-  long group;  // [sequence][KV head][block of chunks]
-  int tile;
-  if (!dealt((long)gx * a.c.nkv * a.b.nseq, tiles, &group, &tile)) return;
+  // the wave's tile, and its first chunk (MANY: part) and the step to the next
+  long group;  // [sequence][KV head][block of chunks (a part)]
+  int tile, c0, step;
+  if (!dealt((long)gx * a.c.nkv * a.b.nseq, MANY ? (tiles + 3) / 4 : tiles, &group, &tile)) return;
+  if (MANY) tile = tile * 4 + wave, c0 = (int)(group % gx), step = gx;
+  else c0 = (int)(group % gx) * 4 + wave, step = gx * 4;
   const Tile tl(a, (int)(group / gx / a.c.nkv), (int)(group / gx % a.c.nkv), tile * 16);
   int tok, head;
   const int last = tl.last(a, n, &tok, &head);
-  const int most = __builtin_amdgcn_readfirstlane(wave_max(last)), c0 = (int)(group % gx) * 4 + wave, step = gx * 4;
-  const int unit = record_len(a, tl.s);
+  const int most = __builtin_amdgcn_readfirstlane(wave_max(last));
+  const int unit = MANY ? PART : record_len(a, tl.s);
+  __shared__ f4 part[MANY ? 4 : 1][MANY ? 2 * NB : 1][64];  // MANY: the part's o, a column per lane (registers hold one sum, not two)
   Sum<8 * NB> u;
   u.clear();
   if (most < (long)c0 * unit) {
@@ -636,6 +640,11 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
   for (int c = c0; (long)c * unit <= most; c += step) {
     const int ns = min(unit / SPAN, (most - c * unit) / SPAN + 1);
     u.clear();
+    float pm = -INFINITY, pl = 0.0f;
+    if (MANY) {
+      #pragma unroll
+      for (int j = 0; j < 2 * NB; j++) part[wave][j][lane] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     for (int sp = 0; sp < ns; sp++) {
       const int p0 = c * unit + sp * SPAN, lim = last - p0;
       const int pn = sp + 1 < ns ? p0 + SPAN : (long)(c + step) * unit <= most ? (c + step) * unit : p0;  // (the last one is read again, for nothing)
@@ -684,6 +693,27 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_chunks(const Kv4At
         #pragma unroll
         for (int v = 0; v < 4; v++) r.o[4 * j + v] = o[j][v];
       u.fold(r);
+      if (MANY && ((sp & (CHUNK / SPAN - 1)) == CHUNK / SPAN - 1 || sp == ns - 1)) {
+        const float M = fmaxf(pm, u.m), ref = M == -INFINITY ? 0.0f : M, x = exp2_(pm - ref), y = exp2_(u.m - ref);
+        pm = M;
+        pl = fmaf(pl, x, u.l * y);
+        #pragma unroll
+        for (int j = 0; j < 2 * NB; j++) {
+          f4 o = part[wave][j][lane];
+          #pragma unroll
+          for (int v = 0; v < 4; v++) o[v] = fmaf(o[v], x, u.o[4 * j + v] * y);
+          part[wave][j][lane] = o;
+        }
+        u.clear();
+      }
+    }
+    if (MANY) {
+      u.m = pm;
+      u.l = pl;
+      #pragma unroll
+      for (int j = 0; j < 2 * NB; j++)
+        #pragma unroll
+        for (int v = 0; v < 4; v++) u.o[4 * j + v] = part[wave][j][lane][v];
     }
     leave<NB, TYPE>(a, tl, last, tok, head, c, c * unit, u, g);
   }
@@ -859,175 +889,6 @@ __global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a, const O
   for (int i = 0; i < NB; i++) out.emit(s, tok, head, 32 * i + fl, last >= 0 ? f.o[i] / f.l : last == ROW_NONE ? 0.0f : NAN);
 }
 
-// Many rows: a block takes PW waves of a tile of 16 rows each through the spans of one part. The waves unpack a span's
-// codes to f16 operands in LDS, a share each, and read all of them, so that a span is unpacked once for 16 PW rows; the
-// next span's words are on their way meanwhile, and two buffers let the block meet once per span. A wave folds its rows'
-// spans, chunks and part in registers; the parts' records are joined.
-template <int NB>
-struct SpanOperands {
-  h8 k[2][2 * NB][64], v[2][2 * NB][64];  // [record][word][lane]
-  u4 ks[2][4 * NB], vs[2][4 * NB];        // the records' scales as they are
-};
-constexpr int part_waves(int nb) { return nb <= 4 ? 8 : 4; }  // (heads of 256: registers for one wave a SIMD)
-template <int NB, int TYPE>
-__global__ __launch_bounds__(64 * part_waves(NB)) void k_kv4_parts(const Kv4Attn a, int blocks) {
-  constexpr int HD = 32 * NB, REC = 36 * HD, RT = 1, PW = part_waves(NB), NW = 2 * NB / PW > 0 ? 2 * NB / PW : 1;  // NW: a lane's 16-byte loads of words
-  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ;
-  extern __shared__ __align__(16) uint8_t lds_raw[];
-  SpanOperands<NB> *buf = (SpanOperands<NB> *)lds_raw;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
-  long group;  // [sequence][KV head][part]
-  int block;
-  if (!dealt((long)a.nrec * a.c.nkv * a.b.nseq, blocks, &group, &block)) return;
-  const int part = (int)(group % a.nrec), row0 = block * (16 * PW) + wave * (16 * RT);
-  int last[RT], tok[RT], head[RT], most = ROW_ABSENT, blockmost;
-  const Tile tl(a, (int)(group / a.nrec / a.c.nkv), (int)(group / a.nrec % a.c.nkv), 0);
-  #pragma unroll
-  for (int r = 0; r < RT; r++) {
-    last[r] = tl.last(a, row0 + 16 * r + n, &tok[r], &head[r]);
-    most = max(most, wave_max(last[r]));
-  }
-  {
-    int *red = (int *)lds_raw;
-    if (lane == 0) red[wave] = most;
-    __syncthreads();
-    blockmost = red[0];
-    for (int w = 1; w < PW; w++) blockmost = max(blockmost, red[w]);
-    __syncthreads();
-  }
-  Sum<8 * NB> f[RT], u[RT];
-  #pragma unroll
-  for (int r = 0; r < RT; r++) f[r].clear(), u[r].clear();
-  if (blockmost < part * PART) {
-    if (a.direct)
-      for (int r = 0; r < RT; r++) leave<NB, TYPE>(a, tl, last[r], tok[r], head[r], 0, 0, f[r], g);
-    return;
-  }
-  typedef typename ValueOf<TYPE>::t T;
-  const Unpack uk;
-  // the wave's share of a span: records' key words then value words, NW 16-byte loads (of NB / 2 per record and kind)
-  const int npos = min(blockmost + 1, (part + 1) * PART), nspan = (npos - part * PART + SPAN - 1) / SPAN;
-  const uint8_t *base = record_of(a.c, tl.slot, tl.kvh, (long)part * (PART / KV4_GROUP));
-  u4 words[NW], scales;
-  auto load = [&](int sp) {
-    const uint8_t *rec = base + (long)sp * (2 * REC);
-    #pragma unroll
-    for (int x = 0; x < NW; x++) {
-      const int idx = wave * NW + x, i = idx / NB, kv = idx / (NB / 2) & 1, j = idx % (NB / 2);
-      if (idx >= 2 * NB) break;
-      words[x] = ((const u4 *)(rec + i * REC + kv * 16 * HD))[j * 64 + lane];
-    }
-    // 16 NB pieces of scales: [record][keys | values][4 NB]
-    const int e = tid, i = e / (8 * NB), r = e % (8 * NB);
-    if (e < 16 * NB) scales = ((const u4 *)(rec + i * REC + 32 * HD))[r];
-  };
-  auto stage = [&](SpanOperands<NB> &d) {
-    #pragma unroll
-    for (int x = 0; x < NW; x++) {
-      const int idx = wave * NW + x, i = idx / NB, kv = idx / (NB / 2) & 1, j = idx % (NB / 2);
-      if (idx >= 2 * NB) break;
-      #pragma unroll
-      for (int y = 0; y < 4; y++) (kv ? d.v : d.k)[i][4 * j + y][lane] = unpack8<TINY>(words[x][y], uk);
-    }
-    const int e = tid, i = e / (8 * NB), r = e % (8 * NB);
-    if (e < 16 * NB) (r < 4 * NB ? d.ks : d.vs)[i][r % (4 * NB)] = scales;
-  };
-  load(0);
-  Queries<NB, TINY> q[RT];
-  #pragma unroll
-  for (int r = 0; r < RT; r++) {
-    float qv[NB][8];
-    fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last[r] >= 0 ? tok[r] * a.q.tok + head[r] * a.q.head : 0), a.qvec, lane);
-    set_queries<NB, TINY>(q[r], qv, a.scale);
-  }
-  stage(buf[0]);
-  load(min(1, nspan - 1));
-  __syncthreads();
-  for (int sp = 0; sp < nspan; sp++) {
-    const SpanOperands<NB> &d = buf[sp & 1];
-    const int p0 = part * PART + sp * SPAN;
-    if (p0 <= most) {
-      f4 s[RT][2][2];
-      #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        u4 ks[NB];
-        #pragma unroll
-        for (int j = 0; j < NB; j++) ks[j] = d.ks[i][g * NB + j];
-        #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          h8 k[NB];
-          #pragma unroll
-          for (int b = 0; b < NB; b++) k[b] = d.k[i][t * NB + b][lane];
-          #pragma unroll
-          for (int r = 0; r < RT; r++) s[r][i][t] = tile_scores<NB, LOQ>([&](int b) { return k[b]; }, ks, t, q[r]);
-        }
-      }
-      Sum<8 * NB> z[RT];
-      bool masked[RT];
-      Weights<LOW> pw[RT];
-      #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        masked[r] = __ballot(last[r] - p0 < SPAN - 1) != 0;
-        if (masked[r]) mask_scores(s[r], last[r] - p0, g);
-        span_softmax<LOW>(s[r], q[r].c, pw[r], z[r].m, z[r].l);
-      }
-      f4 o[RT][2 * NB], wsum[RT][NB];
-      #pragma unroll
-      for (int r = 0; r < RT; r++)
-        #pragma unroll
-        for (int j = 0; j < 2 * NB; j++) o[r][j] = f4{0.0f, 0.0f, 0.0f, 0.0f}, wsum[r][j >> 1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-      #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        u4 vs[RT][NB];
-        #pragma unroll
-        for (int j = 0; j < NB; j++) vs[0][j] = d.vs[i][g * NB + j];
-        #pragma unroll
-        for (int r = RT - 1; r >= 0; r--) {
-          #pragma unroll
-          for (int j = 0; j < NB; j++) vs[r][j] = vs[0][j];
-          if (masked[r]) mask_scales<NB>(vs[r], i, last[r] - p0, g);
-        }
-        #pragma unroll
-        for (int b = 0; b < NB; b++) {
-          const h8 x0 = d.v[i][2 * b][lane], x1 = d.v[i][2 * b + 1][lane];
-          #pragma unroll
-          for (int r = 0; r < RT; r++) {
-            h8 hi, lo;
-            weigh<NB, LOW>(pw[r], vs[r], i, b, hi, lo);
-            weighted_sums<LOW, TINY>(o[r][2 * b], o[r][2 * b + 1], wsum[r][b], x0, x1, hi, lo);
-          }
-        }
-      }
-      if (TINY) {
-        #pragma unroll
-        for (int r = 0; r < RT; r++) take_off<NB>(o[r], wsum[r]);
-      }
-      #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        #pragma unroll
-        for (int j = 0; j < 2 * NB; j++)
-          #pragma unroll
-          for (int v = 0; v < 4; v++) z[r].o[4 * j + v] = o[r][j][v];
-        u[r].fold(z[r]);
-      }
-    }
-    if ((sp & (CHUNK / SPAN - 1)) == CHUNK / SPAN - 1 || sp == nspan - 1) {
-      #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        f[r].fold(u[r]);
-        u[r].clear();
-      }
-    }
-    if (sp + 1 < nspan) {
-      stage(buf[(sp + 1) & 1]);
-      load(min(sp + 2, nspan - 1));
-    }
-    __syncthreads();
-  }
-  #pragma unroll
-  for (int r = 0; r < RT; r++) leave<NB, TYPE>(a, tl, last[r], tok[r], head[r], part, part * PART, f[r], g);
-}
-
 // Tiles of 16 rows times KV heads times sequences.
 static long tile_count(const Kv4View &c, int nseq, int ntok, int nhead) { return ((long)ntok * (nhead / c.nkv) + 15) / 16 * c.nkv * nseq; }
 // Whether a call's rows fill the GPU with a wave per (tile, part).
@@ -1053,16 +914,17 @@ static void launch_attention_k(Kv4Attn a, const OUT &out, bool direct, hipStream
   a.qvec = whole_pieces(a.q, TYPE);
   a.direct = direct && a.nrec == 1;
   const long rows = (long)a.b.ntok * group;
+  const int tiles = (int)((rows + 15) / 16);
+  // waves up to two a SIMD (all on the GPU at once, whichever CUs the blocks are dealt to), each with an even share of the
+  // parts (chunks) beyond; or of spans
+  const int units = many ? a.nrec : (int)((a.c.cap + CHUNK - 1) / CHUNK);
+  const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (units * y + 2047) / 2048;
   if (many) {
-    constexpr int PW = part_waves(NB);
-    const long nb = (rows + 16 * PW - 1) / (16 * PW);
-    hipLaunchKernelGGL((k_kv4_parts<NB, TYPE>), dim3((unsigned)deal_blocks((long)a.nrec * a.c.nkv * a.b.nseq, (int)nb)), dim3(64 * PW), 2 * sizeof(SpanOperands<NB>), st, a, (int)nb);
+    const int gx = (int)((units + rounds - 1) / rounds);
+    hipLaunchKernelGGL((k_kv4_rows<NB, TYPE, true>), dim3((unsigned)deal_blocks((long)gx * a.c.nkv * a.b.nseq, (tiles + 3) / 4)), dim3(256), 0, st, a, tiles, gx);
   } else {
-    // waves of chunks up to two a SIMD, each with an even share of the chunks beyond; or of spans
-    const int tiles = (int)((rows + 15) / 16), nch = (int)((a.c.cap + CHUNK - 1) / CHUNK);
-    const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (nch * y + 2047) / 2048;
-    const int gx = std::max((int)((nch + 4 * rounds - 1) / (4 * rounds)), (a.spanmax + 3) / 4);
-    hipLaunchKernelGGL((k_kv4_chunks<NB, TYPE>), dim3((unsigned)deal_blocks((long)gx * a.c.nkv * a.b.nseq, tiles)), dim3(256), 0, st, a, tiles, gx);
+    const int gx = std::max((int)((units + 4 * rounds - 1) / (4 * rounds)), (a.spanmax + 3) / 4);
+    hipLaunchKernelGGL((k_kv4_rows<NB, TYPE, false>), dim3((unsigned)deal_blocks((long)gx * a.c.nkv * a.b.nseq, tiles)), dim3(256), 0, st, a, tiles, gx);
   }
   ZL_HIP(hipGetLastError());
   if (!a.direct) {
@@ -1072,23 +934,6 @@ static void launch_attention_k(Kv4Attn a, const OUT &out, bool direct, hipStream
     else hipLaunchKernelGGL((k_kv4_join_chunks<8, OUT>), dim3((unsigned)n, NB), dim3(256), 0, st, a, out);
     ZL_HIP(hipGetLastError());
   }
-}
-
-// Dynamic LDS above 64 KB is requested per kernel, once per GPU, when a cache is created: no launch changes an attribute.
-template <int NB, int TYPE>
-static void prepare_k() {
-  ZL_HIP(hipFuncSetAttribute((const void *)k_kv4_parts<NB, TYPE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * sizeof(SpanOperands<NB>))));
-}
-template <int NB>
-static void prepare_nb() {
-  prepare_k<NB, T_F32>();
-  prepare_k<NB, T_F16>();
-  prepare_k<NB, T_BF16>();
-}
-void kv4_prepare(int hd) {
-  if (hd == 64) prepare_nb<2>();
-  else if (hd == 128) prepare_nb<4>();
-  else prepare_nb<8>();
 }
 
 template <int NB>

@@ -78,7 +78,6 @@ int zl_kv4_create(int n_slot, int n_head_kv, int head_dim, int64_t capacity, zl_
   c->dev = device();
   OnDevice on(c->dev);
   c->v.nslot = n_slot; c->v.nkv = n_head_kv; c->v.hd = head_dim; c->v.cap = capacity;
-  kv4_prepare(head_dim);
   c->v.ngroup = kv4_groups(capacity);
   c->bytes = kv4_bytes(n_slot, n_head_kv, head_dim, capacity);
   ZL_HIP(hipMalloc(&c->v.base, c->bytes));

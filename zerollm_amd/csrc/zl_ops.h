@@ -107,7 +107,6 @@ struct Kv4Attn {
   int nrec, spanmax;
   bool qvec, direct;  // direct: no records, a row's only ones are its output
 };
-void kv4_prepare(int hd);  // once before launches of this head size
 long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead);
 void launch_kv4_attention(const Kv4Attn &a, int type, hipStream_t st);
 // f32 queries of one sequence, outputs to a model's rows (a.out is not used).

@@ -461,7 +461,6 @@ static void finish_model(zl_model *m, const float *ropeFreqs) {
     const int64_t bytes = kv4_bytes(m->kv4.nslot, c.n_head_kv, c.head_dim, m->ctx);
     m->kv4.base = (uint8_t *)m->ar.alloc(bytes);
     zero_now(m->kv4.base, bytes);
-    kv4_prepare(c.head_dim);
     long work = 0;  // (fewer rows split into more records: the most of any pass)
     for (int b = 1; b <= m->maxBatch; b++) work = std::max(work, kv4_attention_work(m->kv4, 1, b, c.n_head));
     m->kv4Work = m->ar.alloc(work);
