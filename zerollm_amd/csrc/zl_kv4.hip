@@ -592,14 +592,18 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
   if (g == 0) *record_ml(a, row, rec) = make_float2(f.m, f.l);
 }
 
-// Few rows: a wave takes one tile of 16 rows and a chunk at a time, span by span, and leaves the chunk's record; no wave waits
-// for another. Sequences of so few spans that a wave for each does not overfill the GPU (a.spanmax, by the call's tiles) leave
-// a record per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 8.5). The next
-// span's keys are requested when the scores are done with this one's, its values after the weighted sums, so that the loads run
-// under the rest. (A chunk of 512 per block, one span per wave, folded in LDS behind a barrier: 9 tokens of 32 heads after 16384
-// positions took 48 us against 41, the waves waiting for each other and for the fold.) A token
-// of 32 heads of 128 over 8 KV heads after 131000 positions: 44 us, 151 MB at 3.4 TB/s, near a read's own rate (4.1). 9 tokens after
-// 16384: 27 us, bound by the vector units and by the waves' start and end.
+// A wave takes one tile of 16 rows through chunks (few rows) or parts (MANY), span by span, and leaves the piece's record; no wave
+// waits for another. The next span's keys are requested when the scores are done with this one's, its values after the weighted
+// sums, so that the loads run under the rest. (A chunk of 512 per block, one span per wave, folded in LDS behind a barrier: 9 tokens
+// of 32 heads after 16384 positions 48 us against 41. Eight waves of a block sharing spans unpacked into LDS, one meeting a span:
+// 256 tokens after 12000 positions 240 us against 189.)
+// Few rows: sequences of so few spans that a wave for each does not overfill the GPU (a.spanmax, by the call's tiles) leave a record
+// per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 8.5). A token of 32 heads of
+// 128 over 8 KV heads after 131000 positions: 44 us, 151 MB at 3.4 TB/s, near a read's own rate (4.1). 9 tokens after 16384: 27 us,
+// bound by the vector units, 1.5 waves a SIMD, and by the waves' start and end.
+// MANY: the block's waves have neighbouring tiles of the same part, whose records they read at about the same time. 256 tokens of 32
+// heads over 8 after 12000 positions, f16: 189 us, bound by the vector units: 720 vector instructions and 63 matrix ones a span of a
+// tile, 4300 cycles where those alone are 3200, with two waves a SIMD to hide the matrix instructions' latency.
 template <int NB, int TYPE, bool MANY>
 __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
@@ -891,8 +895,18 @@ __global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a, const O
 
 // Tiles of 16 rows times KV heads times sequences.
 static long tile_count(const Kv4View &c, int nseq, int ntok, int nhead) { return ((long)ntok * (nhead / c.nkv) + 15) / 16 * c.nkv * nseq; }
-// Whether a call's rows fill the GPU with a wave per (tile, part).
-static bool many_rows(const Kv4View &c, int nseq, int ntok, int nhead) { return tile_count(c, nseq, ntok, nhead) >= 128; }
+// Whether a call takes a wave per (tile, part): where they fill the GPU's SIMDs, and there are enough rows that the records of chunks
+// would cost more than the longer runs. (Queries of 32 heads over 8, us, records of chunks : of parts, 16 tokens a call = 32 tiles:
+//   after    16 tokens  32        48        64        128
+//   1000     23 : 42    32 : 42   40 : 42   43 : 42   57 : 45
+//   4000     30 : 42    38 : 44   42 : 44   47 : 44   78 : 66
+//   16000    36 : 47    55 : 48   87 : 70   91 : 71   164 : 125
+//   60000    114 : 83   215 : 136 356 : 187 433 : 239 882 : 443.) The cache's capacity stands for the length, which the host does
+// not know; with fewer tiles a short sequence in a large cache would lose more than a long one gains.
+static bool many_rows(const Kv4View &c, int nseq, int ntok, int nhead) {
+  const long tiles = tile_count(c, nseq, ntok, nhead);
+  return tiles >= 128 || (tiles >= 32 && tiles * ((c.cap + PART - 1) / PART) >= 1024);
+}
 // Spans of a sequence up to which its rows have a record per span: as many as give about two waves a SIMD.
 static int span_max(const Kv4View &c, long tiles) { return (int)std::min((c.cap + SPAN - 1) / SPAN, 2048 / tiles); }
 static int record_count(const Kv4View &c, int nseq, int ntok, int nhead) {
