@@ -221,8 +221,9 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 // The eight codes of a word as f16 operands: pair r of (word >> 4 r).
 // TINY: as they lie, f16 denormals of code 2^-24, which the matrix cores take (16 cycles of a SIMD a word); the 2^24 and the
-// 8 to be taken off follow the sums. Sums of codes are larger than sums of codes less 8, and they lose bits: 7e-6 of an output
-// against 2e-7, so this is for 16-bit rows, whose own rounding is 30 times that.
+// 8 to be taken off follow the sums. Sums of codes are larger than sums of codes less 8, and lose bits: 7e-6 of an output from f32
+// rows against 2e-7, and where 131000 values cancel to 1 in 360 of their size, 2e-4 of it, as much as an f16 output's own rounding.
+// So this is for the scores of 16-bit rows and the sums of bf16 ones.
 // Else: less 8, under the exponent of 1024 and less 1032 (40 cycles a word).
 // The constants are in vector registers: a 32-bit operation takes 2 cycles of a SIMD from two waves' vector operands and 4 with a
 // scalar one, and and-or takes a single scalar one.
@@ -607,7 +608,7 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 template <int NB, int TYPE, bool MANY>
 __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
-  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
+  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ, TINYV = TYPE == T_BF16, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   // the wave's tile, and its first chunk (MANY: part) and the step to the next
   long group;  // [sequence][KV head][block of chunks (a part)]
@@ -684,14 +685,14 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
         for (int b = 0; b < NB; b++) {
           h8 hi, lo;
           weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
-          const h8 x0 = unpack8<TINY>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<TINY>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
-          weighted_sums<LOW, TINY>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
+          const h8 x0 = unpack8<TINYV>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<TINYV>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
+          weighted_sums<LOW, TINYV>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
           __builtin_amdgcn_sched_barrier(0);
         }
       if (AHEAD) w.load_values(next, lane);
       else w.load_keys(next, lane);
       __builtin_amdgcn_sched_barrier(0);
-      if (TINY) take_off<NB>(o, wsum);
+      if (TINYV) take_off<NB>(o, wsum);
       #pragma unroll
       for (int j = 0; j < 2 * NB; j++)
         #pragma unroll
