@@ -935,7 +935,8 @@ static void launch_attention_k(Kv4Attn a, const OUT &out, bool direct, hipStream
   const int units = many ? a.nrec : (int)((a.c.cap + CHUNK - 1) / CHUNK);
   const long y = (long)tiles * a.c.nkv * a.b.nseq, rounds = (units * y + 2047) / 2048;
   if (many) {
-    const int gx = (int)((units + rounds - 1) / rounds);
+    // (not units / rounds: the last part of a cache is seldom full)
+    const int gx = (int)std::min((long)units, std::max(1L, 2048 / y));
     hipLaunchKernelGGL((k_kv4_rows<NB, TYPE, true>), dim3((unsigned)deal_blocks((long)gx * a.c.nkv * a.b.nseq, (tiles + 3) / 4)), dim3(256), 0, st, a, tiles, gx);
   } else {
     const int gx = std::max((int)((units + 4 * rounds - 1) / (4 * rounds)), (a.spanmax + 3) / 4);
