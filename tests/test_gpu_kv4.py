@@ -239,6 +239,24 @@ def test_nan_and_large_scores(gpu):
     c.close()
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_queries_near_the_end_of_their_type(gpu, t):
+    """Scores of 1e37, within float32's range: the largest takes all of the weight (an output off by its own rounding, and by two
+    f16 parts of weights, one for bf16)."""
+    D = 64
+    c = cache(1, 1, D, 40)
+    k, v = rows(45, (1, 40, 1, D)), rows(46, (1, 40, 1, D))
+    c.append(k, v, ints(0))
+    q = rows(47, (1, 40, 1, D), t)
+    q *= 1e38 / float(q.abs().max())
+    got = f64(c.attend(q, ints(0)))[0, :, 0]
+    kk, vv = stored(f64(k))[0, :, 0], stored(f64(v))[0, :, 0]
+    for r in range(40):
+        want = vv[(kk[:r + 1] @ f64(q)[0, r, 0]).argmax()]
+        assert (np.abs(got[r] - want) <= (half_step(TYPES[t]) + (2.0 ** -11 if t == "bf16" else 2.0 ** -20)) * np.abs(want).max()).all()
+    c.close()
+
+
 @pytest.mark.parametrize("magnitude", [1e-6, 1e-3, 1.0, 2000.0])
 def test_values_of_every_magnitude(gpu, magnitude):
     """Values far below and above 1: weights are held in two f16 parts, which end at 2^-25 of a scale of 8."""

@@ -221,9 +221,9 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 // The eight codes of a word as f16 operands: pair r of (word >> 4 r).
 // TINY: as they lie, f16 denormals of code 2^-24, which the matrix cores take (16 cycles of a SIMD a word); the 2^24 and the
-// 8 to be taken off follow the sums. Sums of codes are larger than sums of codes less 8, and lose bits: 7e-6 of an output from f32
-// rows against 2e-7, and where 131000 values cancel to 1 in 360 of their size, 2e-4 of it, as much as an f16 output's own rounding.
-// So this is for the scores of 16-bit rows and the sums of bf16 ones.
+// 8 to be taken off follow the sums. Sums of denormals lose bits (of codes less 8 too: 5e-6 of an output from f32 rows against
+// 2e-7), to one side: where 131000 values cancel to 1 in 360 of their size, 2e-4 of it, as much as an f16 output's own rounding. So
+// this is for the scores of 16-bit rows and the sums of bf16 ones.
 // Else: less 8, under the exponent of 1024 and less 1032 (40 cycles a word).
 // The constants are in vector registers: a 32-bit operation takes 2 cycles of a SIMD from two waves' vector operands and 4 with a
 // scalar one, and and-or takes a single scalar one.
@@ -367,7 +367,8 @@ __device__ __forceinline__ void set_queries(Queries<NB, TINY> &q, const float (&
     sum = TINY ? sum4(sum) * (-8.0f / TINY_ONE) : 0.0f;
     q.z[b] = f4{sum, sum, sum, sum};
   }
-  q.c = fmaxf((float)ldexp((double)scale * 1.4426950408889634, TINY ? 24 - ex : -ex), 1.17549435e-38f);  // (not 0: it multiplies -inf)
+  // (neither 0 nor infinite: it multiplies infinities and zeros)
+  q.c = fminf(fmaxf((float)ldexp((double)scale * 1.4426950408889634, TINY ? 24 - ex : -ex), 1.17549435e-38f), 3.40282347e38f);
 }
 
 // A lane's share of a span (two records): code words and scales, loaded with every lane's 16-byte loads side by side.
