@@ -234,7 +234,7 @@ typedef struct {
 /* The tokens of a call: n_seq sequences of up to n_tok tokens each. Device arrays of n_seq int32: pos, the position of each
  * sequence's first token (its others follow); count, how many of its n_tok tokens there are (NULL: all; more than n_tok
  * counts as n_tok; rows behind a count are not read and outputs there are left as they were); slot, the cache slot of each
- * sequence (NULL: 0 .. n_seq - 1; not used by zl_rope_apply). */
+ * sequence (NULL: 0 .. n_seq - 1; not used by zl_rope_apply). At most 65535 sequences, 2^26 tokens and 2^26 query rows a call. */
 typedef struct {
   int n_seq, n_tok;
   const int32_t *pos, *count, *slot;
@@ -290,7 +290,7 @@ int zl_rope_apply(const zl_rope *r, const zl_batch *b, int type, int head_dim, c
  * NaN for an id outside the vocabulary), the entropy in nats, and the n_top (0 .. 64, at most the vocabulary) largest
  * logits' ids and log probabilities, largest first, the lowest id first among equals. Any output may be NULL. Logits of
  * -inf have probability 0. A row that holds NaN or +inf, or nothing above -inf, has NaN for every float output (top_ids:
- * NaN below all). work: zl_logprobs_work bytes. */
+ * NaN below all). work: zl_logprobs_work bytes. At most 2^24 - 1 rows a call. */
 int zl_logprobs(const void *logits, int type, int64_t ld, int rows, int vocab, const int32_t *tokens, int n_top, float *lp,
                 float *entropy, int32_t *top_ids, float *top_lp, void *work, int64_t work_bytes, void *stream);
 int zl_logprobs_work(int rows, int vocab, int n_top, int64_t *bytes);

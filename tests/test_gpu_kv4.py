@@ -403,6 +403,8 @@ def test_refusals(gpu):
             bad()
     for bad, msg in ((lambda: c.attend(q[:, :, :3], p), "3 query heads over 2 KV heads"),
                      (lambda: c.attend(q, p, scale=float("inf")), "finite"),
+                     (lambda: c.work_bytes(60000, 60000, 4), "query rows a call"),
+                     (lambda: c.append(k[:, :1].expand(2, 2 ** 26, 2, 64), k[:, :1].expand(2, 2 ** 26, 2, 64), p), "tokens a call"),
                      (lambda: c.append(k.repeat(2, 1, 1, 1), k.repeat(2, 1, 1, 1), ints(0, 0, 0, 0)), "4 sequences in a cache of 2 slots")):
         with pytest.raises(ZLError, match=msg):
             bad()

@@ -223,6 +223,8 @@ def test_refusals_of_models(gpu, tiny_files):
         Mdl.HipModel.load(tiny_files[0], kv="q8_0")
     with pytest.raises(ValueError, match="scaling must be"):
         Mdl.HipModel.load(tiny_files[0], rope=dict(scaling="ntk", factor=2.0))
+    with pytest.raises(ValueError, match="rope does not take base, n_rot"):
+        Mdl.HipModel.load(tiny_files[0], rope=dict(scaling="linear", factor=2.0, base=1e4, n_rot=64))
     with pytest.raises(ZLError, match="factor"):
         Mdl.HipModel.load(tiny_files[0], rope=dict(scaling="linear", factor=0.5))
     m = Mdl.HipModel.load(tiny_files[0], ctx=64, kv="q4_0")

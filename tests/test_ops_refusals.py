@@ -55,7 +55,7 @@ def test_null_arguments_and_bad_types():
         call("zl_logprobs", None, 8, 10, 0, 10, None, 0, None, None, None, None, None, 0, None)
 
 
-@pytest.mark.parametrize("args,msg", [((1, 10, 11), "n_top must be"), ((1, 100, 65), "n_top must be"), ((-1, 10, 1), "bad row count"),
+@pytest.mark.parametrize("args,msg", [((1, 10, 11), "n_top must be"), ((1, 100, 65), "n_top must be"), ((-1, 10, 1), "bad row count"), ((1 << 24, 10, 1), "bad row count"),
                                       ((1, 0, 0), "bad row count")])
 def test_logprobs_sizes(args, msg):
     with pytest.raises(ZLError, match=msg):

@@ -1,6 +1,7 @@
 // C entry points of the long-context operators: argument checks, handles, launches.
 #include <math.h>
 
+#include <algorithm>
 #include <memory>
 #include <vector>
 
@@ -40,12 +41,15 @@ static void need_type(const char *f, int type) {
   ZL_REQUIRE(value_bytes(type) > 0, ZL_ERR_UNSUPPORTED, std::string(f) + ": values must be F32, F16 or BF16 (got type " + std::to_string(type) + ")");
 }
 
+constexpr int64_t MOST_ROWS = 1 << 26;  // tokens or query rows of a call: grids of a few lanes for each stay within 2^32
+
 // The batch; heads and sequences are grid dimensions of at most 65535. Returns whether there is anything to do.
 static bool take_batch(const char *f, const zl_batch *b, OpBatch *o) {
   ZL_REQUIRE(b, ZL_ERR_ARG, std::string(f) + ": null argument");
   ZL_REQUIRE(b->n_seq >= 0 && b->n_tok >= 0, ZL_ERR_ARG, std::string(f) + ": negative batch size");
   ZL_REQUIRE(b->n_seq <= 65535, ZL_ERR_ARG, std::string(f) + ": at most 65535 sequences (got " + std::to_string(b->n_seq) + ")");
   if (b->n_seq == 0 || b->n_tok == 0) return false;
+  ZL_REQUIRE((int64_t)b->n_seq * b->n_tok <= MOST_ROWS, ZL_ERR_ARG, std::string(f) + ": at most " + std::to_string(MOST_ROWS) + " tokens a call");
   ZL_REQUIRE(b->pos, ZL_ERR_ARG, std::string(f) + ": positions missing");
   *o = OpBatch{b->n_seq, b->n_tok, b->pos, b->count, b->slot};
   return true;
@@ -57,7 +61,7 @@ static OpRows take_rows(const char *f, const zl_rows *r, int type) {
 }
 
 static void check_logprobs(int rows, int vocab, int n_top) {
-  ZL_REQUIRE(rows >= 0 && rows <= (1 << 30) && vocab >= 1 && vocab <= (1 << 30), ZL_ERR_ARG, "logprobs: bad row count or vocabulary");
+  ZL_REQUIRE(rows >= 0 && rows < (1 << 24) && vocab >= 1 && vocab <= (1 << 30), ZL_ERR_ARG, "logprobs: bad row count or vocabulary");
   ZL_REQUIRE(n_top >= 0 && n_top <= LOGPROB_MAX_TOP && n_top <= vocab, ZL_ERR_ARG,
              "logprobs: n_top must be 0 to " + std::to_string(LOGPROB_MAX_TOP) + " and at most the vocabulary (got " + std::to_string(n_top) + ")");
 }
@@ -130,16 +134,17 @@ int zl_kv4_read(const zl_kv4 *c, const zl_batch *b, int type, const zl_rows *k, 
   ZL_API_END
 }
 
-static void check_heads(const char *f, const zl_kv4 *c, int n_head) {
+static void check_heads(const char *f, const zl_kv4 *c, int n_seq, int n_tok, int n_head) {
   ZL_REQUIRE(n_head >= 1 && n_head % c->v.nkv == 0 && n_head <= 65535, ZL_ERR_ARG,
              std::string(f) + ": " + std::to_string(n_head) + " query heads over " + std::to_string(c->v.nkv) + " KV heads");
+  ZL_REQUIRE((int64_t)n_seq * n_tok <= MOST_ROWS / n_head, ZL_ERR_ARG, std::string(f) + ": at most " + std::to_string(MOST_ROWS) + " query rows a call");
 }
 
 int zl_kv4_attention_work(const zl_kv4 *c, int n_seq, int n_tok, int n_head, int64_t *bytes) {
   ZL_API_BEGIN
   ZL_REQUIRE(c && bytes, ZL_ERR_ARG, "null argument");
   ZL_REQUIRE(n_seq >= 0 && n_tok >= 0, ZL_ERR_ARG, "zl_kv4_attention_work: negative batch size");
-  check_heads("zl_kv4_attention_work", c, n_head);
+  check_heads("zl_kv4_attention_work", c, n_seq, n_tok, n_head);
   *bytes = kv4_attention_work(c->v, n_seq, n_tok, n_head);
   ZL_API_END
 }
@@ -150,7 +155,8 @@ int zl_kv4_attention(const zl_kv4 *c, const zl_batch *b, int type, const zl_rows
   const char *f = "zl_kv4_attention";
   ZL_REQUIRE(c, ZL_ERR_ARG, "null argument");
   need_type(f, type);
-  check_heads(f, c, n_head);
+  ZL_REQUIRE(b, ZL_ERR_ARG, std::string(f) + ": null argument");
+  check_heads(f, c, std::max(b->n_seq, 0), std::max(b->n_tok, 0), n_head);
   ZL_REQUIRE(scale >= 0.0f && scale < INFINITY, ZL_ERR_ARG, std::string(f) + ": the scale must be finite and not negative");
   Kv4Attn a{};
   if (take_batch(f, b, &a.b)) {
@@ -207,7 +213,7 @@ int zl_rope_apply(const zl_rope *r, const zl_batch *b, int type, int head_dim, c
   need_type(f, type);
   ZL_REQUIRE(head_dim >= r->n_rot && head_dim <= 65536, ZL_ERR_ARG, std::string(f) + ": head_dim " + std::to_string(head_dim) + " below the " + std::to_string(r->n_rot) + " rotated values, or above 65536");
   ZL_REQUIRE(!k == !k_out, ZL_ERR_ARG, std::string(f) + ": k and k_out come together");
-  ZL_REQUIRE(n_head >= 1 && n_head <= 65535 && (!k || (n_head_kv >= 1 && n_head_kv <= 65535)), ZL_ERR_ARG, std::string(f) + ": bad head count");
+  ZL_REQUIRE(n_head >= 1 && n_head <= 65535 && (!k || (n_head_kv >= 1 && n_head_kv <= 65535 - n_head)), ZL_ERR_ARG, std::string(f) + ": bad head count");
   RopeArgs a{};
   if (take_batch(f, b, &a.b)) {
     a.turns = r->turns; a.gain = (float)r->gain; a.half = r->n_rot / 2; a.neox = r->neox; a.hd = head_dim;

@@ -40,6 +40,8 @@ def _ext(kv, rope):
         return None
     e = _lib.zl_model_ext(kv_q4=1 if kv == "q4_0" else 0)
     if rope is not None:
+        if unknown := set(rope) - {"scaling", "factor", "orig_ctx", "beta_fast", "beta_slow", "attn_factor"}:
+            raise ValueError(f"rope does not take {', '.join(sorted(unknown))}: a model has its own")
         e._rope = rope_opts(**rope)
         e.rope = C.pointer(e._rope)
     return e
