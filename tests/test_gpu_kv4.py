@@ -150,7 +150,7 @@ def check(c, q, pos, count=None, slot=None, k=None, v=None, scale=None, t="f32",
     return got, worst
 
 
-LENGTHS = [1, 2, 31, 32, 33, 63, 64, 65, 511, 512, 513, 2047, 2048, 2049, 4100]
+LENGTHS = [1, 2, 31, 32, 33, 63, 64, 65, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049, 4100]
 
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
@@ -293,6 +293,48 @@ def test_a_row_has_the_same_bits_in_every_batch(gpu, dim, kv, group):
                 assert (got == want[:, j:j + m]).all(), (m, j)
     c.close()
     big.close()
+
+
+@pytest.mark.parametrize("kv,group,tokens,n", [(8, 4, 16, 40000), (8, 4, 256, 9000), (1, 8, 64, 140000)])
+def test_long_calls_have_the_bits_of_single_tokens(gpu, kv, group, tokens, n):
+    """Calls that take a record per part of 1024 (several parts a wave, more than 128 of them) against single tokens and float64; the
+    cache behind the tokens holds NaN."""
+    c = cache(1, kv, 64, n + 1000)
+    nan = torch.full((1, 1000, kv, 64), float("nan"), device="cuda")
+    c.append(nan, nan, ints(n))
+    k, v = rows(63, (1, n, kv, 64)), rows(64, (1, n, kv, 64))
+    c.append(k, v, ints(0))
+    q = rows(65, (1, tokens, kv * group, 64))
+    for first in (n - tokens, n // 2, 3):
+        print(f"case long {tokens} tokens at {first}", flush=True)
+        got = c.attend(q, ints(first))
+        assert torch.isfinite(got).all()
+        for j in (0, tokens // 2, tokens - 1):
+            assert (c.attend(q[:, j:j + 1], ints(first + j)) == got[:, j:j + 1]).all(), j
+    j, h = tokens - 1, kv * group - 1
+    p = n - tokens + j
+    got = f64(c.attend(q, ints(n - tokens)))[0, j, h]
+    kk, vv = stored(f64(k[0, :p + 1, -1])), stored(f64(v[0, :p + 1, -1]))
+    want, size = attention(f64(q)[0, j, h][None], kk, vv, [p], 64 ** -0.5)
+    assert (np.abs(got - want[0]) <= attention_bound(size, 64, np.abs(vv).max(), want, torch.float32)[0]).all()
+    c.close()
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """The last slot, head and positions of a cache of 6 GB."""
+    c = cache(20, 8, 256, 131072)
+    assert c.nbytes > 2 ** 32
+    k, v, q = rows(66, (1, 72, 8, 256)), rows(67, (1, 72, 8, 256)), rows(68, (1, 2, 8, 256))
+    c.append(k, v, ints(131000), slot=ints(19))
+    rk, rv = read(c, [131000], 72, slot=[19])
+    assert (rk == stored(f64(k))).all() and (rv == stored(f64(v))).all()
+    got = f64(c.attend(q, ints(131070), slot=ints(19)))[0]
+    for h in (0, 7):  # the positions before hold zeros
+        kk, vv = (np.concatenate([np.zeros((131000, 256)), x[0, :, h]]) for x in (rk, rv))
+        want, size = attention(f64(q)[0, :, h], kk, vv, [131070, 131071], 1 / 16)
+        assert (np.abs(got[:, h] - want) <= attention_bound(size, 256, np.abs(vv).max(), want, torch.float32)).all()
+    assert (read(c, [131000], 72, slot=[18])[0] == 0).all()
+    c.close()
 
 
 def test_unaligned_rows_scales_and_output_in_place(gpu):

@@ -23,19 +23,26 @@ _TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
 _type_of = {}  # by torch's type objects, filled as they come: a call on few rows is as long as its checks
 
 
+def _elsewhere(x, name):
+    return ValueError(f"{name} must be a tensor on GPU {_lib.DEVICE} (got {getattr(x, 'device', None)})")
+
+
 def _place(x, name):
-    if not getattr(x, "is_cuda", False) or x.get_device() != _lib.DEVICE:
-        raise ValueError(f"{name} must be a tensor on GPU {_lib.DEVICE} (got {getattr(x, 'device', None)})")
+    if not hasattr(x, "get_device") or x.get_device() != _lib.DEVICE:  # (-1 for a tensor in host memory)
+        raise _elsewhere(x, name)
 
 
 def _type(x, name):
+    try:
+        if x.get_device() == _lib.DEVICE:
+            return _type_of[x.dtype]
+    except (AttributeError, KeyError):
+        pass
     _place(x, name)
-    t = _type_of.get(x.dtype)
+    t = _TYPES.get(str(x.dtype))
     if t is None:
-        t = _TYPES.get(str(x.dtype))
-        if t is None:
-            raise ValueError(f"{name} must be float32, float16 or bfloat16 (got {x.dtype})")
-        _type_of[x.dtype] = t
+        raise ValueError(f"{name} must be float32, float16 or bfloat16 (got {x.dtype})")
+    _type_of[x.dtype] = t
     return t
 
 
@@ -49,28 +56,32 @@ def _ints(x, n, name):
 
 
 def _rows(x, name, shape=None, type_=None, written=False):
-    """(zl_rows, type, shape as [sequence, token, head, dim]) of a tensor."""
+    """(zl_rows, type, shape as (sequence, token, head, dim)) of a tensor."""
     t = _type(x, name)
-    s, st = tuple(x.shape), x.stride()
-    if len(s) == 3:
-        s, st = (s[0], 1, *s[1:]), (st[0], 0, *st[1:])
-    if len(s) != 4:
-        raise ValueError(f"{name} must be [sequence, token, head, dim] or [sequence, head, dim] (got {tuple(x.shape)})")
-    if st[3] != 1 and s[3] > 1:
-        raise ValueError(f"the values of a head of {name} must be contiguous (stride {st[3]})")
+    s = tuple(x.shape)
+    if len(s) == 4:
+        a, b, c, d = x.stride()
+    elif len(s) == 3:
+        a, c, d = x.stride()
+        b, s = 0, (s[0], 1, s[1], s[2])
+    else:
+        raise ValueError(f"{name} must be [sequence, token, head, dim] or [sequence, head, dim] (got {s})")
+    if d != 1 and s[3] > 1:
+        raise ValueError(f"the values of a head of {name} must be contiguous (stride {d})")
     if shape is not None and s != shape:
         raise ValueError(f"{name} must be {shape} (got {s})")
     if type_ is not None and t != type_:
         raise ValueError(f"{name} must have the type of the other rows (got {x.dtype})")
-    if written and 0 in st and any(n > 1 and d == 0 for n, d in zip(s, st)):
+    if written and ((a == 0 and s[0] > 1) or (b == 0 and s[1] > 1) or (c == 0 and s[2] > 1)):
         raise ValueError(f"{name} is written, so its rows must not share memory")
-    return _lib.zl_rows(x.data_ptr(), st[0], st[1], st[2]), t, s
+    return _lib.zl_rows(x.data_ptr(), a, b, c), t, s
 
 
 def _batch(n_seq, n_tok, pos, count, slot=None):
     if pos is None:
         raise ValueError("positions missing")
-    return _lib.zl_batch(n_seq, n_tok, _ints(pos, n_seq, "pos"), _ints(count, n_seq, "count"), _ints(slot, n_seq, "slot"))
+    return _lib.zl_batch(n_seq, n_tok, _ints(pos, n_seq, "pos"), count if count is None else _ints(count, n_seq, "count"),
+                         slot if slot is None else _ints(slot, n_seq, "slot"))
 
 
 def _torch():
