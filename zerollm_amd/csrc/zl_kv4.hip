@@ -224,29 +224,28 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 // 8 to be taken off follow the sums. Sums of denormals lose bits (of codes less 8 too: 5e-6 of an output from f32 rows against
 // 2e-7), to one side: where 131000 values cancel to 1 in 360 of their size, 2e-4 of it, as much as an f16 output's own rounding. So
 // this is for the scores of 16-bit rows and the sums of bf16 ones.
-// Else: less 8, under the exponent of 1024 and less 1032 (40 cycles a word).
+// Else: less 8, under an exponent and less the sum of both: 1024 where the code is in the lowest bits, 64 where it is four higher
+// (no shift; 36 cycles a word).
 // The constants are in vector registers: a 32-bit operation takes 2 cycles of a SIMD from two waves' vector operands and 4 with a
 // scalar one, and and-or takes a single scalar one.
 struct Unpack {
-  uint32_t mask = 0x000f000fu, k1024 = 0x64006400u;
-  __device__ __forceinline__ Unpack() { __asm__("" : "+v"(mask), "+v"(k1024)); }
+  uint32_t mask = 0x000f000fu, k1024 = 0x64006400u, mask4 = 0x00f000f0u, k64 = 0x54005400u;
+  __device__ __forceinline__ Unpack() { __asm__("" : "+v"(mask), "+v"(k1024), "+v"(mask4), "+v"(k64)); }
 };
 template <bool TINY>
 __device__ __forceinline__ h8 unpack8(uint32_t w, const Unpack &k) {
-  if constexpr (TINY) {
-    u4 x;
-    #pragma unroll
-    for (int r = 0; r < 4; r++) x[r] = (w >> (4 * r)) & k.mask;
-    return __builtin_bit_cast(h8, x);
-  }
-  h8 x;
+  u4 x;
   #pragma unroll
   for (int r = 0; r < 4; r++) {
-    const h2 p = __builtin_bit_cast(h2, ((w >> (4 * r)) & k.mask) | k.k1024) - (h2){1032, 1032};
-    x[2 * r] = p[0];
-    x[2 * r + 1] = p[1];
+    if constexpr (TINY) {
+      x[r] = (w >> (4 * r)) & k.mask;
+    } else {
+      const uint32_t v = r < 2 ? w : w >> 8;
+      const h2 p = r & 1 ? __builtin_bit_cast(h2, (v & k.mask4) | k.k64) - (h2){72, 72} : __builtin_bit_cast(h2, (v & k.mask) | k.k1024) - (h2){1032, 1032};
+      x[r] = __builtin_bit_cast(uint32_t, p);
+    }
   }
-  return x;
+  return __builtin_bit_cast(h8, x);
 }
 constexpr float TINY_ONE = 16777216.0f;  // 2^24: a code's unit
 constexpr h8 ONES = {1, 1, 1, 1, 1, 1, 1, 1};
