@@ -285,9 +285,9 @@ struct Sum {
   __device__ __forceinline__ void fold(const Sum &p) {
     const float M = fmaxf(m, p.m), r = M == -INFINITY ? 0.0f : M, a = exp2_(m - r), b = exp2_(p.m - r);
     m = M;
-    l = fmaf(l, a, p.l * b);
+    l = fmaf(p.l, b, l * a);
     #pragma unroll
-    for (int i = 0; i < N; i++) o[i] = fmaf(o[i], a, p.o[i] * b);
+    for (int i = 0; i < N; i++) o[i] = fmaf(p.o[i], b, o[i] * a);
   }
 };
 
@@ -306,9 +306,9 @@ __device__ __forceinline__ void fold_all(Sum<N> &f, const float2 (&ml)[K], const
   #pragma unroll
   for (int k = 0; k < K; k++) {
     if (k >= n) break;
-    f.l = fmaf(f.l, a[k], ml[k].y * b[k]);
+    f.l = fmaf(ml[k].y, b[k], f.l * a[k]);
     #pragma unroll
-    for (int i = 0; i < N; i++) f.o[i] = fmaf(f.o[i], a[k], o[k][i] * b[k]);
+    for (int i = 0; i < N; i++) f.o[i] = fmaf(o[k][i], b[k], f.o[i] * a[k]);
   }
 }
 
@@ -644,72 +644,73 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
   }
   for (int c = c0; (long)c * unit <= most; c += step) {
     const int ns = min(unit / SPAN, (most - c * unit) / SPAN + 1);
-    u.clear();
     float pm = -INFINITY, pl = 0.0f;
     if (MANY) {
       #pragma unroll
       for (int j = 0; j < 2 * NB; j++) part[wave][j][lane] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    for (int sp = 0; sp < ns; sp++) {
-      const int p0 = c * unit + sp * SPAN, lim = last - p0;
-      const int pn = sp + 1 < ns ? p0 + SPAN : (long)(c + step) * unit <= most ? (c + step) * unit : p0;  // (the last one is read again, for nothing)
-      const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, p0 / KV4_GROUP), *next = record_of(a.c, tl.slot, tl.kvh, pn / KV4_GROUP);
-      const bool masked = __ballot(lim < SPAN - 1) != 0;
-      f4 s[2][2];
-      #pragma unroll
-      for (int i = 0; i < 2; i++)
+    for (int sp = 0; sp < ns;) {
+      u.clear();
+      for (const int end = min(sp + CHUNK / SPAN, ns); sp < end; sp++) {
+        const int p0 = c * unit + sp * SPAN, lim = last - p0;
+        const int pn = sp + 1 < ns ? p0 + SPAN : (long)(c + step) * unit <= most ? (c + step) * unit : p0;  // (the last one is read again, for nothing)
+        const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, p0 / KV4_GROUP), *next = record_of(a.c, tl.slot, tl.kvh, pn / KV4_GROUP);
+        const bool masked = __ballot(lim < SPAN - 1) != 0;
+        f4 s[2][2];
         #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], uk); }, w.ks[i], t, q);
-          __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < 2; i++)
+          #pragma unroll
+          for (int t = 0; t < 2; t++) {
+            s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], uk); }, w.ks[i], t, q);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        if (AHEAD) w.load_keys(next, lane);
+        else w.load_values(rec, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        if (masked) {
+          mask_scores(s, lim, g);
+          mask_scales<NB>(w.vs[0], 0, lim, g);
+          mask_scales<NB>(w.vs[1], 1, lim, g);
         }
-      if (AHEAD) w.load_keys(next, lane);
-      else w.load_values(rec, lane);
-      __builtin_amdgcn_sched_barrier(0);
-      if (masked) {
-        mask_scores(s, lim, g);
-        mask_scales<NB>(w.vs[0], 0, lim, g);
-        mask_scales<NB>(w.vs[1], 1, lim, g);
+        Sum<8 * NB> r;
+        Weights<LOW> pw;
+        span_softmax<LOW>(s, q.c, pw, r.m, r.l);
+        f4 o[2 * NB], wsum[NB];
+        #pragma unroll
+        for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        #pragma unroll
+        for (int b = 0; b < NB; b++) wsum[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        #pragma unroll
+        for (int i = 0; i < 2; i++)
+          #pragma unroll
+          for (int b = 0; b < NB; b++) {
+            h8 hi, lo;
+            weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
+            const h8 x0 = unpack8<TINYV>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<TINYV>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
+            weighted_sums<LOW, TINYV>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        if (AHEAD) w.load_values(next, lane);
+        else w.load_keys(next, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        if (TINYV) take_off<NB>(o, wsum);
+        #pragma unroll
+        for (int j = 0; j < 2 * NB; j++)
+          #pragma unroll
+          for (int v = 0; v < 4; v++) r.o[4 * j + v] = o[j][v];
+        u.fold(r);
       }
-      Sum<8 * NB> r;
-      Weights<LOW> pw;
-      span_softmax<LOW>(s, q.c, pw, r.m, r.l);
-      f4 o[2 * NB], wsum[NB];
-      #pragma unroll
-      for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-      #pragma unroll
-      for (int b = 0; b < NB; b++) wsum[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-      #pragma unroll
-      for (int i = 0; i < 2; i++)
-        #pragma unroll
-        for (int b = 0; b < NB; b++) {
-          h8 hi, lo;
-          weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
-          const h8 x0 = unpack8<TINYV>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<TINYV>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
-          weighted_sums<LOW, TINYV>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      if (AHEAD) w.load_values(next, lane);
-      else w.load_keys(next, lane);
-      __builtin_amdgcn_sched_barrier(0);
-      if (TINYV) take_off<NB>(o, wsum);
-      #pragma unroll
-      for (int j = 0; j < 2 * NB; j++)
-        #pragma unroll
-        for (int v = 0; v < 4; v++) r.o[4 * j + v] = o[j][v];
-      u.fold(r);
-      if (MANY && ((sp & (CHUNK / SPAN - 1)) == CHUNK / SPAN - 1 || sp == ns - 1)) {
+      if (MANY) {
         const float M = fmaxf(pm, u.m), ref = M == -INFINITY ? 0.0f : M, x = exp2_(pm - ref), y = exp2_(u.m - ref);
         pm = M;
-        pl = fmaf(pl, x, u.l * y);
+        pl = fmaf(u.l, y, pl * x);
         #pragma unroll
         for (int j = 0; j < 2 * NB; j++) {
           f4 o = part[wave][j][lane];
           #pragma unroll
-          for (int v = 0; v < 4; v++) o[v] = fmaf(o[v], x, u.o[4 * j + v] * y);
+          for (int v = 0; v < 4; v++) o[v] = fmaf(u.o[4 * j + v], y, o[v] * x);
           part[wave][j][lane] = o;
         }
-        u.clear();
       }
     }
     if (MANY) {
