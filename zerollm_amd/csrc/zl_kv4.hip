@@ -597,14 +597,14 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 // waits for another. The next span's keys are requested when the scores are done with this one's, its values after the weighted
 // sums, so that the loads run under the rest. (A chunk of 512 per block, one span per wave, folded in LDS behind a barrier: 9 tokens
 // of 32 heads after 16384 positions 48 us against 41. Eight waves of a block sharing spans unpacked into LDS, one meeting a span:
-// 256 tokens after 12000 positions 240 us against 189.)
+// 256 tokens after 12000 positions 240 us against 189, as both were then.)
 // Few rows: sequences of so few spans that a wave for each does not overfill the GPU (a.spanmax, by the call's tiles) leave a record
-// per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 8.5). A token of 32 heads of
-// 128 over 8 KV heads after 131000 positions: 44 us, 151 MB at 3.4 TB/s, near a read's own rate (4.1). 9 tokens after 16384: 27 us,
+// per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 8). A token of 32 heads of
+// 128 over 8 KV heads after 131000 positions: 42 us, 151 MB at 3.6 TB/s, near a read's own rate (4.1). 9 tokens after 16384: 26 us,
 // bound by the vector units, 1.5 waves a SIMD, and by the waves' start and end.
 // MANY: the block's waves have neighbouring tiles of the same part, whose records they read at about the same time. 256 tokens of 32
-// heads over 8 after 12000 positions, f16: 189 us, bound by the vector units: 720 vector instructions and 63 matrix ones a span of a
-// tile, 4300 cycles where those alone are 3200, with two waves a SIMD to hide the matrix instructions' latency.
+// heads over 8 after 12000 positions, f16: 155 us in a stream of calls, bound by the vector units: some 650 vector instructions and 48
+// matrix ones a span of a tile, 3500 cycles of a SIMD, with two waves to hide the matrix instructions' latency.
 template <int NB, int TYPE, bool MANY>
 __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
@@ -898,13 +898,13 @@ __global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a, const O
 // Tiles of 16 rows times KV heads times sequences.
 static long tile_count(const Kv4View &c, int nseq, int ntok, int nhead) { return ((long)ntok * (nhead / c.nkv) + 15) / 16 * c.nkv * nseq; }
 // Whether a call takes a wave per (tile, part): where they fill the GPU's SIMDs, and there are enough rows that the records of chunks
-// would cost more than the longer runs. (Queries of 32 heads over 8, us, records of chunks : of parts, 16 tokens a call = 32 tiles:
-//   after    16 tokens  32        48        64        128
-//   1000     23 : 42    32 : 42   40 : 42   43 : 42   57 : 45
-//   4000     30 : 42    38 : 44   42 : 44   47 : 44   78 : 66
-//   16000    36 : 47    55 : 48   87 : 70   91 : 71   164 : 125
-//   60000    114 : 83   215 : 136 356 : 187 433 : 239 882 : 443.) The cache's capacity stands for the length, which the host does
-// not know; with fewer tiles a short sequence in a large cache would lose more than a long one gains.
+// would cost more than the longer runs. (f16 queries of 32 heads over 8, us, records of chunks : of parts, 16 tokens a call = 32 tiles:
+//   after    16 tokens  32        48        64        128       256
+//   1000     23 : 40    31 : 40   41 : 40   41 : 40   58 : 42   95 : 43
+//   4000     29 : 40    36 : 41   41 : 42   45 : 42   76 : 65   136 : 80
+//   16000    34 : 46    52 : 47   82 : 69   87 : 70   158 : 121 316 : 216
+//   60000    109 : 81   205 : 131 337 : 178 416 : 227 857 : 418 1693 : 778.) The cache's capacity stands for the length, which the
+// host does not know; with fewer tiles a short sequence in a large cache would lose more than a long one gains.
 static bool many_rows(const Kv4View &c, int nseq, int ntok, int nhead) {
   const long tiles = tile_count(c, nseq, ntok, nhead);
   return tiles >= 128 || (tiles >= 32 && tiles * ((c.cap + PART - 1) / PART) >= 1024);
