@@ -163,9 +163,10 @@ class KVCacheQ4:
         if out is None:
             out = _torch().empty(tuple(q.shape), dtype=q.dtype, device=q.device)
         o = _rows(out, "out", s, t, True)[0]
-        if s != self._sized[0]:
-            self._sized = s, self.work_bytes(s[0], s[1], s[2])
-        w = _work(work, self._sized[1], q)
+        sized = self._sized
+        if s != sized[0]:
+            sized = self._sized = s, self.work_bytes(s[0], s[1], s[2])
+        w = _work(work, sized[1], q)
         call("zl_kv4_attention", self._handle(), b, t, qr, s[2], scale or 0.0, o, w.data_ptr(), w.numel() * w.element_size(), _stream())
         return out
 
