@@ -220,10 +220,11 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 // The eight codes of a word as f16 operands: pair r of (word >> 4 r).
-// TINY: as they lie, f16 denormals of code 2^-24, which the matrix cores take (16 cycles of a SIMD a word); the 2^24 and the
-// 8 to be taken off follow the sums. Sums of denormals lose bits (of codes less 8 too: 5e-6 of an output from f32 rows against
-// 2e-7), to one side: where 131000 values cancel to 1 in 360 of their size, 2e-4 of it, as much as an f16 output's own rounding. So
-// this is for the scores of 16-bit rows and the sums of bf16 ones.
+// TINY: as they lie, f16 denormals of code 2^-24, which the matrix cores take; the 2^24 and the 8 to be taken off follow the
+// sums. Sums of denormals lose bits (of codes less 8 too: 5e-6 of an output from f32 rows against 2e-7), to one side: where 131000
+// values cancel to 1 in 360 of their size, 2e-4 of it, as much as an f16 output's own rounding. So this is for the scores of 16-bit
+// rows and the sums of bf16 ones. Scores take pairs 1 and 3 four bits higher (16 code 2^-24, and a sixteenth of their queries): a
+// shift a word (12 cycles of a SIMD) for three (16).
 // Else: less 8, under an exponent and less the sum of both: 1024 where the code is in the lowest bits, 64 where it is four higher
 // (no shift; 36 cycles a word).
 // The constants are in vector registers: a 32-bit operation takes 2 cycles of a SIMD from two waves' vector operands and 4 with a
@@ -232,15 +233,18 @@ struct Unpack {
   uint32_t mask = 0x000f000fu, k1024 = 0x64006400u, mask4 = 0x00f000f0u, k64 = 0x54005400u;
   __device__ __forceinline__ Unpack() { __asm__("" : "+v"(mask), "+v"(k1024), "+v"(mask4), "+v"(k64)); }
 };
-template <bool TINY>
+enum { SIGNED, CODES, CODES16 };  // codes less 8; codes; codes, those of odd pairs times 16
+template <int HOW>
 __device__ __forceinline__ h8 unpack8(uint32_t w, const Unpack &k) {
   u4 x;
   #pragma unroll
   for (int r = 0; r < 4; r++) {
-    if constexpr (TINY) {
+    const uint32_t v = r < 2 ? w : w >> 8;
+    if constexpr (HOW == CODES) {
       x[r] = (w >> (4 * r)) & k.mask;
+    } else if constexpr (HOW == CODES16) {
+      x[r] = v & (r & 1 ? k.mask4 : k.mask);
     } else {
-      const uint32_t v = r < 2 ? w : w >> 8;
       const h2 p = r & 1 ? __builtin_bit_cast(h2, (v & k.mask4) | k.k64) - (h2){72, 72} : __builtin_bit_cast(h2, (v & k.mask) | k.k1024) - (h2){1032, 1032};
       x[r] = __builtin_bit_cast(uint32_t, p);
     }
@@ -354,12 +358,13 @@ __device__ __forceinline__ void set_queries(Queries<NB, TINY> &q, const float (&
     u4 hi, lo;
     #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float x0 = v[b][2 * e] * up, x1 = v[b][2 * e + 1] * up;
+      const float pair = TINY && (e & 1) ? up * 0.0625f : up;
+      const float x0 = v[b][2 * e] * pair, x1 = v[b][2 * e + 1] * pair;
       const h2 h = {(_Float16)x0, (_Float16)x1};
       const h2 r = {(_Float16)fmaf(-1.0f, (float)h[0], x0), (_Float16)fmaf(-1.0f, (float)h[1], x1)};
       hi[e] = __builtin_bit_cast(uint32_t, h);
       lo[e] = __builtin_bit_cast(uint32_t, r);
-      if (TINY) sum += (float)h[0] + (float)h[1];
+      if (TINY) sum = fmaf((float)h[0] + (float)h[1], e & 1 ? 16.0f : 1.0f, sum);
     }
     q.hi[b] = __builtin_bit_cast(h8, hi);
     q.lo[b] = __builtin_bit_cast(h8, lo);
@@ -661,7 +666,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
         for (int i = 0; i < 2; i++)
           #pragma unroll
           for (int t = 0; t < 2; t++) {
-            s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], uk); }, w.ks[i], t, q);
+            s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY ? CODES16 : SIGNED>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], uk); }, w.ks[i], t, q);
             __builtin_amdgcn_sched_barrier(0);
           }
         if (AHEAD) w.load_keys(next, lane);
@@ -686,7 +691,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
           for (int b = 0; b < NB; b++) {
             h8 hi, lo;
             weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
-            const h8 x0 = unpack8<TINYV>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<TINYV>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
+            const h8 x0 = unpack8<TINYV ? CODES : SIGNED>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<TINYV ? CODES : SIGNED>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
             weighted_sums<LOW, TINYV>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
             __builtin_amdgcn_sched_barrier(0);
           }
