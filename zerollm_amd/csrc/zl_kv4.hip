@@ -605,11 +605,11 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 // 256 tokens after 12000 positions 240 us against 189, as both were then.)
 // Few rows: sequences of so few spans that a wave for each does not overfill the GPU (a.spanmax, by the call's tiles) leave a record
 // per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 8). A token of 32 heads of
-// 128 over 8 KV heads after 131000 positions: 42 us, 151 MB at 3.6 TB/s, near a read's own rate (4.1). 9 tokens after 16384: 26 us,
+// 128 over 8 KV heads after 131000 positions: 41 us, 151 MB at 3.7 TB/s, near a read's own rate (4.1). 9 tokens after 16384: 26 us,
 // bound by the vector units, 1.5 waves a SIMD, and by the waves' start and end.
 // MANY: the block's waves have neighbouring tiles of the same part, whose records they read at about the same time. 256 tokens of 32
-// heads over 8 after 12000 positions, f16: 155 us in a stream of calls, bound by the vector units: some 650 vector instructions and 48
-// matrix ones a span of a tile, 3500 cycles of a SIMD, with two waves to hide the matrix instructions' latency.
+// heads over 8 after 12000 positions, f16: 150 us in a stream of calls, bound by the vector units: some 620 vector instructions and 48
+// matrix ones a span of a tile, 3400 cycles of a SIMD, with two waves to hide the matrix instructions' latency.
 template <int NB, int TYPE, bool MANY>
 __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
