@@ -295,28 +295,31 @@ def test_a_row_has_the_same_bits_in_every_batch(gpu, dim, kv, group):
     big.close()
 
 
-@pytest.mark.parametrize("kv,group,tokens,n", [(8, 4, 16, 40000), (8, 4, 256, 9000), (1, 8, 64, 140000)])
-def test_long_calls_have_the_bits_of_single_tokens(gpu, kv, group, tokens, n):
-    """Calls that take a record per part of 1024 (several parts a wave, more than 128 of them) against single tokens and float64; the
-    cache behind the tokens holds NaN."""
-    c = cache(1, kv, 64, n + 1000)
-    nan = torch.full((1, 1000, kv, 64), float("nan"), device="cuda")
+@pytest.mark.parametrize("kv,group,tokens,n,dim,t", [(8, 4, 16, 40000, 64, "f32"), (8, 4, 256, 9000, 64, "f32"), (1, 8, 64, 140000, 64, "f32"),
+                                                     (8, 4, 256, 5000, 128, "f16"), (4, 2, 300, 3000, 256, "bf16"), (4, 2, 300, 2100, 256, "f32"),
+                                                     (4, 2, 260, 700, 256, "f16"), (2, 7, 300, 1500, 128, "bf16")])
+def test_long_calls_have_the_bits_of_single_tokens(gpu, kv, group, tokens, n, dim, t):
+    """Calls that take a record per part of 1024 (several parts a wave, more than 128 of them, a single one) against single tokens and
+    float64; the cache behind the tokens holds NaN."""
+    c = cache(1, kv, dim, n + 324)
+    nan = torch.full((1, 324, kv, dim), float("nan"), device="cuda")
     c.append(nan, nan, ints(n))
-    k, v = rows(63, (1, n, kv, 64)), rows(64, (1, n, kv, 64))
+    k, v = rows(63, (1, n, kv, dim), t), rows(64, (1, n, kv, dim), t)
     c.append(k, v, ints(0))
-    q = rows(65, (1, tokens, kv * group, 64))
-    for first in (n - tokens, n // 2, 3):
+    q = rows(65, (1, tokens, kv * group, dim), t)
+    for first in (n - tokens, n // 2 - 100, 3):
         print(f"case long {tokens} tokens at {first}", flush=True)
         got = c.attend(q, ints(first))
         assert torch.isfinite(got).all()
         for j in (0, tokens // 2, tokens - 1):
             assert (c.attend(q[:, j:j + 1], ints(first + j)) == got[:, j:j + 1]).all(), j
-    j, h = tokens - 1, kv * group - 1
-    p = n - tokens + j
-    got = f64(c.attend(q, ints(n - tokens)))[0, j, h]
-    kk, vv = stored(f64(k[0, :p + 1, -1])), stored(f64(v[0, :p + 1, -1]))
-    want, size = attention(f64(q)[0, j, h][None], kk, vv, [p], 64 ** -0.5)
-    assert (np.abs(got - want[0]) <= attention_bound(size, 64, np.abs(vv).max(), want, torch.float32)[0]).all()
+    got = f64(c.attend(q, ints(n - tokens)))[0]
+    h = kv * group - 1
+    kk, vv = stored(f64(k[0, :, -1])), stored(f64(v[0, :, -1]))
+    for j in (0, tokens // 3, tokens - 1):
+        p = n - tokens + j
+        want, size = attention(f64(q)[0, j, h][None], kk[:p + 1], vv[:p + 1], [p], dim ** -0.5)
+        assert (np.abs(got[j, h] - want[0]) <= attention_bound(size, dim, np.abs(vv).max(), want, TYPES[t])[0]).all()
     c.close()
 
 
