@@ -97,6 +97,27 @@ def test_masked_infinite_and_nan_logits(gpu):
     assert np.isnan(check(x[6:], [-1, 3000], 3).logprobs.cpu().numpy()).all()
 
 
+def test_many_rows_of_ties_and_masks(gpu):
+    """Rows that one block takes whole, tile by tile, against the same rows a few at a time (twice the bound of one)."""
+    from zerollm_amd.ops import logprobs as own
+    inf, vocab = float("inf"), 40000
+    x = torch.randn((8, vocab), generator=torch.Generator().manual_seed(4)).cuda()
+    x[0] = 0.0
+    x[1, 3:] = -inf
+    x[2, :-2] = -inf
+    x[3] = x[3].round()
+    x[4, 30000:] = x[4, 0]
+    x[5] = -inf
+    x[6] = torch.where(torch.arange(vocab) % 3 == 0, 0.0, -0.0).cuda()
+    few = check(x, list(range(8)), 20)
+    print("case many rows", flush=True)
+    many = own(x.repeat(1300, 1), ints(list(range(8)) * 1300), top=20)
+    assert (many.top_ids.view(1300, 8, 20) == few.top_ids).all()
+    for a, b in ((many.logprobs.view(1300, 8), few.logprobs), (many.entropy.view(1300, 8), few.entropy), (many.top_logprobs.view(1300, 8, 20), few.top_logprobs)):
+        same = (a == b) | (a.isnan() & b.isnan())
+        assert (same | ((a - b).abs() <= 2 * (2.0 ** -19 + 2.0 ** -22 * 5 * 16))).all()
+
+
 def test_row_strides_outputs_and_work_of_the_caller(gpu):
     from zerollm_amd.ops import LogProbs, logprobs as own, logprobs_work_bytes
     w = torch.full((40, 1001), 1e30, device="cuda")
