@@ -17,16 +17,21 @@ __device__ __forceinline__ void turn_sincos(double t, float *c, float *s) {
   *s = k >= 2 ? -b : b;
 }
 
+template <int TYPE> constexpr int value_size() { return sizeof(typename ValueOf<TYPE>::t); }
 template <class T, int W> struct Piece { typedef T t __attribute__((ext_vector_type(W))); };
 
 // A block takes `tb` tokens of a sequence and a share of their heads (blockIdx.z): the tokens' cos and sin go to LDS once, then
-// every lane takes pieces of W values: W pairs' firsts and seconds from the two halves, W / 2 neighbouring pairs, or W values
-// that pass through. W > 1 (16 bytes) where every row starts on a 16-byte boundary and the parts of a head do. Bound by HBM: each
-// value is read and written once.
-template <int TYPE, int W, bool HALF>
+// every lane takes pieces of the rows. WHOLE: every row is whole 16-byte pieces of V values. Neighbouring pairs: a piece's pairs
+// are rotated or pass through one by one. Halves: W pairs' firsts and seconds, W the largest that divides the half, then the pieces
+// behind the rotated values, of which the first may start among them. Bound by HBM: each value is read and written once (16384
+// tokens of 40 heads of 128, 64 rotated, bf16: 84 us, 4.0 TB/s; with whole pieces only where the parts of the head were some too,
+// 2 of 64 values rotated took 59 us a call of 11269 tokens of 24 heads, and take 21).
+template <int TYPE, int W, bool HALF, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) {
   typedef typename ValueOf<TYPE>::t T;
+  constexpr int V = WHOLE ? 16 / sizeof(T) : 1;
   typedef typename Piece<T, W>::t vec;
+  typedef typename Piece<T, V>::t whole;
   extern __shared__ float2 cs[];  // [tokens][half]
   const int s = blockIdx.y, tid = threadIdx.x, t0 = blockIdx.x * tb, half = a.half, nrot = 2 * half;
   const int nt = min(tb, (a.b.count ? max(0, min(a.b.count[s], a.b.ntok)) : a.b.ntok) - t0);
@@ -39,8 +44,8 @@ __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) 
     cs[i] = make_float2(c * a.gain, n * a.gain);
   }
   __syncthreads();
-  constexpr int PW = HALF || W > 1 ? W : 2;  // values of a neighbouring-pairs piece
-  const int rp = HALF ? half / W : nrot / PW, items = rp + (a.hd - nrot) / W;  // pieces of a head: rotated, then passed through
+  // pieces of a head: rotated ones, then those behind
+  const int rp = HALF ? half / W : WHOLE ? a.hd / V : half, items = rp + (HALF || !WHOLE ? a.hd / V - nrot / V : 0);
   const int h0 = blockIdx.z * hb, nh = min(hb, a.nq + a.nk - h0), total = nt * nh * items;
   for (int i = tid; i < total; i += 256) {
     const int row = i / items, r = i - row * items, t = row / nh, h = h0 + row - t * nh;
@@ -50,8 +55,15 @@ __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) 
     const T *xp = (const T *)x.p + s * x.seq + (t0 + t) * x.tok + hh * x.head;
     T *yp = (T *)y.p + s * y.seq + (t0 + t) * y.tok + hh * y.head;
     if (r >= rp) {
-      const int d = nrot + (r - rp) * W;
-      *(vec *)(yp + d) = *(const vec *)(xp + d);
+      const int d = (nrot / V + r - rp) * V;
+      const whole u = *(const whole *)(xp + d);
+      if (d >= nrot) {
+        *(whole *)(yp + d) = u;
+      } else {
+        #pragma unroll
+        for (int e = 0; e < V; e++)
+          if (d + e >= nrot) yp[d + e] = u[e];
+      }
       continue;
     }
     const float2 *f = cs + t * half;
@@ -68,18 +80,18 @@ __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) 
       }
       *(vec *)(yp + d) = w;
       *(vec *)(yp + d + half) = z;
-    } else if constexpr (W > 1) {
-      const int d = r * W;
-      const vec u = *(const vec *)(xp + d);
-      vec w;
+    } else if constexpr (WHOLE) {
+      const int d = r * V;
+      whole u = *(const whole *)(xp + d);
       #pragma unroll
-      for (int e = 0; e < W; e += 2) {
+      for (int e = 0; e < V; e += 2) {
+        if (d + e >= nrot) break;
         const float x0 = load_value<TYPE>(u[e]), x1 = load_value<TYPE>(u[e + 1]);
         const float2 g = f[(d + e) >> 1];
-        w[e] = store_value<TYPE>(fmaf(x0, g.x, -(x1 * g.y)));
-        w[e + 1] = store_value<TYPE>(fmaf(x0, g.y, x1 * g.x));
+        u[e] = store_value<TYPE>(fmaf(x0, g.x, -(x1 * g.y)));
+        u[e + 1] = store_value<TYPE>(fmaf(x0, g.y, x1 * g.x));
       }
-      *(vec *)(yp + d) = w;
+      *(whole *)(yp + d) = u;
     } else {
       const float x0 = load_value<TYPE>(xp[2 * r]), x1 = load_value<TYPE>(xp[2 * r + 1]);
       const float2 g = f[r];
@@ -89,36 +101,41 @@ __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) 
   }
 }
 
-// Rows of 16-byte pieces: every start and stride, and the head's parts.
+// Rows of 16-byte pieces: every start and stride, and the head.
 static bool whole_pieces(const RopeArgs &a, int vb) {
   const int w = 16 / vb;
   auto ok = [&](const OpRows &r) {
     return (uintptr_t)r.p % 16 == 0 && r.seq % w == 0 && r.tok % w == 0 && r.head % w == 0;
   };
-  return ok(a.q) && ok(a.qo) && (!a.nk || (ok(a.k) && ok(a.ko))) && (a.neox ? a.half : 2 * a.half) % w == 0 && (a.hd - 2 * a.half) % w == 0;
+  return ok(a.q) && ok(a.qo) && (!a.nk || (ok(a.k) && ok(a.ko))) && a.hd % w == 0;
 }
 
-template <int TYPE, int W>
+template <int TYPE, int W, bool HALF, bool WHOLE>
 static void launch_rope_k(const RopeArgs &a, hipStream_t st) {
   // Tokens and heads per block: pieces for every lane a few times over where there are many tokens, as many blocks as CUs
   // where there are few (each of which forms its tokens' cos and sin itself: 2 half values a block).
-  const int heads = a.nq + a.nk, pieces = std::max(1, a.hd / W);
+  constexpr int V = WHOLE ? 16 / value_size<TYPE>() : 1;
+  const int heads = a.nq + a.nk, nrot = 2 * a.half;
+  const int pieces = HALF ? a.half / W + a.hd / V - nrot / V : WHOLE ? a.hd / V : a.half + a.hd - nrot;
   const long all = (long)a.b.ntok * a.b.nseq * heads * pieces;
   const long per = std::max(256L, std::min(4096L, all / 512));  // pieces per block
   const int hb = (int)std::max(1L, std::min((long)heads, per / pieces));
   const int tb = (int)std::max(1L, std::min({(long)a.b.ntok, per / ((long)hb * pieces), 16L}));
   const dim3 grid((unsigned)((a.b.ntok + tb - 1) / tb), a.b.nseq, (heads + hb - 1) / hb);
-  const size_t lds = (size_t)tb * a.half * sizeof(float2);
-  if (a.neox) hipLaunchKernelGGL((k_rope<TYPE, W, true>), grid, dim3(256), lds, st, a, tb, hb);
-  else hipLaunchKernelGGL((k_rope<TYPE, W, false>), grid, dim3(256), lds, st, a, tb, hb);
+  hipLaunchKernelGGL((k_rope<TYPE, W, HALF, WHOLE>), grid, dim3(256), (size_t)tb * a.half * sizeof(float2), st, a, tb, hb);
   ZL_HIP(hipGetLastError());
 }
 
 template <int TYPE>
 static void launch_rope_t(const RopeArgs &a, hipStream_t st) {
-  constexpr int W = 16 / sizeof(typename ValueOf<TYPE>::t);
-  if (whole_pieces(a, sizeof(typename ValueOf<TYPE>::t))) launch_rope_k<TYPE, W>(a, st);
-  else launch_rope_k<TYPE, 1>(a, st);
+  constexpr int V = 16 / value_size<TYPE>();
+  const bool whole = whole_pieces(a, value_size<TYPE>());
+  if (!a.neox) whole ? launch_rope_k<TYPE, 1, false, true>(a, st) : launch_rope_k<TYPE, 1, false, false>(a, st);
+  else if (!whole) launch_rope_k<TYPE, 1, true, false>(a, st);
+  else if (a.half % V == 0) launch_rope_k<TYPE, V, true, true>(a, st);
+  else if (a.half % (V / 2) == 0) launch_rope_k<TYPE, V / 2, true, true>(a, st);
+  else if (a.half % 2 == 0) launch_rope_k<TYPE, 2, true, true>(a, st);
+  else launch_rope_k<TYPE, 1, true, true>(a, st);
 }
 void launch_rope(const RopeArgs &a, int type, hipStream_t st) {
   if (type == T_F32) launch_rope_t<T_F32>(a, st);
