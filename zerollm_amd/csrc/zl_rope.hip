@@ -18,20 +18,23 @@ __device__ __forceinline__ void turn_sincos(double t, float *c, float *s) {
 }
 
 template <int TYPE> constexpr int value_size() { return sizeof(typename ValueOf<TYPE>::t); }
-template <class T, int W> struct Piece { typedef T t __attribute__((ext_vector_type(W))); };
+template <class T, int W> struct Piece {
+  typedef T t __attribute__((ext_vector_type(W)));
+  typedef t loose __attribute__((aligned(sizeof(T))));  // one that starts at any value
+};
 
 // A block takes `tb` tokens of a sequence and a share of their heads (blockIdx.z): the tokens' cos and sin go to LDS once, then
 // every lane takes pieces of the rows. WHOLE: every row is whole 16-byte pieces of V values. Neighbouring pairs: a piece's pairs
-// are rotated or pass through one by one. Halves: W pairs' firsts and seconds, W the largest that divides the half, then the pieces
-// behind the rotated values, of which the first may start among them. Bound by HBM: each value is read and written once (16384
-// tokens of 40 heads of 128, 64 rotated, bf16: 84 us, 4.0 TB/s; with whole pieces only where the parts of the head were some too,
-// 2 of 64 values rotated took 59 us a call of 11269 tokens of 24 heads, and take 21).
-template <int TYPE, int W, bool HALF, bool WHOLE>
+// are rotated or pass through one by one. Halves: V pairs' firsts and seconds (which start anywhere), the last ones of a half one by
+// one, then the pieces behind the rotated values, of which the first may start among them. Bound by HBM: each value is read and written once (16384
+// tokens of 40 heads of 128, 64 rotated, bf16: 80 us, 4.2 TB/s; with whole pieces only where the parts of the head were some too,
+// 2 of 64 values rotated took 59 us a call of 11269 tokens of 24 heads; they take 18 as neighbours, 35 as halves).
+template <int TYPE, bool HALF, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) {
   typedef typename ValueOf<TYPE>::t T;
   constexpr int V = WHOLE ? 16 / sizeof(T) : 1;
-  typedef typename Piece<T, W>::t vec;
   typedef typename Piece<T, V>::t whole;
+  typedef typename Piece<T, V>::loose loose;
   extern __shared__ float2 cs[];  // [tokens][half]
   const int s = blockIdx.y, tid = threadIdx.x, t0 = blockIdx.x * tb, half = a.half, nrot = 2 * half;
   const int nt = min(tb, (a.b.count ? max(0, min(a.b.count[s], a.b.ntok)) : a.b.ntok) - t0);
@@ -45,7 +48,7 @@ __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) 
   }
   __syncthreads();
   // pieces of a head: rotated ones, then those behind
-  const int rp = HALF ? half / W : WHOLE ? a.hd / V : half, items = rp + (HALF || !WHOLE ? a.hd / V - nrot / V : 0);
+  const int rp = HALF ? (half + V - 1) / V : WHOLE ? a.hd / V : half, items = rp + (HALF || !WHOLE ? a.hd / V - nrot / V : 0);
   const int h0 = blockIdx.z * hb, nh = min(hb, a.nq + a.nk - h0), total = nt * nh * items;
   for (int i = tid; i < total; i += 256) {
     const int row = i / items, r = i - row * items, t = row / nh, h = h0 + row - t * nh;
@@ -60,26 +63,44 @@ __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int tb, int hb) 
       if (d >= nrot) {
         *(whole *)(yp + d) = u;
       } else {
+        typedef typename Piece<T, 2>::t two;
         #pragma unroll
-        for (int e = 0; e < V; e++)
-          if (d + e >= nrot) yp[d + e] = u[e];
+        for (int e = 0; e < V; e += 2)  // (rotated values come in twos)
+          if (d + e >= nrot) *(two *)(yp + d + e) = two{u[e], u[e + 1]};
       }
       continue;
     }
     const float2 *f = cs + t * half;
     if constexpr (HALF) {
-      const int d = r * W;
-      const vec u = *(const vec *)(xp + d), v = *(const vec *)(xp + d + half);
-      vec w, z;
-      #pragma unroll
-      for (int e = 0; e < W; e++) {
-        const float x0 = load_value<TYPE>(u[e]), x1 = load_value<TYPE>(v[e]);
-        const float2 g = f[d + e];
-        w[e] = store_value<TYPE>(fmaf(x0, g.x, -(x1 * g.y)));
-        z[e] = store_value<TYPE>(fmaf(x0, g.y, x1 * g.x));
+      const int d = r * V;
+      auto turn = [&](float x0, float x1, int i, T *y0, T *y1) {
+        const float2 g = f[i];
+        *y0 = store_value<TYPE>(fmaf(x0, g.x, -(x1 * g.y)));
+        *y1 = store_value<TYPE>(fmaf(x0, g.y, x1 * g.x));
+      };
+      if (d + V <= half) {
+        whole u = *(const whole *)(xp + d), v = *(const loose *)(xp + d + half);
+        #pragma unroll
+        for (int e = 0; e < V; e++) {
+          T y0, y1;
+          turn(load_value<TYPE>(u[e]), load_value<TYPE>(v[e]), d + e, &y0, &y1);
+          u[e] = y0;
+          v[e] = y1;
+        }
+        *(whole *)(yp + d) = u;
+        *(loose *)(yp + d + half) = v;
+      } else {
+        T u[V], v[V];  // (all loads before the stores: one wait)
+        #pragma unroll
+        for (int e = 0; e < V - 1; e++) {
+          const int i = min(d + e, half - 1);
+          u[e] = xp[i];
+          v[e] = xp[i + half];
+        }
+        #pragma unroll
+        for (int e = 0; e < V - 1; e++)
+          if (d + e < half) turn(load_value<TYPE>(u[e]), load_value<TYPE>(v[e]), d + e, yp + d + e, yp + d + e + half);
       }
-      *(vec *)(yp + d) = w;
-      *(vec *)(yp + d + half) = z;
     } else if constexpr (WHOLE) {
       const int d = r * V;
       whole u = *(const whole *)(xp + d);
@@ -110,32 +131,27 @@ static bool whole_pieces(const RopeArgs &a, int vb) {
   return ok(a.q) && ok(a.qo) && (!a.nk || (ok(a.k) && ok(a.ko))) && a.hd % w == 0;
 }
 
-template <int TYPE, int W, bool HALF, bool WHOLE>
+template <int TYPE, bool HALF, bool WHOLE>
 static void launch_rope_k(const RopeArgs &a, hipStream_t st) {
   // Tokens and heads per block: pieces for every lane a few times over where there are many tokens, as many blocks as CUs
   // where there are few (each of which forms its tokens' cos and sin itself: 2 half values a block).
   constexpr int V = WHOLE ? 16 / value_size<TYPE>() : 1;
   const int heads = a.nq + a.nk, nrot = 2 * a.half;
-  const int pieces = HALF ? a.half / W + a.hd / V - nrot / V : WHOLE ? a.hd / V : a.half + a.hd - nrot;
+  const int pieces = HALF ? (a.half + V - 1) / V + a.hd / V - nrot / V : WHOLE ? a.hd / V : a.half + a.hd - nrot;
   const long all = (long)a.b.ntok * a.b.nseq * heads * pieces;
   const long per = std::max(256L, std::min(4096L, all / 512));  // pieces per block
   const int hb = (int)std::max(1L, std::min((long)heads, per / pieces));
   const int tb = (int)std::max(1L, std::min({(long)a.b.ntok, per / ((long)hb * pieces), 16L}));
   const dim3 grid((unsigned)((a.b.ntok + tb - 1) / tb), a.b.nseq, (heads + hb - 1) / hb);
-  hipLaunchKernelGGL((k_rope<TYPE, W, HALF, WHOLE>), grid, dim3(256), (size_t)tb * a.half * sizeof(float2), st, a, tb, hb);
+  hipLaunchKernelGGL((k_rope<TYPE, HALF, WHOLE>), grid, dim3(256), (size_t)tb * a.half * sizeof(float2), st, a, tb, hb);
   ZL_HIP(hipGetLastError());
 }
 
 template <int TYPE>
 static void launch_rope_t(const RopeArgs &a, hipStream_t st) {
-  constexpr int V = 16 / value_size<TYPE>();
   const bool whole = whole_pieces(a, value_size<TYPE>());
-  if (!a.neox) whole ? launch_rope_k<TYPE, 1, false, true>(a, st) : launch_rope_k<TYPE, 1, false, false>(a, st);
-  else if (!whole) launch_rope_k<TYPE, 1, true, false>(a, st);
-  else if (a.half % V == 0) launch_rope_k<TYPE, V, true, true>(a, st);
-  else if (a.half % (V / 2) == 0) launch_rope_k<TYPE, V / 2, true, true>(a, st);
-  else if (a.half % 2 == 0) launch_rope_k<TYPE, 2, true, true>(a, st);
-  else launch_rope_k<TYPE, 1, true, true>(a, st);
+  if (a.neox) whole ? launch_rope_k<TYPE, true, true>(a, st) : launch_rope_k<TYPE, true, false>(a, st);
+  else whole ? launch_rope_k<TYPE, false, true>(a, st) : launch_rope_k<TYPE, false, false>(a, st);
 }
 void launch_rope(const RopeArgs &a, int type, hipStream_t st) {
   if (type == T_F32) launch_rope_t<T_F32>(a, st);
