@@ -208,9 +208,9 @@ void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows 
 // Products run on the matrix cores (v_mfma_f32_16x16x32_f16) for 16 rows at a time: keys times queries first, which leaves
 // lane l with the scores of row l % 16 at four neighbouring positions, then values (as the left operand) times weights,
 // which takes those positions as they lie. Codes less 8 are exact in f16. Queries are scaled per row by a power of two to
-// below 2^14 and split into two f16 parts (22 bits; 16-bit queries need one); a weight times its value's scale likewise where
-// the output is f32 or f16: rounded to one f16 part, and the product again, it would be off by 2^-11 twice, more than the
-// rounding of an f16 output (3.4e-4 of the output together, against 2.0e-4). bf16 outputs are rounded by 2^-8, and have one. Scores are scaled by their key's scale in f32, block by block.
+// below 2^14 and split into two f16 parts (22 bits; 16-bit queries need one); a weight times its value's scale likewise, whatever the
+// output's type: rounded to one f16 part, and the product again, it would be off by 2^-11 twice, more than an f16 output's own
+// rounding, and one bf16 output in eight or so would be another number than the rounded f32 one. Scores are scaled by their key's scale in f32, block by block.
 constexpr int SPAN = 64, CHUNK = 256, PART = 1024;
 constexpr int CHUNKS = PART / CHUNK;
 
@@ -223,8 +223,8 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 // TINY: as they lie, f16 denormals of code 2^-24, which the matrix cores take; the 2^24 and the 8 to be taken off follow the
 // sums. Sums of denormals lose bits (of codes less 8 too: 5e-6 of an output from f32 rows against 2e-7), to one side: where 131000
 // values cancel to 1 in 360 of their size, 2e-4 of it, as much as an f16 output's own rounding. So this is for the scores of 16-bit
-// rows and the sums of bf16 ones. Scores take pairs 1 and 3 four bits higher (16 code 2^-24, and a sixteenth of their queries): a
-// shift a word (12 cycles of a SIMD) for three (16).
+// rows. They take pairs 1 and 3 four bits higher (16 code 2^-24, and a sixteenth of their queries): a shift a word (12 cycles of a
+// SIMD).
 // Else: less 8, under an exponent and less the sum of both: 1024 where the code is in the lowest bits, 64 where it is four higher
 // (no shift; 36 cycles a word).
 // The constants are in vector registers: a 32-bit operation takes 2 cycles of a SIMD from two waves' vector operands and 4 with a
@@ -233,16 +233,14 @@ struct Unpack {
   uint32_t mask = 0x000f000fu, k1024 = 0x64006400u, mask4 = 0x00f000f0u, k64 = 0x54005400u;
   __device__ __forceinline__ Unpack() { __asm__("" : "+v"(mask), "+v"(k1024), "+v"(mask4), "+v"(k64)); }
 };
-enum { SIGNED, CODES, CODES16 };  // codes less 8; codes; codes, those of odd pairs times 16
+enum { SIGNED, CODES16 };  // codes less 8; codes, those of odd pairs times 16
 template <int HOW>
 __device__ __forceinline__ h8 unpack8(uint32_t w, const Unpack &k) {
   u4 x;
   #pragma unroll
   for (int r = 0; r < 4; r++) {
     const uint32_t v = r < 2 ? w : w >> 8;
-    if constexpr (HOW == CODES) {
-      x[r] = (w >> (4 * r)) & k.mask;
-    } else if constexpr (HOW == CODES16) {
+    if constexpr (HOW == CODES16) {
       x[r] = v & (r & 1 ? k.mask4 : k.mask);
     } else {
       const h2 p = r & 1 ? __builtin_bit_cast(h2, (v & k.mask4) | k.k64) - (h2){72, 72} : __builtin_bit_cast(h2, (v & k.mask) | k.k1024) - (h2){1032, 1032};
@@ -252,7 +250,6 @@ __device__ __forceinline__ h8 unpack8(uint32_t w, const Unpack &k) {
   return __builtin_bit_cast(h8, x);
 }
 constexpr float TINY_ONE = 16777216.0f;  // 2^24: a code's unit
-constexpr h8 ONES = {1, 1, 1, 1, 1, 1, 1, 1};
 // Scale v (of four positions) of entry i (position tile and block) of a lane's loads: taken out of its register where it is
 // used, as an operand half.
 template <int N>
@@ -444,13 +441,11 @@ __device__ __forceinline__ void mask_scales(u4 (&vs)[NB], int i, int lim, int g)
 }
 
 // Weights of a lane's positions (four neighbouring ones of each tile of both records) in two f16 parts.
-template <bool LOW>
 struct Weights {
   h2 hi[2][2][2], lo[2][2][2];  // [record][tile][pair]
 };
 // Scores to weights; the span's reference and the sum of its weights.
-template <bool LOW>
-__device__ __forceinline__ void span_softmax(const f4 (&s)[2][2], float c, Weights<LOW> &w, float &m, float &l) {
+__device__ __forceinline__ void span_softmax(const f4 (&s)[2][2], float c, Weights &w, float &m, float &l) {
   float x = -INFINITY;
   #pragma unroll
   for (int i = 0; i < 2; i++)
@@ -473,27 +468,25 @@ __device__ __forceinline__ void span_softmax(const f4 (&s)[2][2], float c, Weigh
         const h2 h = {(_Float16)p0, (_Float16)p1};
         w.hi[i][t][v >> 1] = h;
         // (the differences are exact, so that they are rounded once in whatever instructions they are formed)
-        if (LOW) w.lo[i][t][v >> 1] = (h2){(_Float16)fmaf(-1.0f, (float)h[0], p0), (_Float16)fmaf(-1.0f, (float)h[1], p1)};
+        w.lo[i][t][v >> 1] = (h2){(_Float16)fmaf(-1.0f, (float)h[0], p0), (_Float16)fmaf(-1.0f, (float)h[1], p1)};
       }
   m = x * c - 3.0f;
   l = sum4(l);
 }
 
-// Weights of record i times the value scales d of block b, as right operands, in packed f16: hi = f16(ph d), and with LOW the
-// rest lo = f16(f16(ph d - hi) + pl d), the inner difference exact. Every step rounds once, in whichever kernel it is.
-template <int NB, bool LOW>
-__device__ __forceinline__ void weigh(const Weights<LOW> &w, const u4 (&vs)[NB], int i, int b, h8 &hi, h8 &lo) {
+// Weights of record i times the value scales d of block b, as right operands, in packed f16: hi = f16(ph d), and the rest
+// lo = f16(f16(ph d - hi) + pl d), the inner difference exact. Every step rounds once, in whichever kernel it is.
+template <int NB>
+__device__ __forceinline__ void weigh(const Weights &w, const u4 (&vs)[NB], int i, int b, h8 &hi, h8 &lo) {
   const uint32_t d[4] = {vs[b >> 1][2 * (b & 1)], vs[b >> 1][2 * (b & 1) + 1], vs[(NB + b) >> 1][2 * (b & 1)], vs[(NB + b) >> 1][2 * (b & 1) + 1]};
   #pragma unroll
   for (int k = 0; k < 4; k++) {
     const h2 e = __builtin_bit_cast(h2, d[k]), p = w.hi[i][k >> 1][k & 1], h = p * e;
     hi[2 * k] = h[0];
     hi[2 * k + 1] = h[1];
-    if (LOW) {
-      const h2 r = __builtin_elementwise_fma(w.lo[i][k >> 1][k & 1], e, __builtin_elementwise_fma(p, e, -h));
-      lo[2 * k] = r[0];
-      lo[2 * k + 1] = r[1];
-    }
+    const h2 r = __builtin_elementwise_fma(w.lo[i][k >> 1][k & 1], e, __builtin_elementwise_fma(p, e, -h));
+    lo[2 * k] = r[0];
+    lo[2 * k + 1] = r[1];
   }
 }
 
@@ -549,28 +542,15 @@ struct ToModel {
   __device__ __forceinline__ void emit(int, int tok, int head, int dim, float o) const { attn_emit(h, tok, head, dim, o + 0.0f); }
 };
 
-// A span's two products of block b and record: values times weights, and with TINY the weights' sums.
-template <bool LOW, bool TINY>
-__device__ __forceinline__ void weighted_sums(f4 &o0, f4 &o1, f4 &wsum, h8 x0, h8 x1, h8 hi, h8 lo) {
+// A span's products of block b and record: values times weights.
+__device__ __forceinline__ void weighted_sums(f4 &o0, f4 &o1, h8 x0, h8 x1, h8 hi, h8 lo) {
   o0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, hi, o0, 0, 0, 0);
   o1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, hi, o1, 0, 0, 0);
-  if (TINY) wsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ONES, hi, wsum, 0, 0, 0);
-  if (LOW) {
-    o0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, lo, o0, 0, 0, 0);
-    o1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, lo, o1, 0, 0, 0);
-    if (TINY) wsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ONES, lo, wsum, 0, 0, 0);
-  }
-}
-// TINY: sums of codes to sums of codes less 8.
-template <int NB>
-__device__ __forceinline__ void take_off(f4 (&o)[2 * NB], const f4 (&wsum)[NB]) {
-  #pragma unroll
-  for (int j = 0; j < 2 * NB; j++)
-    #pragma unroll
-    for (int v = 0; v < 4; v++) o[j][v] = fmaf(o[j][v], TINY_ONE, -8.0f * wsum[j >> 1][0]);  // (all rows of wsum are the same)
+  o0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, lo, o0, 0, 0, 0);
+  o1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, lo, o1, 0, 0, 0);
 }
 
-// Positions per record of a sequence's rows (of k_kv4_chunks): by the sequence's last position, so that all its rows agree.
+// Positions per record of a sequence's rows (of k_kv4_rows<.., false>): by the sequence's last position, so that all its rows agree.
 __device__ __forceinline__ int record_len(const Kv4Attn &a, int s) {
   const long last = min((long)a.b.pos[s] + count_of(a.b, s), a.c.cap) - 1;
   return last < (long)a.spanmax * SPAN ? SPAN : CHUNK;
@@ -613,7 +593,7 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 template <int NB, int TYPE, bool MANY>
 __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
-  constexpr bool LOQ = TYPE == T_F32, LOW = TYPE != T_BF16, TINY = !LOQ, TINYV = TYPE == T_BF16, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
+  constexpr bool LOQ = TYPE == T_F32, TINY = !LOQ, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   // the wave's tile, and its first chunk (MANY: part) and the step to the next
   long group;  // [sequence][KV head][block of chunks (a part)]
@@ -678,27 +658,24 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
           mask_scales<NB>(w.vs[1], 1, lim, g);
         }
         Sum<8 * NB> r;
-        Weights<LOW> pw;
-        span_softmax<LOW>(s, q.c, pw, r.m, r.l);
-        f4 o[2 * NB], wsum[NB];
+        Weights pw;
+        span_softmax(s, q.c, pw, r.m, r.l);
+        f4 o[2 * NB];
         #pragma unroll
         for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        #pragma unroll
-        for (int b = 0; b < NB; b++) wsum[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         #pragma unroll
         for (int i = 0; i < 2; i++)
           #pragma unroll
           for (int b = 0; b < NB; b++) {
             h8 hi, lo;
-            weigh<NB, LOW>(pw, w.vs[i], i, b, hi, lo);
-            const h8 x0 = unpack8<TINYV ? CODES : SIGNED>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<TINYV ? CODES : SIGNED>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
-            weighted_sums<LOW, TINYV>(o[2 * b], o[2 * b + 1], wsum[b], x0, x1, hi, lo);
+            weigh<NB>(pw, w.vs[i], i, b, hi, lo);
+            const h8 x0 = unpack8<SIGNED>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<SIGNED>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
+            weighted_sums(o[2 * b], o[2 * b + 1], x0, x1, hi, lo);
             __builtin_amdgcn_sched_barrier(0);
           }
         if (AHEAD) w.load_values(next, lane);
         else w.load_keys(next, lane);
         __builtin_amdgcn_sched_barrier(0);
-        if (TINYV) take_off<NB>(o, wsum);
         #pragma unroll
         for (int j = 0; j < 2 * NB; j++)
           #pragma unroll
