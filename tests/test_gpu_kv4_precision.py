@@ -39,3 +39,20 @@ def test_outputs_of_16_bits_are_rounded_once(gpu, dim, kv, group, tokens, t):
         ok = is_rounding(got[:, h], want, off, t)
         assert ok.all(), (h, (~ok).sum(), ok.size, np.abs(got[:, h] - want).max())
     c.close()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,kv,group,tokens,n", [(64, 2, 1, 1, 700), (128, 2, 4, 9, 5000), (256, 1, 3, 5, 1300), (128, 8, 8, 160, 2100), (64, 8, 4, 64, 33000)])
+def test_16_bit_rows_are_the_f32_rows_rounded(gpu, dim, kv, group, tokens, n, t):
+    """Queries of 16 bits are exact in the f16 part that f32 queries have too, and every step after that is the same: the outputs are
+    the roundings of the f32 ones, bit for bit. Also keys with a few channels much larger than the rest."""
+    c = cache(1, kv, dim, n)
+    for spread in (0.5, 1.5):
+        k, v = rows(7, (1, n, kv, dim), spread=spread), rows(8, (1, n, kv, dim))
+        c.append(k, v, ints(0))
+        q = (rows(9, (1, tokens, kv * group, dim)) * 4).to(TYPES[t])
+        print(f"case rounded f32 dim {dim} tokens {tokens} {t} spread {spread}", flush=True)
+        for first in (0, n - tokens):
+            got, want = c.attend(q, ints(first)), c.attend(q.float(), ints(first))
+            assert torch.isfinite(got).all() and (got == want.to(TYPES[t])).all()
+    c.close()

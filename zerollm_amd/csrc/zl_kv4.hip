@@ -219,37 +219,26 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// The eight codes of a word as f16 operands: pair r of (word >> 4 r).
-// TINY: as they lie, f16 denormals of code 2^-24, which the matrix cores take; the 2^24 and the 8 to be taken off follow the
-// sums. Sums of denormals lose bits (of codes less 8 too: 5e-6 of an output from f32 rows against 2e-7), to one side: where 131000
-// values cancel to 1 in 360 of their size, 2e-4 of it, as much as an f16 output's own rounding. So this is for the scores of 16-bit
-// rows. They take pairs 1 and 3 four bits higher (16 code 2^-24, and a sixteenth of their queries): a shift a word (12 cycles of a
-// SIMD).
-// Else: less 8, under an exponent and less the sum of both: 1024 where the code is in the lowest bits, 64 where it is four higher
-// (no shift; 36 cycles a word).
+// The eight codes of a word, less 8, as f16 operands: pair r of (word >> 4 r), under an exponent and less the sum of both: 1024 where
+// the code is in the lowest bits, 64 where it is four higher (no shift; 36 cycles a word). (Codes as they lie, as f16 denormals, take
+// 12, but the matrix cores' sums of those lose bits: outputs of f16 rows other than the rounded f32 ones 2 to 4 % instead of 0.1 to
+// 0.4, for 190 us instead of 200 a call of 256 tokens after 12000 positions.)
 // The constants are in vector registers: a 32-bit operation takes 2 cycles of a SIMD from two waves' vector operands and 4 with a
 // scalar one, and and-or takes a single scalar one.
 struct Unpack {
   uint32_t mask = 0x000f000fu, k1024 = 0x64006400u, mask4 = 0x00f000f0u, k64 = 0x54005400u;
   __device__ __forceinline__ Unpack() { __asm__("" : "+v"(mask), "+v"(k1024), "+v"(mask4), "+v"(k64)); }
 };
-enum { SIGNED, CODES16 };  // codes less 8; codes, those of odd pairs times 16
-template <int HOW>
 __device__ __forceinline__ h8 unpack8(uint32_t w, const Unpack &k) {
   u4 x;
   #pragma unroll
   for (int r = 0; r < 4; r++) {
     const uint32_t v = r < 2 ? w : w >> 8;
-    if constexpr (HOW == CODES16) {
-      x[r] = v & (r & 1 ? k.mask4 : k.mask);
-    } else {
-      const h2 p = r & 1 ? __builtin_bit_cast(h2, (v & k.mask4) | k.k64) - (h2){72, 72} : __builtin_bit_cast(h2, (v & k.mask) | k.k1024) - (h2){1032, 1032};
-      x[r] = __builtin_bit_cast(uint32_t, p);
-    }
+    const h2 p = r & 1 ? __builtin_bit_cast(h2, (v & k.mask4) | k.k64) - (h2){72, 72} : __builtin_bit_cast(h2, (v & k.mask) | k.k1024) - (h2){1032, 1032};
+    x[r] = __builtin_bit_cast(uint32_t, p);
   }
   return __builtin_bit_cast(h8, x);
 }
-constexpr float TINY_ONE = 16777216.0f;  // 2^24: a code's unit
 // Scale v (of four positions) of entry i (position tile and block) of a lane's loads: taken out of its register where it is
 // used, as an operand half.
 template <int N>
@@ -315,10 +304,9 @@ __device__ __forceinline__ void fold_all(Sum<N> &f, const float2 (&ml)[K], const
 
 // The queries of a tile of 16 rows as right operands: lane l has row l % 16, dimensions 32 b + 8 (l / 16) + e; and the factor
 // from the products (code units, scaled queries) to scores in powers of two.
-template <int NB, bool TINY>
+template <int NB>
 struct Queries {
   h8 hi[NB], lo[NB];
-  f4 z[NB];  // TINY: -8 2^-24 times the sum of block b of the lane's row, where the scores' sums start; else 0
   float c;
 };
 template <int NB, int TYPE>
@@ -332,8 +320,8 @@ __device__ __forceinline__ void fetch_queries(float (&v)[NB][8], const typename 
     for (int b = 0; b < NB; b++) load8<TYPE, false>(p + 32 * b, v[b]);
   }
 }
-template <int NB, bool TINY>
-__device__ __forceinline__ void set_queries(Queries<NB, TINY> &q, const float (&v)[NB][8], float scale) {
+template <int NB>
+__device__ __forceinline__ void set_queries(Queries<NB> &q, const float (&v)[NB][8], float scale) {
   float am = 0.0f, any = 0.0f;
   #pragma unroll
   for (int b = 0; b < NB; b++)
@@ -351,25 +339,20 @@ __device__ __forceinline__ void set_queries(Queries<NB, TINY> &q, const float (&
   const float up = __uint_as_float((uint32_t)(127 + ex) << 23) + any;
   #pragma unroll
   for (int b = 0; b < NB; b++) {
-    float sum = 0.0f;
     u4 hi, lo;
     #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float pair = TINY && (e & 1) ? up * 0.0625f : up;
-      const float x0 = v[b][2 * e] * pair, x1 = v[b][2 * e + 1] * pair;
+      const float x0 = v[b][2 * e] * up, x1 = v[b][2 * e + 1] * up;
       const h2 h = {(_Float16)x0, (_Float16)x1};
       const h2 r = {(_Float16)fmaf(-1.0f, (float)h[0], x0), (_Float16)fmaf(-1.0f, (float)h[1], x1)};
       hi[e] = __builtin_bit_cast(uint32_t, h);
       lo[e] = __builtin_bit_cast(uint32_t, r);
-      if (TINY) sum = fmaf((float)h[0] + (float)h[1], e & 1 ? 16.0f : 1.0f, sum);
     }
     q.hi[b] = __builtin_bit_cast(h8, hi);
     q.lo[b] = __builtin_bit_cast(h8, lo);
-    sum = TINY ? sum4(sum) * (-8.0f / TINY_ONE) : 0.0f;
-    q.z[b] = f4{sum, sum, sum, sum};
   }
   // (neither 0 nor infinite: it multiplies infinities and zeros)
-  q.c = fminf(fmaxf((float)ldexp((double)scale * 1.4426950408889634, TINY ? 24 - ex : -ex), 1.17549435e-38f), 3.40282347e38f);
+  q.c = fminf(fmaxf((float)ldexp((double)scale * 1.4426950408889634, -ex), 1.17549435e-38f), 3.40282347e38f);
 }
 
 // A lane's share of a span (two records): code words and scales, loaded with every lane's 16-byte loads side by side.
@@ -399,12 +382,12 @@ struct SpanWords {
 
 // Scores of 16 positions (tile t of a record) in code units, from the tile's operands k(b) and key scales.
 template <int NB, bool LOQ, class K>
-__device__ __forceinline__ f4 tile_scores(const K &k, const u4 (&ks)[NB], int t, const Queries<NB, !LOQ> &q) {
+__device__ __forceinline__ f4 tile_scores(const K &k, const u4 (&ks)[NB], int t, const Queries<NB> &q) {
   f4 s = f4{0.0f, 0.0f, 0.0f, 0.0f};
   #pragma unroll
   for (int b = 0; b < NB; b++) {
     const h8 x = k(b);
-    f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[b], q.z[b], 0, 0, 0);
+    f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[b], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
     if (LOQ) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.lo[b], acc, 0, 0, 0);
     #pragma unroll
     for (int v = 0; v < 4; v++) s[v] = fmaf(acc[v], scale_at(ks, t * NB + b, v), s[v]);
@@ -593,7 +576,7 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 template <int NB, int TYPE, bool MANY>
 __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
-  constexpr bool LOQ = TYPE == T_F32, TINY = !LOQ, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
+  constexpr bool LOQ = TYPE == T_F32, AHEAD = NB <= 4;  // (heads of 256 leave no registers for loads ahead)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   // the wave's tile, and its first chunk (MANY: part) and the step to the next
   long group;  // [sequence][KV head][block of chunks (a part)]
@@ -617,7 +600,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
   const Unpack uk;
   // (loads complete in order: the queries, which take a while to prepare, are requested first)
   SpanWords<NB> w;
-  Queries<NB, TINY> q;
+  Queries<NB> q;
   {
     float qv[NB][8];
     fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.qvec, lane);
@@ -625,7 +608,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
     w.load_keys(rec, lane);
     if (AHEAD) w.load_values(rec, lane);
     __builtin_amdgcn_sched_barrier(0);
-    set_queries<NB, TINY>(q, qv, a.scale);
+    set_queries<NB>(q, qv, a.scale);
   }
   for (int c = c0; (long)c * unit <= most; c += step) {
     const int ns = min(unit / SPAN, (most - c * unit) / SPAN + 1);
@@ -646,7 +629,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
         for (int i = 0; i < 2; i++)
           #pragma unroll
           for (int t = 0; t < 2; t++) {
-            s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8<TINY ? CODES16 : SIGNED>(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], uk); }, w.ks[i], t, q);
+            s[i][t] = tile_scores<NB, LOQ>([&](int b) { return unpack8(w.kw[i][(t * NB + b) >> 2][(t * NB + b) & 3], uk); }, w.ks[i], t, q);
             __builtin_amdgcn_sched_barrier(0);
           }
         if (AHEAD) w.load_keys(next, lane);
@@ -669,7 +652,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
           for (int b = 0; b < NB; b++) {
             h8 hi, lo;
             weigh<NB>(pw, w.vs[i], i, b, hi, lo);
-            const h8 x0 = unpack8<SIGNED>(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8<SIGNED>(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
+            const h8 x0 = unpack8(w.vw[i][(2 * b) >> 2][(2 * b) & 3], uk), x1 = unpack8(w.vw[i][(2 * b + 1) >> 2][(2 * b + 1) & 3], uk);
             weighted_sums(o[2 * b], o[2 * b + 1], x0, x1, hi, lo);
             __builtin_amdgcn_sched_barrier(0);
           }
