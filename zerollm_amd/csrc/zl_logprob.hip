@@ -28,7 +28,7 @@ struct RowSum {
   __device__ __forceinline__ void raise(float to) {  // to >= m, above -inf
     if (m == -INFINITY) { m = to; return; }
     const float d = m - to, f = __builtin_amdgcn_exp2f(d * 1.44269504f);
-    e = d == -INFINITY ? 0.0f : f * fmaf(l, d, e);
+    e = f == 0.0f ? 0.0f : f * fmaf(l, d, e);  // (f is 0 from d = -104 on, where l d may be infinite: masks of -1e38, a type's lowest value)
     l *= f;
     m = to;
   }
