@@ -1,5 +1,5 @@
 """How exact the attention over the 4-bit cache is, where a bound relative to the largest values would not show it: 16-bit outputs
-are the roundings of numbers within f32's errors of float64's."""
+are the roundings of numbers within f32's errors of float64's, f32 rows of values of any size relative to those."""
 import numpy as np
 import pytest
 import torch
@@ -55,4 +55,55 @@ def test_16_bit_rows_are_the_f32_rows_rounded(gpu, dim, kv, group, tokens, n, t)
         for first in (0, n - tokens):
             got, want = c.attend(q, ints(first)), c.attend(q.float(), ints(first))
             assert torch.isfinite(got).all() and (got == want.to(TYPES[t])).all()
+    c.close()
+
+
+def whole_scores(dim, kv, group, n, tokens, t, seed):
+    """Keys in blocks of scale 1 and queries of whole numbers, and a scale: every product and sum of a score is a whole number below
+    2^24, so that its order does not matter, over a range of some 10 after the scale. The products are up to 200 times what their
+    sums come to."""
+    g = torch.Generator().manual_seed(seed)
+    k = torch.randint(-7, 8, (1, n, kv, dim), generator=g).float()
+    k[..., ::32] = -8.0
+    q = torch.randint(-250, 251, (1, tokens, kv * group, dim), generator=g).float()
+    return k.cuda(), q.to(TYPES[t]).cuda(), 2.0 ** -12 * (64 / dim) ** 0.5
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("magnitude", [1e-1, 3e-2, 1e-2, 1e-3, 1e-4, 1e-5, 1e-6, "mixed", "one"])
+@pytest.mark.parametrize("dim,tokens,group", [(64, 1, 2), (128, 9, 4), (256, 3, 1), (128, 300, 8)])
+def test_small_values_keep_their_bits(gpu, dim, tokens, group, magnitude, t):
+    """Values of a size, of another size in every block of 32, and one position a thousand times the others. With the largest value
+    scale of a span's block raised to 2^-5 at least and the largest weight 8, a weight times its scale is off by 2^-25 and 2^-22 of
+    itself, at a code of at most 8, over 64 positions whose weights sum to 8 or more: 2^-17 of the block's largest value. Whole scores,
+    and f32 sums of spans (64 terms) and their folds (some 40), relative to the mean |v|."""
+    kv, n = (2, 1000) if tokens > 100 else (1, 1000)
+    k, q, scale = whole_scores(dim, kv, group, n, tokens, t, dim + tokens)
+    v = rows(52, (1, n, kv, dim))
+    if magnitude == "mixed":
+        v = v * (10.0 ** -(torch.arange(dim // 32) * 5 % 7)).repeat_interleave(32).cuda()
+    elif magnitude == "one":
+        v *= 1e-4
+        v[:, 777] *= 1e3
+    else:
+        v *= magnitude
+    c = cache(1, kv, dim, n + 2000 * (tokens > 100))
+    c.append(k, v, ints(0))
+    print(f"case small values {magnitude} dim {dim} tokens {tokens} {t}", flush=True)
+    got = f64(c.attend(q, ints(n - tokens), scale=scale))[0]
+    kk, vv, qq = stored(f64(k))[0], stored(f64(v))[0], f64(q)[0]
+    last = n - tokens + np.arange(tokens)
+    worst = 0.0
+    for h in range(kv * group):
+        x, y = kk[:, h // group], vv[:, h // group]
+        want, _ = attention(qq[:, h], x, y, last, scale)
+        mean, _ = attention(qq[:, h], x, np.abs(y), last, scale)
+        top = np.abs(x @ qq[:, h].T).max() * scale
+        assert top < 20
+        big = np.repeat(np.abs(y).reshape(n, -1, 32).max((0, 2)), 32)
+        off = mean * (4 * top * 2.0 ** -22 + 2 * 128 * 2.0 ** -24 + 2.0 ** -20) + big * 2.0 ** -17
+        ok = is_rounding(got[:, h], want, off, t)
+        assert ok.all(), (h, (~ok).sum(), ok.size, (np.abs(got[:, h] - want) / off).max())
+        worst = max(worst, (np.abs(got[:, h] - want) / off).max())
+    print(f"worst error / bound {worst:.3f}", flush=True)
     c.close()

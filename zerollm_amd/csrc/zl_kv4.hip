@@ -248,14 +248,14 @@ __device__ __forceinline__ float scale_at(const u4 (&s)[N], int i, int v) {
 }
 __device__ __forceinline__ int wave_max(int v) { return group_reduce(v, 64, [](int x, int y) { return max(x, y); }); }
 // Over the four lanes l % 16 + 0, 16, 32, 48: rows of 16 lanes are swapped pairwise (16, then 32 apart), no trip through LDS.
-template <class Op>
-__device__ __forceinline__ float over4(float x, Op op) {
-  const uint32_t a = __float_as_uint(x);
+template <class T, class Op>
+__device__ __forceinline__ T over4(T x, Op op) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, x);
   const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false);
-  const float y = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
-  const uint32_t b = __float_as_uint(y);
+  const uint32_t p0 = p[0], p1 = p[1], b = __builtin_bit_cast(uint32_t, op(__builtin_bit_cast(T, p0), __builtin_bit_cast(T, p1)));
   const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-  return op(__uint_as_float(q[0]), __uint_as_float(q[1]));
+  const uint32_t q0 = q[0], q1 = q[1];
+  return op(__builtin_bit_cast(T, q0), __builtin_bit_cast(T, q1));
 }
 __device__ __forceinline__ float sum4(float x) { return over4(x, [](float a, float b) { return a + b; }); }
 __device__ __forceinline__ float max4(float x) { return over4(x, [](float a, float b) { return fmaxf(a, b); }); }
@@ -420,6 +420,66 @@ __device__ __forceinline__ void mask_scales(u4 (&vs)[NB], int i, int lim, int g)
       vs[e >> 1][2 * (e & 1)] &= m0;
       vs[e >> 1][2 * (e & 1) + 1] &= m1;
     }
+  }
+}
+
+// Value scales d of a block that are all below 2^-5: a weight times such a scale would end, in two f16 parts, at 2^-25 of the
+// weights' 8, 2^-23 of itself and less. Where a span's largest one is, for the lane's row, they are taken times 2^15, twice if that
+// leaves them there (denormals), which is exact, and the block's sums times the same less. By the row and the span's positions alone, so that a
+// row's bits do not depend on the batch. Returns two bits a block, the times.
+constexpr uint32_t SMALL_SCALE = 0x2800;  // 2^-5 in f16
+// Whether a block of the span may be such a one for any row that sees the span: none is where every lane has a scale of 2^-5 or more
+// among its four positions of tile 0 of record 0, in every block. The rest is left out then, which changes no bit.
+template <int NB>
+__device__ __forceinline__ bool maybe_small(const u4 (&vs)[NB], int lim) {
+  uint32_t all = 0x80008000u;
+  #pragma unroll
+  for (int b = 0; b < NB; b++) {
+    // (no carry from the lower half: 0x7fff + 0x5800 < 2^16)
+    constexpr uint32_t up = (0x8000u - SMALL_SCALE) * 0x10001u;
+    uint32_t x = ((vs[b >> 1][2 * (b & 1)] & 0x7fff7fffu) + up) | ((vs[b >> 1][2 * (b & 1) + 1] & 0x7fff7fffu) + up);
+    x |= x << 16;
+    all &= x;
+  }
+  return __ballot((all >> 31) == 0 && lim >= 0) != 0;
+}
+template <int NB>
+__device__ __forceinline__ uint32_t raise_small(u4 (&v0)[NB], u4 (&v1)[NB]) {
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+  uint32_t times = 0;
+  #pragma unroll 1
+  for (int round = 0; round < 2; round++) {
+    #pragma unroll
+    for (int b = 0; b < NB; b++) {
+      us2 m = {0, 0};
+      #pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const uint32_t x = v0[((k >> 1) * NB + b) >> 1][2 * (b & 1) + (k & 1)] & 0x7fff7fffu, y = v1[((k >> 1) * NB + b) >> 1][2 * (b & 1) + (k & 1)] & 0x7fff7fffu;
+        m = __builtin_elementwise_max(m, __builtin_elementwise_max(__builtin_bit_cast(us2, x), __builtin_bit_cast(us2, y)));
+      }
+      const uint32_t top = over4((uint32_t)max(m[0], m[1]), [](uint32_t x, uint32_t y) { return max(x, y); });  // (NaN above all)
+      const bool small = top < SMALL_SCALE;
+      const h2 f = small ? (h2){32768, 32768} : (h2){1, 1};
+      times += (small ? 1u : 0u) << (2 * b);
+      #pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int i = ((k >> 1) * NB + b) >> 1, j = 2 * (b & 1) + (k & 1);
+        const uint32_t w0 = v0[i][j], w1 = v1[i][j];
+        v0[i][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, w0) * f);
+        v1[i][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, w1) * f);
+      }
+    }
+    if (!__ballot(times != 0)) break;
+  }
+  return times;
+}
+template <int NB>
+__device__ __forceinline__ void lower_sums(f4 (&o)[2 * NB], uint32_t times) {
+  #pragma unroll
+  for (int b = 0; b < NB; b++) {
+    const float f = __uint_as_float((127u - 15u * (times >> (2 * b) & 3u)) << 23);
+    #pragma unroll
+    for (int v = 0; v < 4; v++) o[2 * b][v] *= f, o[2 * b + 1][v] *= f;
   }
 }
 
@@ -643,6 +703,10 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
         Sum<8 * NB> r;
         Weights pw;
         span_softmax(s, q.c, pw, r.m, r.l);
+        // (only here, where the values' loads have had the softmax to arrive)
+        const bool small = maybe_small<NB>(w.vs[0], lim);
+        uint32_t times = 0;
+        if (small) times = raise_small<NB>(w.vs[0], w.vs[1]);
         f4 o[2 * NB];
         #pragma unroll
         for (int j = 0; j < 2 * NB; j++) o[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -659,6 +723,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
         if (AHEAD) w.load_values(next, lane);
         else w.load_keys(next, lane);
         __builtin_amdgcn_sched_barrier(0);
+        if (small) lower_sums<NB>(o, times);
         #pragma unroll
         for (int j = 0; j < 2 * NB; j++)
           #pragma unroll
