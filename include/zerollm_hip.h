@@ -260,7 +260,8 @@ int zl_kv4_read(const zl_kv4 *c, const zl_batch *b, int type, const zl_rows *k, 
  * heads share a KV head; scale 0 means 1/sqrt(head_dim). A token at a negative position sees nothing: zeros. One at a
  * position past the capacity, or of a slot that does not exist: NaN. A row's bits depend on its query, its position and
  * the cache alone, not on the batch it comes in. q and out may be the same rows. work: zl_kv4_attention_work bytes of
- * device memory, contents of no matter before or after. */
+ * device memory, contents of no matter before or after: by the rows and the capacity, at most 2^29 (larger calls run in slabs
+ * that share them), or one token's where those are more: 8 (head_dim + 2) bytes a query head and 512 positions. */
 int zl_kv4_attention(const zl_kv4 *c, const zl_batch *b, int type, const zl_rows *q, int n_head, float scale, const zl_rows *out,
                      void *work, int64_t work_bytes, void *stream);
 int zl_kv4_attention_work(const zl_kv4 *c, int n_seq, int n_tok, int n_head, int64_t *bytes);

@@ -7,7 +7,9 @@ namespace zl {
 __device__ __forceinline__ uint8_t *record_of(const Kv4View &c, int slot, int head, long group) {
   return c.base + (((long)slot * c.nkv + head) * c.ngroup + group) * kv4_record(c.hd);
 }
-__device__ __forceinline__ int count_of(const OpBatch &b, int s) { return b.count ? max(0, min(b.count[s], b.ntok)) : b.ntok; }
+// The batch's tokens of sequence s, and the position of the first.
+__device__ __forceinline__ int count_of(const OpBatch &b, int s) { return b.count ? max(0, min(b.count[s], b.tok0 + b.ntok) - b.tok0) : b.ntok; }
+__device__ __forceinline__ long pos_of(const OpBatch &b, int s) { return (long)b.pos[s] + b.tok0; }
 __device__ __forceinline__ int slot_of(const OpBatch &b, int s) { return b.slot ? b.slot[s] : s; }
 
 // ---------------------------------------------------------------------------------------------- append
@@ -559,7 +561,7 @@ struct Tile {
     *tok = t;
     *head = kvh * group + i - t * group;
     if (t >= ntok) return ROW_ABSENT;
-    const long p = (long)a.b.pos[s] + t;
+    const long p = pos_of(a.b, s) + t;
     return !ok || p >= a.c.cap ? ROW_BAD : p < 0 ? ROW_NONE : (int)p;
   }
 };
@@ -579,10 +581,12 @@ struct ToRows {
   __device__ __forceinline__ void emit(int s, int tok, int head, int dim, float o) const {
     ((typename ValueOf<TYPE>::t *)r.p)[s * r.seq + tok * r.tok + head * r.head + dim] = store_value<TYPE>(o + 0.0f);
   }
+  void skip(int seqs) { r.p = (char *)r.p + seqs * r.seq * value_bytes(TYPE); }
 };
 struct ToModel {
   HeadOut h;
   __device__ __forceinline__ void emit(int, int tok, int head, int dim, float o) const { attn_emit(h, tok, head, dim, o + 0.0f); }
+  void skip(int) {}  // (one sequence)
 };
 
 // A span's products of block b and record: values times weights.
@@ -595,7 +599,7 @@ __device__ __forceinline__ void weighted_sums(f4 &o0, f4 &o1, h8 x0, h8 x1, h8 h
 
 // Positions per record of a sequence's rows (of k_kv4_rows<.., false>): by the sequence's last position, so that all its rows agree.
 __device__ __forceinline__ int record_len(const Kv4Attn &a, int s) {
-  const long last = min((long)a.b.pos[s] + count_of(a.b, s), a.c.cap) - 1;
+  const long last = min(pos_of(a.b, s) + count_of(a.b, s), a.c.cap) - 1;
   return last < (long)a.spanmax * SPAN ? SPAN : CHUNK;
 }
 
@@ -610,7 +614,7 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
     for (int j = 0; j < 2 * NB; j++)
       #pragma unroll
       for (int v = 0; v < 4; v++)
-        out.emit(tl.s, tok, head, 16 * j + 4 * g + v, last >= 0 ? f.o[4 * j + v] / f.l : last == ROW_NONE ? 0.0f : NAN);
+        out.emit(tl.s, a.b.tok0 + tok, head, 16 * j + 4 * g + v, last >= 0 ? f.o[4 * j + v] / f.l : last == ROW_NONE ? 0.0f : NAN);
     return;
   }
   if (last < first) return;
@@ -663,7 +667,7 @@ __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn
   Queries<NB> q;
   {
     float qv[NB][8];
-    fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? tok * a.q.tok + head * a.q.head : 0), a.qvec, lane);
+    fetch_queries<NB, TYPE>(qv, (const T *)a.q.p + tl.s * a.q.seq + (last >= 0 ? (a.b.tok0 + tok) * a.q.tok + head * a.q.head : 0), a.qvec, lane);
     const uint8_t *rec = record_of(a.c, tl.slot, tl.kvh, (long)c0 * (unit / KV4_GROUP));
     w.load_keys(rec, lane);
     if (AHEAD) w.load_values(rec, lane);
@@ -762,7 +766,7 @@ __device__ __forceinline__ int row_of(const Kv4Attn &a, long row, int *s, int *t
   *s = (int)(row / a.nhead / a.b.ntok);
   if (*tok >= count_of(a.b, *s)) return ROW_ABSENT;
   const int slot = slot_of(a.b, *s);
-  const long p = (long)a.b.pos[*s] + *tok;
+  const long p = pos_of(a.b, *s) + *tok;
   return slot < 0 || slot >= a.c.nslot || p >= a.c.cap ? ROW_BAD : p < 0 ? ROW_NONE : (int)p;
 }
 
@@ -784,7 +788,7 @@ __global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a
   const int last = row_of(a, blockIdx.x, &s, &tok, &head);
   if (last == ROW_ABSENT) return;
   if (last < 0) {
-    if (grp == 0) out.emit(s, tok, head, dim, last == ROW_NONE ? 0.0f : NAN);
+    if (grp == 0) out.emit(s, a.b.tok0 + tok, head, dim, last == ROW_NONE ? 0.0f : NAN);
     return;
   }
   const int len = record_len(a, s), nrec = last / len + 1;
@@ -873,7 +877,7 @@ __global__ __launch_bounds__(32 * GROUPS) void k_kv4_join_chunks(const Kv4Attn a
       f.fold(u);
     }
   }
-  if (grp == 0) out.emit(s, tok, head, dim, f.o[0] / f.l);
+  if (grp == 0) out.emit(s, a.b.tok0 + tok, head, dim, f.o[0] / f.l);
 }
 
 // Rows of part records, many of them: 32 lanes per row.
@@ -922,7 +926,7 @@ __global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a, const O
     f.fold(u[0]);
   }
   #pragma unroll
-  for (int i = 0; i < NB; i++) out.emit(s, tok, head, 32 * i + fl, last >= 0 ? f.o[i] / f.l : last == ROW_NONE ? 0.0f : NAN);
+  for (int i = 0; i < NB; i++) out.emit(s, a.b.tok0 + tok, head, 32 * i + fl, last >= 0 ? f.o[i] / f.l : last == ROW_NONE ? 0.0f : NAN);
 }
 
 // Tiles of 16 rows times KV heads times sequences.
@@ -941,24 +945,43 @@ static bool many_rows(const Kv4View &c, int nseq, int ntok, int nhead) {
 }
 // Spans of a sequence up to which its rows have a record per span: as many as give about two waves a SIMD.
 static int span_max(const Kv4View &c, long tiles) { return (int)std::min((c.cap + SPAN - 1) / SPAN, 2048 / tiles); }
-static int record_count(const Kv4View &c, int nseq, int ntok, int nhead) {
-  if (many_rows(c, nseq, ntok, nhead)) return (int)((c.cap + PART - 1) / PART);
-  return (int)std::max((c.cap + CHUNK - 1) / CHUNK, (long)span_max(c, tile_count(c, nseq, ntok, nhead)));
+// How a call is run: the records of a row, and slabs of `seqs` sequences and `toks` tokens one after the other in the same work space, so
+// that it stays below WORK_MOST bytes (one token's records apart), however long the prompt and large the cache are, and the
+// launches within 2^32 threads. A row has the same bits in any slab. (2048 tokens of 32 heads of 128 in a cache of 131072: 4.1 GB as
+// one, nine slabs of 240 tokens.)
+struct AttnPlan {
+  bool many;
+  int nrec, spanmax, seqs, toks;
+};
+constexpr long WORK_MOST = 1L << 29, BLOCKS_MOST = 1L << 22;
+static AttnPlan attn_plan(const Kv4View &c, int nseq, int ntok, int nhead) {
+  AttnPlan p;
+  p.many = many_rows(c, nseq, ntok, nhead);
+  p.spanmax = p.many ? 0 : span_max(c, tile_count(c, nseq, ntok, nhead));
+  p.nrec = p.many ? (int)((c.cap + PART - 1) / PART) : (int)std::max((c.cap + CHUNK - 1) / CHUNK, (long)p.spanmax);
+  const long token = (long)nhead * p.nrec * (c.hd + 2) * 4, fit = WORK_MOST / token;
+  p.seqs = nseq;
+  p.toks = ntok;
+  if (fit < ntok) {
+    p.seqs = 1;
+    p.toks = (int)(fit >= 16 ? fit / 16 * 16 : std::max(1L, fit));  // (whole tiles)
+  } else {
+    p.seqs = (int)std::min((long)nseq, fit / ntok);
+    const long blocks = tile_count(c, 1, ntok, nhead);  // of a sequence, at most
+    p.seqs = (int)std::max(1L, std::min((long)p.seqs, BLOCKS_MOST / blocks));
+  }
+  return p;
 }
 
 long kv4_attention_work(const Kv4View &c, int nseq, int ntok, int nhead) {
   if (nseq == 0 || ntok == 0) return 16;
-  return std::max(16L, (long)nseq * ntok * nhead * record_count(c, nseq, ntok, nhead) * (c.hd + 2) * 4);
+  const AttnPlan p = attn_plan(c, nseq, ntok, nhead);
+  return std::max(16L, (long)p.seqs * p.toks * nhead * p.nrec * (c.hd + 2) * 4);
 }
 
 template <int NB, int TYPE, class OUT>
-static void launch_attention_k(Kv4Attn a, const OUT &out, bool direct, hipStream_t st) {
-  const bool many = many_rows(a.c, a.b.nseq, a.b.ntok, a.nhead);
+static void launch_slab(const Kv4Attn &a, bool many, const OUT &out, hipStream_t st) {
   const int group = a.nhead / a.c.nkv;
-  a.nrec = record_count(a.c, a.b.nseq, a.b.ntok, a.nhead);
-  a.spanmax = many ? 0 : span_max(a.c, tile_count(a.c, a.b.nseq, a.b.ntok, a.nhead));
-  a.qvec = whole_pieces(a.q, TYPE);
-  a.direct = direct && a.nrec == 1;
   const long rows = (long)a.b.ntok * group;
   const int tiles = (int)((rows + 15) / 16);
   // waves up to two a SIMD (all on the GPU at once, whichever CUs the blocks are dealt to), each with an even share of the
@@ -980,6 +1003,34 @@ static void launch_attention_k(Kv4Attn a, const OUT &out, bool direct, hipStream
     else if (a.c.cap > 32 * PART) hipLaunchKernelGGL((k_kv4_join_chunks<32, OUT>), dim3((unsigned)n, NB), dim3(1024), 0, st, a, out);
     else hipLaunchKernelGGL((k_kv4_join_chunks<8, OUT>), dim3((unsigned)n, NB), dim3(256), 0, st, a, out);
     ZL_HIP(hipGetLastError());
+  }
+}
+
+template <int NB, int TYPE, class OUT>
+static void launch_attention_k(Kv4Attn a, OUT out, bool direct, hipStream_t st) {
+  const AttnPlan p = attn_plan(a.c, a.b.nseq, a.b.ntok, a.nhead);
+  a.nrec = p.nrec;
+  a.spanmax = p.spanmax;
+  a.qvec = whole_pieces(a.q, TYPE);
+  a.direct = direct && a.nrec == 1;
+  const OpBatch all = a.b;
+  for (int s = 0; s < all.nseq; s += p.seqs) {
+    a.b.nseq = std::min(p.seqs, all.nseq - s);
+    for (a.b.tok0 = 0; a.b.tok0 < all.ntok; a.b.tok0 += p.toks) {
+      a.b.ntok = std::min(p.toks, all.ntok - a.b.tok0);
+      launch_slab<NB, TYPE>(a, p.many, out, st);
+    }
+    a.b.pos += p.seqs;
+    if (a.b.count) a.b.count += p.seqs;
+    if (a.b.slot) {
+      a.b.slot += p.seqs;
+    } else {
+      a.c.base += (long)p.seqs * a.c.nkv * a.c.ngroup * kv4_record(a.c.hd);
+      a.c.nslot -= p.seqs;
+    }
+    a.q.p = (char *)a.q.p + p.seqs * a.q.seq * value_bytes(TYPE);
+    if (a.direct) a.out.p = (char *)a.out.p + p.seqs * a.out.seq * value_bytes(TYPE);
+    out.skip(p.seqs);
   }
 }
 

@@ -90,7 +90,11 @@ inline int64_t kv4_bytes(int nslot, int nkv, int hd, long cap) { return (int64_t
 
 // The batch and its rows (strides in values).
 struct OpRows { void *p; long seq, tok, head; };
-struct OpBatch { int nseq, ntok; const int *pos, *count, *slot; };
+struct OpBatch {
+  int nseq, ntok;
+  const int *pos, *count, *slot;
+  int tok0 = 0;  // attention: the tokens are tok0 .. tok0 + ntok - 1 of each sequence
+};
 
 void launch_kv4_append(const Kv4View &c, const OpBatch &b, int type, const OpRows &k, const OpRows &v, hipStream_t st);
 void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows &k, const OpRows &v, hipStream_t st);
@@ -103,7 +107,7 @@ struct Kv4Attn {
   float scale;
   void *work;
   // set by the launcher: records per row in work, spans of a sequence up to which they are spans', whether the queries are whole
-  // 16-byte pieces
+  // 16-byte pieces; b is a slab of the call
   int nrec, spanmax;
   bool qvec, direct;  // direct: no records, a row's only ones are its output
 };
