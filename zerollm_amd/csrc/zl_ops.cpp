@@ -41,7 +41,7 @@ static void need_type(const char *f, int type) {
   ZL_REQUIRE(value_bytes(type) > 0, ZL_ERR_UNSUPPORTED, std::string(f) + ": values must be F32, F16 or BF16 (got type " + std::to_string(type) + ")");
 }
 
-constexpr int64_t MOST_ROWS = 1 << 26;  // tokens or query rows of a call: grids of a few lanes for each stay within 2^32
+constexpr int64_t MOST_ROWS = 1 << 26;  // tokens or query rows of a call: the launchers keep their grids within 2^32 threads up to here
 
 // The batch; heads and sequences are grid dimensions of at most 65535. Returns whether there is anything to do.
 static bool take_batch(const char *f, const zl_batch *b, OpBatch *o) {

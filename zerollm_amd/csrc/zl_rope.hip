@@ -141,7 +141,8 @@ static void launch_rope_k(const RopeArgs &a, hipStream_t st) {
   const long all = (long)a.b.ntok * a.b.nseq * heads * pieces;
   const long per = std::max(256L, std::min(4096L, all / 512));  // pieces per block
   const int hb = (int)std::max(1L, std::min((long)heads, per / pieces));
-  const int tb = (int)std::max(1L, std::min({(long)a.b.ntok, per / ((long)hb * pieces), 16L}));
+  // (at least the tokens that keep the grid's first dimension below 2^32 threads: up to 8 of the 2^26 a call may have)
+  const int tb = (int)std::max({1L, std::min({(long)a.b.ntok, per / ((long)hb * pieces), 16L}), ((long)a.b.ntok + (1 << 23) - 1) >> 23});
   const dim3 grid((unsigned)((a.b.ntok + tb - 1) / tb), a.b.nseq, (heads + hb - 1) / hb);
   hipLaunchKernelGGL((k_rope<TYPE, HALF, WHOLE>), grid, dim3(256), (size_t)tb * a.half * sizeof(float2), st, a, tb, hb);
   ZL_HIP(hipGetLastError());
