@@ -1,0 +1,39 @@
+"""What the Python calls of the long-context operators refuse, on tensors in host memory that stand for the GPU's."""
+import pytest
+import torch
+
+from zerollm_amd import _lib, ops
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Host tensors pass for tensors on the library's GPU; a call that would reach the library fails the test."""
+    monkeypatch.setattr(_lib, "DEVICE", -1)
+
+    def reached(name, *a):
+        raise AssertionError(f"{name} was called")
+
+    monkeypatch.setattr(ops, "call", reached)
+
+
+def bare(cls, **kw):
+    x = object.__new__(cls)
+    x.__dict__.update(closed=True, **kw)  # (nothing to free)
+    return x
+
+
+def test_tensors_that_require_gradients(host):
+    q = torch.zeros((1, 2, 4, 64), requires_grad=True)
+    plain, pos = torch.zeros((1, 2, 4, 64)), torch.zeros(1, dtype=torch.int32)
+    c = bare(ops.KVCacheQ4, n_head_kv=4, head_dim=64)
+    r = bare(ops.Rope)
+    r.closed = False
+    for call, name in ((lambda: c.attend(q, pos), "q"), (lambda: c.attend(plain, pos, out=q), "out"), (lambda: c.append(q, plain, pos), "k"),
+                       (lambda: c.append(plain, q, pos), "v"), (lambda: r.apply(q, None, pos), "q"), (lambda: r.apply(plain, q * 2, pos), "k"),
+                       (lambda: ops.logprobs(q[0, 0]), "logits")):
+        with pytest.raises(ValueError, match=f"^{name} requires a gradient"):
+            call()
+    with torch.no_grad():
+        assert ops._rows(q, "q")[2] == (1, 2, 4, 64)
+    assert ops._rows(q.detach(), "q")[2] == (1, 2, 4, 64)
+    r.closed = True

@@ -5,8 +5,9 @@ Tensors are torch's (this module imports no torch of its own: it takes any tenso
 GPU, float32, float16 or bfloat16, with any strides as long as the values of a head (of a logits row) are contiguous. Rows of
 several sequences are [sequence, token, head, dim], or [sequence, head, dim] for one token each. Positions, counts and slots
 are int32 tensors on the GPU, one entry per sequence, read when the work runs. Calls are enqueued on torch's current stream
-and return at once; with `out` and `work` given they allocate nothing and may be captured into a graph. Wrong shapes, types or
-places raise ValueError, what the library refuses ZLError.
+and return at once; with `out` and `work` given they allocate nothing and may be captured into a graph. They have no gradients: a
+tensor that requires one is refused while gradients are recorded. Wrong shapes, types or places raise ValueError, what the library
+refuses ZLError.
 """
 from __future__ import annotations
 
@@ -46,6 +47,11 @@ def _type(x, name):
     return t
 
 
+def _no_gradient(x, name):
+    if x.requires_grad and _torch().is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which these operators do not give: detach it, or call under torch.no_grad()")
+
+
 def _ints(x, n, name):
     if x is None:
         return None
@@ -58,6 +64,7 @@ def _ints(x, n, name):
 def _rows(x, name, shape=None, type_=None, written=False):
     """(zl_rows, type, shape as (sequence, token, head, dim)) of a tensor."""
     t = _type(x, name)
+    _no_gradient(x, name)
     s = tuple(x.shape)
     if len(s) == 4:
         a, b, c, d = x.stride()
@@ -269,6 +276,7 @@ def logprobs(logits, tokens=None, top: int = 0, out=None, work=None) -> LogProbs
     """LogProbs of logits rows [rows, vocab] (any row stride). tokens: int32 [rows]; an id outside the vocabulary gives NaN.
     top: 0 to 64 alternatives. Logits of -inf have probability 0; a row with NaN or +inf, or with nothing above -inf, is NaN."""
     t = _type(logits, "logits")
+    _no_gradient(logits, "logits")
     if len(logits.shape) != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
