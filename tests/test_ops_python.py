@@ -37,3 +37,13 @@ def test_tensors_that_require_gradients(host):
         assert ops._rows(q, "q")[2] == (1, 2, 4, 64)
     assert ops._rows(q.detach(), "q")[2] == (1, 2, 4, 64)
     r.closed = True
+
+
+def test_position_scaling_of_models_says_which():
+    from zerollm_amd import model
+    for kw in (dict(factor=4.0), dict(scaling=None, factor=4.0, orig_ctx=32768), dict(attn_factor=1.0)):
+        with pytest.raises(ValueError, match="rope needs a scaling"):
+            model.HipModel.load("none.gguf", rope=kw)
+    assert model._ext("f16", dict(scaling="linear", factor=4.0)).rope.contents.factor == 4.0
+    assert model._ext("f16", dict(scaling="none", factor=4.0)).rope.contents.scaling == 0
+    assert model._ext("q4_0", dict()).kv_q4 == 1 and model._ext("f16", None) is None

@@ -42,6 +42,8 @@ def _ext(kv, rope):
     if rope is not None:
         if unknown := set(rope) - {"scaling", "factor", "orig_ctx", "beta_fast", "beta_slow", "attn_factor"}:
             raise ValueError(f"rope does not take {', '.join(sorted(unknown))}: a model has its own")
+        if rope.get("scaling") is None and any(v is not None for v in rope.values()):
+            raise ValueError('rope needs a scaling ("linear", "yarn", or "none" to leave the rest unused)')
         e._rope = rope_opts(**rope)
         e.rope = C.pointer(e._rope)
     return e
