@@ -47,3 +47,12 @@ def test_position_scaling_of_models_says_which():
     assert model._ext("f16", dict(scaling="linear", factor=4.0)).rope.contents.factor == 4.0
     assert model._ext("f16", dict(scaling="none", factor=4.0)).rope.contents.scaling == 0
     assert model._ext("q4_0", dict()).kv_q4 == 1 and model._ext("f16", None) is None
+
+
+def test_scales_that_float32_rounds_to_nothing(host):
+    """0 means 1 / sqrt(head_dim) to the library."""
+    q, pos = torch.zeros((1, 2, 4, 64)), torch.zeros(1, dtype=torch.int32)
+    c = bare(ops.KVCacheQ4, n_head_kv=4, head_dim=64)
+    for scale in (1e-50, 0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="scale must be positive"):
+            c.attend(q, pos, scale=scale)

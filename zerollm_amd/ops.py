@@ -164,8 +164,8 @@ class KVCacheQ4:
         qr, t, s = _rows(q, "q")
         if s[3] != self.head_dim:
             raise ValueError(f"q must have heads of {self.head_dim} values (got {s[3]})")
-        if scale is not None and not scale > 0:
-            raise ValueError(f"scale must be positive (got {scale})")
+        if scale is not None and not (scale > 0 and C.c_float(scale).value > 0):
+            raise ValueError(f"scale must be positive in float32 (got {scale})")
         b = _batch(s[0], s[1], pos, count, slot)
         if out is None:
             out = _torch().empty(tuple(q.shape), dtype=q.dtype, device=q.device)
