@@ -1,4 +1,6 @@
 """What the Python calls of the long-context operators refuse, on tensors in host memory that stand for the GPU's."""
+import gc
+
 import pytest
 import torch
 
@@ -18,7 +20,7 @@ def host(monkeypatch):
 
 def bare(cls, **kw):
     x = object.__new__(cls)
-    x.__dict__.update(closed=True, **kw)  # (nothing to free)
+    x.__dict__.update(closed=True, _h=None, **kw)  # (nothing to free)
     return x
 
 
@@ -56,3 +58,32 @@ def test_scales_that_float32_rounds_to_nothing(host):
     for scale in (1e-50, 0.0, -1.0, float("nan")):
         with pytest.raises(ValueError, match="scale must be positive"):
             c.attend(q, pos, scale=scale)
+
+
+def test_handles_that_come_and_go_while_a_graph_is_captured(monkeypatch):
+    """Nothing is allocated or freed then: making and closing one is refused, one that is collected is freed later."""
+    done, capturing = [], [False]
+    monkeypatch.setattr(ops, "call", lambda name, *a: done.append(name))
+    monkeypatch.setattr(ops, "_capturing", lambda: capturing[0])
+    r, c = ops.Rope(64), ops.KVCacheQ4(1, 2, 64, 100)
+    assert done == ["zl_rope_create", "zl_kv4_create"]
+    done.clear()
+    capturing[0] = True
+    for bad in (lambda: ops.Rope(64), lambda: ops.KVCacheQ4(1, 2, 64, 100), r.close, c.close):
+        with pytest.raises(_lib.ZLError, match="a graph is being captured"):
+            bad()
+    del r
+    gc.collect()
+    assert done == [] and not c.closed
+    capturing[0] = False
+    c.close()
+    c.close()
+    assert done == ["zl_kv4_free"]
+    with pytest.raises(_lib.ZLError, match="cache is closed"):
+        c.work_bytes(1, 1, 2)
+    done.clear()
+    r = ops.Rope(64)
+    assert done == ["zl_rope_free", "zl_rope_create"]
+    del r
+    gc.collect()
+    assert done[2:] == ["zl_rope_free"]

@@ -112,15 +112,66 @@ def _work(work, nbytes, like):
     return work
 
 
-class KVCacheQ4:
+def _capturing():
+    t = sys.modules.get("torch")
+    return t is not None and t.cuda.is_initialized() and t.cuda.is_current_stream_capturing()
+
+
+class _Handle:
+    """An object of the library's. Making and freeing one allocates and waits for the GPU, which would break a graph that is being
+    captured on the current stream: refused there; an object that goes in the meantime (a garbage collection) is freed later, when
+    the next one is made or goes."""
+
+    _gone = []  # of those: (entry point, handle)
+
+    def _make(self, name, *args):
+        if _capturing():
+            raise _lib.ZLError(5, f"{name}: a graph is being captured")
+        self._free_later()
+        self._h = C.c_void_p()
+        call(name, *args, C.byref(self._h))
+        self.closed = False
+
+    def _handle(self):
+        if self.closed:
+            raise _lib.ZLError(5, f"{self._what} is closed")
+        return self._h
+
+    @classmethod
+    def _free_later(cls):
+        while cls._gone:
+            call(*cls._gone.pop())
+
+    def close(self):
+        """Release it once the GPU is done with it (idempotent)."""
+        if self.closed:
+            return
+        if _capturing():
+            raise _lib.ZLError(5, f"{self._free}: a graph is being captured")
+        self.closed = True
+        call(self._free, self._h)
+
+    def __del__(self):
+        try:
+            if not _capturing():
+                self.close()
+                self._free_later()
+            elif not self.closed:
+                self.closed = True
+                self._gone.append((self._free, self._h))
+        except Exception:
+            pass
+
+
+class KVCacheQ4(_Handle):
     """A KV cache of n_slot sequences of up to `capacity` positions, held as Q4_0 blocks: 1.125 bytes per (position, KV head,
     dimension) for key and value together, where float16 takes 4."""
 
+    _what, _free, closed = "cache", "zl_kv4_free", True
+
     def __init__(self, n_slot: int, n_head_kv: int, head_dim: int, capacity: int):
-        self._h = C.c_void_p()
-        call("zl_kv4_create", int(n_slot), int(n_head_kv), int(head_dim), int(capacity), C.byref(self._h))
+        self._make("zl_kv4_create", int(n_slot), int(n_head_kv), int(head_dim), int(capacity))
         self.n_slot, self.n_head_kv, self.head_dim, self.capacity = int(n_slot), int(n_head_kv), int(head_dim), int(capacity)
-        self.closed = False
         self._sized = None, 0  # the last queries' shape and its work space
 
     @property
@@ -128,11 +179,6 @@ class KVCacheQ4:
         n = C.c_int64()
         call("zl_kv4_bytes", self._handle(), C.byref(n))
         return n.value
-
-    def _handle(self):
-        if self.closed:
-            raise _lib.ZLError(5, "cache is closed")
-        return self._h
 
     def _kv(self, k, v, written):
         kr, t, s = _rows(k, "k", written=written)
@@ -177,18 +223,6 @@ class KVCacheQ4:
         call("zl_kv4_attention", self._handle(), b, t, qr, s[2], scale or 0.0, o, w.data_ptr(), w.numel() * w.element_size(), _stream())
         return out
 
-    def close(self):
-        """Release the cache once the GPU is done with it (idempotent)."""
-        if not self.closed:
-            self.closed = True
-            call("zl_kv4_free", self._h)
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
-
 
 SCALINGS = {None: 0, "none": 0, "linear": 1, "yarn": 2}
 
@@ -211,25 +245,24 @@ def rope_opts(n_rot=0, neox=True, base=10000.0, scaling=None, factor=1.0, orig_c
     return o
 
 
-class Rope:
+class Rope(_Handle):
     """Rotary positions of the first n_rot values of a head: pairs (i, i + n_rot/2) (neox) or (2i, 2i + 1), by
     pos * base^(-2i/n_rot) / freq_factors[i] radians. scaling "linear": angles divided by factor; "yarn": by parts, between
     pairs that turn beta_fast (32) and beta_slow (1) times within orig_ctx positions, and everything times attn_factor
     (0.1 ln factor + 1)."""
 
+    _what, _free, closed = "rope", "zl_rope_free", True
+
     def __init__(self, n_rot, neox=True, base=10000.0, scaling=None, factor=1.0, orig_ctx=0, beta_fast=0.0, beta_slow=0.0,
                  attn_factor=0.0, freq_factors=None):
         o = rope_opts(n_rot, neox, base, scaling, factor, orig_ctx, beta_fast, beta_slow, attn_factor, freq_factors)
-        self._h = C.c_void_p()
-        call("zl_rope_create", C.byref(o), C.byref(self._h))
+        self._make("zl_rope_create", C.byref(o))
         self.n_rot = int(n_rot)
-        self.closed = False
 
     def apply(self, q, k, pos, count=None, out=None):
         """q and k (or None) rotated to positions pos[s], pos[s] + 1, ... of each sequence, in one launch. out: (q', k'), which
         may be q and k themselves; new tensors without it. Returns (q', k')."""
-        if self.closed:
-            raise _lib.ZLError(5, "rope is closed")
+        handle = self._handle()
         qr, t, s = _rows(q, "q")
         if out is None:
             out = tuple(None if x is None else _torch().empty(tuple(x.shape), dtype=x.dtype, device=x.device) for x in (q, k))
@@ -240,20 +273,8 @@ class Rope:
             nk = k.shape[-2] if len(k.shape) >= 3 else 0
             ks = (s[0], s[1], nk, s[3])
             kr, ko = _rows(k, "k", ks, t)[0], _rows(out[1], "out[1]", ks, t, True)[0]
-        call("zl_rope_apply", self._h, _batch(s[0], s[1], pos, count), t, s[3], qr, qo, s[2], kr, ko, nk, _stream())
+        call("zl_rope_apply", handle, _batch(s[0], s[1], pos, count), t, s[3], qr, qo, s[2], kr, ko, nk, _stream())
         return out
-
-    def close(self):
-        """Release the tables once the GPU is done with them (idempotent)."""
-        if not self.closed:
-            self.closed = True
-            call("zl_rope_free", self._h)
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
 
 
 @dataclass
