@@ -20,7 +20,7 @@ def host(monkeypatch):
 
 def bare(cls, **kw):
     x = object.__new__(cls)
-    x.__dict__.update(closed=True, _h=None, **kw)  # (nothing to free)
+    x.__dict__.update(closed=True, _h=None, _device=-1, **kw)  # (nothing to free)
     return x
 
 
@@ -87,3 +87,18 @@ def test_handles_that_come_and_go_while_a_graph_is_captured(monkeypatch):
     del r
     gc.collect()
     assert done[2:] == ["zl_rope_free"]
+
+
+def test_handles_of_another_gpu(monkeypatch):
+    """model.init of another GPU moves the calls' tensors and streams there."""
+    monkeypatch.setattr(ops, "call", lambda name, *a: None)
+    r, c = ops.Rope(64), ops.KVCacheQ4(1, 2, 64, 100)
+    c.work_bytes(1, 1, 2)
+    q, pos = torch.zeros((1, 2, 2, 64)), torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setattr(_lib, "DEVICE", -1)  # (host tensors stand for that GPU's)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    for bad in (lambda: c.attend(q, pos), lambda: c.append(q, q, pos), lambda: c.read(q, q, pos), lambda: c.work_bytes(1, 1, 2), lambda: r.apply(q, None, pos)):
+        with pytest.raises(_lib.ZLError, match="is on GPU 0, the library on GPU -1"):
+            bad()
+    c.close()
+    r.close()

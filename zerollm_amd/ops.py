@@ -130,11 +130,13 @@ class _Handle:
         self._free_later()
         self._h = C.c_void_p()
         call(name, *args, C.byref(self._h))
-        self.closed = False
+        self.closed, self._device = False, _lib.DEVICE
 
     def _handle(self):
         if self.closed:
             raise _lib.ZLError(5, f"{self._what} is closed")
+        if self._device != _lib.DEVICE:  # (its memory is there, the call's tensors and stream here)
+            raise _lib.ZLError(5, f"{self._what} is on GPU {self._device}, the library on GPU {_lib.DEVICE} by now")
         return self._h
 
     @classmethod
