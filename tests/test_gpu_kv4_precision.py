@@ -107,3 +107,25 @@ def test_small_values_keep_their_bits(gpu, dim, tokens, group, magnitude, t):
         worst = max(worst, (np.abs(got[:, h] - want) / off).max())
     print(f"worst error / bound {worst:.3f}", flush=True)
     c.close()
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("dim,kv,group,tokens", [(64, 2, 4, 40), (128, 8, 4, 300), (256, 1, 2, 70)])
+def test_small_values_have_the_same_bits_in_every_batch(gpu, dim, kv, group, tokens, t):
+    """Rows of one tile that see, in the same span, small values alone and a large one among them; blocks of either kind side by side."""
+    n = 700
+    c = cache(1, kv, dim, n)
+    k, v = rows(21, (1, n, kv, dim)), rows(22, (1, n, kv, dim)) * 1e-4
+    for p in (n - tokens + 5, n - 30, n - 3):
+        v[:, p, :, 32:64] *= 1e4
+    v[..., :16] *= 0.01
+    c.append(k, v, ints(0))
+    q = rows(23, (1, tokens, kv * group, dim)).to(TYPES[t])
+    print(f"case small bits dim {dim} {t}", flush=True)
+    got = c.attend(q, ints(n - tokens))
+    assert torch.isfinite(got).all() and (got != 0).any()
+    for m in (1, 3, 16):
+        for j in (0, 4, 5, 6, tokens - 31, tokens - 29, tokens - m):
+            m = min(m, tokens - j)
+            assert (c.attend(q[:, j:j + m], ints(n - tokens + j)) == got[:, j:j + m]).all(), (m, j)
+    c.close()
