@@ -14,8 +14,10 @@ __device__ __forceinline__ int slot_of(const OpBatch &b, int s) { return b.slot 
 
 // ---------------------------------------------------------------------------------------------- append
 // One block per (32-position record that a sequence may touch, KV head, sequence). A lane takes 8 values, four lanes a block
-// of 32 (kv4_quant). The codes go to LDS and from there in whole words: a key word is one lane's 8 values; a value word holds 8 positions, and those that are not appended
-// keep their codes. The block of the first sequence that touches a record of a slot takes all of them, in order.
+// of 32 (kv4_quant). The codes go to LDS and from there in whole words: a key word is one lane's 8 values; a value word holds 8
+// positions, and those that are not appended keep their codes. With slots, the block of the first sequence that touches a record of
+// its slot takes all of them, in order, found 256 at a time (one by one, 4096 sequences of 8 heads took 17 ms for 0.4, and their square
+// beyond).
 // Bound by the loads' latency: all of a record's are requested together (2048 tokens of 8 heads of 128, bf16: 37 us with a
 // value per lane and a load at a time).
 template <int TYPE, bool VEC>
@@ -34,6 +36,10 @@ __device__ __forceinline__ void load8(const typename ValueOf<TYPE>::t *p, float 
     #pragma unroll
     for (int e = 0; e < 8; e++) x[e] = load_value<TYPE>(p[e]);
   }
+}
+
+__device__ __forceinline__ unsigned long long uniform(unsigned long long x) {
+  return (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
 }
 
 template <int NB, int TYPE, bool VEC>
@@ -55,60 +61,70 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4View c, const OpBat
   };
   long p0, p1;
   if (!touches(s0, &p0, &p1)) return;
-  if (b.slot)
-    for (int s = 0; s < s0; s++) {
-      long x, y;
-      if (b.slot[s] == slot && touches(s, &x, &y)) return;
-    }
   uint8_t *rec = record_of(c, slot, head, g);
-  for (int s = s0; s < (b.slot ? b.nseq : s0 + 1); s++) {
-    if (s != s0 && (b.slot[s] != slot || !touches(s, &p0, &p1))) continue;
-    const int n = (int)(p1 - p0), q0 = (int)(p0 - g * KV4_GROUP);
-    const long t0 = p0 - b.pos[s];
-    float x[2][UNITS][8];
-    #pragma unroll
-    for (int isv = 0; isv < 2; isv++)
-      #pragma unroll
-      for (int u = 0; u < UNITS; u++) {
-        const int i = u * 256 + tid, t = i / (4 * NB), d8 = i % (4 * NB);
-        const OpRows &r = isv ? v : k;
-        if (t < n) load8<TYPE, VEC>((const T *)r.p + s * r.seq + (t0 + t) * r.tok + head * r.head + 8 * d8, x[isv][u]);
-      }
-    #pragma unroll
-    for (int isv = 0; isv < 2; isv++)
-      #pragma unroll
-      for (int u = 0; u < UNITS; u++) {
-        const int i = u * 256 + tid, t = i / (4 * NB), d8 = i % (4 * NB), p = q0 + t;
-        if (t >= n) continue;  // (four lanes of a block of 32 go together)
-        int code[8];
-        const uint16_t scale = kv4_quant(x[isv][u], tid, code);
-        if ((tid & 3) == 0) ((uint16_t *)(rec + (isv ? 34 : 32) * HD))[kv4_scale(p, d8 >> 2, NB)] = scale;
-        uint64_t bytes = 0;
-        #pragma unroll
-        for (int e = 0; e < 8; e++) bytes |= (uint64_t)code[e] << (8 * e);
-        if (isv) vn[p][d8] = bytes;
-        else kw[kv4_word((p >> 4) * NB + (d8 >> 2), (p & 15) + 16 * (d8 & 3))] = kv4_pack(code);
-      }
-    __syncthreads();
-    uint32_t *kd = (uint32_t *)rec, *vd = (uint32_t *)(rec + 16 * HD);
-    #pragma unroll
-    for (int u = 0; u < 4 * HD / 256; u++) {
-      const int i = u * 256 + tid, lane = i >> 2 & 63, w4 = (i >> 8) * 4 + (i & 3);  // dword i of the words
-      const int p = (lane & 15) + 16 * (w4 / NB);
-      if (p >= q0 && p < q0 + n) kd[i] = kw[i];
-      const int dim = 16 * w4 + (lane & 15), gq = lane >> 4;
-      uint32_t w = 0, m = 0;
-      #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int q = 16 * (e >> 2) + 4 * gq + (e & 3);
-        if (q >= q0 && q < q0 + n) {
-          w |= (uint32_t)((const uint8_t *)vn[q])[dim] << (4 * kv4_nibble(e));
-          m |= 0xfu << (4 * kv4_nibble(e));
-        }
-      }
-      if (m) vd[i] = m == 0xffffffffu ? w : (vd[i] & ~m) | w;
+  // with slots: the sequences of the slot that touch the record, 256 at a time; one before s0 has a block that takes them all
+  __shared__ unsigned long long same[4];
+  for (int base = b.slot ? 0 : s0; base < (b.slot ? b.nseq : s0 + 1); base += 256) {
+    if (b.slot) {
+      const int s = base + tid;
+      long x, y;
+      const unsigned long long m = __ballot(s < b.nseq && b.slot[s] == slot && touches(s, &x, &y));
+      if ((tid & 63) == 0) same[tid >> 6] = m;
+      __syncthreads();
     }
-    __syncthreads();
+    for (int sw = 0; sw < (b.slot ? 4 : 1); sw++)
+      for (unsigned long long left = b.slot ? uniform(same[sw]) : 1; left; left &= left - 1) {
+        const int s = base + 64 * sw + __ffsll(left) - 1;
+        if (s < s0) return;
+        touches(s, &p0, &p1);
+        const int n = (int)(p1 - p0), q0 = (int)(p0 - g * KV4_GROUP);
+        const long t0 = p0 - b.pos[s];
+        float x[2][UNITS][8];
+        #pragma unroll
+        for (int isv = 0; isv < 2; isv++)
+          #pragma unroll
+          for (int u = 0; u < UNITS; u++) {
+            const int i = u * 256 + tid, t = i / (4 * NB), d8 = i % (4 * NB);
+            const OpRows &r = isv ? v : k;
+            if (t < n) load8<TYPE, VEC>((const T *)r.p + s * r.seq + (t0 + t) * r.tok + head * r.head + 8 * d8, x[isv][u]);
+          }
+        #pragma unroll
+        for (int isv = 0; isv < 2; isv++)
+          #pragma unroll
+          for (int u = 0; u < UNITS; u++) {
+            const int i = u * 256 + tid, t = i / (4 * NB), d8 = i % (4 * NB), p = q0 + t;
+            if (t >= n) continue;  // (four lanes of a block of 32 go together)
+            int code[8];
+            const uint16_t scale = kv4_quant(x[isv][u], tid, code);
+            if ((tid & 3) == 0) ((uint16_t *)(rec + (isv ? 34 : 32) * HD))[kv4_scale(p, d8 >> 2, NB)] = scale;
+            uint64_t bytes = 0;
+            #pragma unroll
+            for (int e = 0; e < 8; e++) bytes |= (uint64_t)code[e] << (8 * e);
+            if (isv) vn[p][d8] = bytes;
+            else kw[kv4_word((p >> 4) * NB + (d8 >> 2), (p & 15) + 16 * (d8 & 3))] = kv4_pack(code);
+          }
+        __syncthreads();
+        uint32_t *kd = (uint32_t *)rec, *vd = (uint32_t *)(rec + 16 * HD);
+        #pragma unroll
+        for (int u = 0; u < 4 * HD / 256; u++) {
+          const int i = u * 256 + tid, lane = i >> 2 & 63, w4 = (i >> 8) * 4 + (i & 3);  // dword i of the words
+          const int p = (lane & 15) + 16 * (w4 / NB);
+          if (p >= q0 && p < q0 + n) kd[i] = kw[i];
+          const int dim = 16 * w4 + (lane & 15), gq = lane >> 4;
+          uint32_t w = 0, m = 0;
+          #pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const int q = 16 * (e >> 2) + 4 * gq + (e & 3);
+            if (q >= q0 && q < q0 + n) {
+              w |= (uint32_t)((const uint8_t *)vn[q])[dim] << (4 * kv4_nibble(e));
+              m |= 0xfu << (4 * kv4_nibble(e));
+            }
+          }
+          if (m) vd[i] = m == 0xffffffffu ? w : (vd[i] & ~m) | w;
+        }
+        __syncthreads();
+      }
+    if (b.slot) __syncthreads();
   }
 }
 
