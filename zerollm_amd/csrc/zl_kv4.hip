@@ -228,7 +228,8 @@ void launch_kv4_read(const Kv4View &c, const OpBatch &b, int type, const OpRows 
 // which takes those positions as they lie. Codes less 8 are exact in f16. Queries are scaled per row by a power of two to
 // below 2^14 and split into two f16 parts (22 bits; 16-bit queries need one); a weight times its value's scale likewise, whatever the
 // output's type: rounded to one f16 part, and the product again, it would be off by 2^-11 twice, more than an f16 output's own
-// rounding, and one bf16 output in eight or so would be another number than the rounded f32 one. Scores are scaled by their key's scale in f32, block by block.
+// rounding, and 7 to 9 % of bf16 outputs would be other numbers than the rounded f32 ones. Scores are scaled by their key's scale in
+// f32, block by block.
 constexpr int SPAN = 64, CHUNK = 256, PART = 1024;
 constexpr int CHUNKS = PART / CHUNK;
 
@@ -442,9 +443,10 @@ __device__ __forceinline__ void mask_scales(u4 (&vs)[NB], int i, int lim, int g)
 }
 
 // Value scales d of a block that are all below 2^-5: a weight times such a scale would end, in two f16 parts, at 2^-25 of the
-// weights' 8, 2^-23 of itself and less. Where a span's largest one is, for the lane's row, they are taken times 2^15, twice if that
-// leaves them there (denormals), which is exact, and the block's sums times the same less. By the row and the span's positions alone, so that a
-// row's bits do not depend on the batch. Returns two bits a block, the times.
+// weights' 8, few bits below that (values of 1e-5 made outputs 4e-3 off). Where a span's largest one that the lane's row sees is below, they
+// are taken times 2^15, twice if that leaves them there (denormals), which is exact, and the block's sums times the same less. It goes by
+// the row and the span's positions alone, so that a row's bits do not depend on the batch. Returns two bits a block, the times. The look
+// costs 2 to 3 % of a call, the raising 17 to 25 % (256 tokens after 12000 positions, f16: 197 us, values of 0.05 242).
 constexpr uint32_t SMALL_SCALE = 0x2800;  // 2^-5 in f16
 // Whether a block of the span may be such a one for any row that sees the span: none is where every lane has a scale of 2^-5 or more
 // among its four positions of tile 0 of record 0, in every block. The rest is left out then, which changes no bit.
@@ -648,11 +650,13 @@ __device__ __forceinline__ void leave(const Kv4Attn &a, const Tile &tl, int last
 // 256 tokens after 12000 positions 240 us against 189, as both were then.)
 // Few rows: sequences of so few spans that a wave for each does not overfill the GPU (a.spanmax, by the call's tiles) leave a record
 // per span instead: four times the waves, each a quarter as long (a token after 700 positions 13 us -> 8). A token of 32 heads of
-// 128 over 8 KV heads after 131000 positions: 41 us, 151 MB at 3.7 TB/s, near a read's own rate (4.1). 9 tokens after 16384: 26 us,
+// 128 over 8 KV heads after 131000 positions: 43 us, 151 MB at 3.5 TB/s, near a read's own rate (4.1). 9 tokens after 16384: 26 us,
 // bound by the vector units, 1.5 waves a SIMD, and by the waves' start and end.
 // MANY: the block's waves have neighbouring tiles of the same part, whose records they read at about the same time. 256 tokens of 32
-// heads over 8 after 12000 positions, f16: 150 us in a stream of calls, bound by the vector units: some 620 vector instructions and 48
-// matrix ones a span of a tile, 3400 cycles of a SIMD, with two waves to hide the matrix instructions' latency.
+// heads over 8 after 12000 positions, f16: 188 us, bound by the vector units: some 710 vector instructions and 48 matrix ones a span of
+// a tile, with two waves to hide the matrix instructions' latency.
+// Registers: heads of 64 take 173 to 187 VGPRs, heads of 128 all 256 (f32 rows spill 2 to 6 of them, 12 to 28 bytes a lane, outside the
+// loop over spans), heads of 256 also 115 to 150 AGPRs, which leaves them one wave a SIMD.
 template <int NB, int TYPE, bool MANY>
 __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void k_kv4_rows(const Kv4Attn a, int tiles, int gx) {
   constexpr int HD = 32 * NB;
@@ -948,13 +952,18 @@ __global__ __launch_bounds__(256) void k_kv4_join_parts(const Kv4Attn a, const O
 // Tiles of 16 rows times KV heads times sequences.
 static long tile_count(const Kv4View &c, int nseq, int ntok, int nhead) { return ((long)ntok * (nhead / c.nkv) + 15) / 16 * c.nkv * nseq; }
 // Whether a call takes a wave per (tile, part): where they fill the GPU's SIMDs, and there are enough rows that the records of chunks
-// would cost more than the longer runs. (f16 queries of 32 heads over 8, us, records of chunks : of parts, 16 tokens a call = 32 tiles:
+// would cost more than the longer runs. (f16 queries of one sequence, 32 heads over 8, us, records of chunks : of parts, 16 tokens a
+// call = 32 tiles:
 //   after    16 tokens  32        48        64        128       256
-//   1000     23 : 40    31 : 40   41 : 40   41 : 40   58 : 42   95 : 43
-//   4000     29 : 40    36 : 41   41 : 42   45 : 42   76 : 65   136 : 80
-//   16000    34 : 46    52 : 47   82 : 69   87 : 70   158 : 121 316 : 216
-//   60000    109 : 81   205 : 131 337 : 178 416 : 227 857 : 418 1693 : 778.) The cache's capacity stands for the length, which the
+//   1000     21 : 40    30 : 42   38 : 42   42 : 42   57 : 43   98 : 46
+//   4000     28 : 42    36 : 43   41 : 44   47 : 44   78 : 68   141 : 84
+//   16000    34 : 48    54 : 51   86 : 72   91 : 74   165 : 133 337 : 241
+//   60000    112 : 86   212 : 139 349 : 192 422 : 245 872 : 455 1744 : 841.) The cache's capacity stands for the length, which the
 // host does not know; with fewer tiles a short sequence in a large cache would lose more than a long one gains.
+// Batches of single tokens are not told apart, and mostly lose by parts: a block's four waves take four tiles of one (sequence, KV
+// head), so that three of them have nothing to do. (The same heads, 4 / 8 / 16 / 32 / 64 sequences, chunks : parts after 500: 14 : 23,
+// 14 : 23, 17 : 23, 24 : 23, 38 : 25; after 4000 20 : 44, 29 : 44, 32 : 46, 53 : 69, 92 : 89; after 16000 29 : 50, 45 : 73, 78 : 119,
+// 143 : 220, 270 : 428; parts from 16 sequences on, and from 4 in caches of 32768.)
 static bool many_rows(const Kv4View &c, int nseq, int ntok, int nhead) {
   const long tiles = tile_count(c, nseq, ntok, nhead);
   return tiles >= 128 || (tiles >= 32 && tiles * ((c.cap + PART - 1) / PART) >= 1024);

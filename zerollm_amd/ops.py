@@ -296,7 +296,7 @@ def logprobs_work_bytes(rows: int, vocab: int, top: int = 0) -> int:
 
 
 def logprobs(logits, tokens=None, top: int = 0, out=None, work=None) -> LogProbs:
-    """LogProbs of logits rows [rows, vocab] (any row stride). tokens: int32 [rows]; an id outside the vocabulary gives NaN.
+    """LogProbs of logits rows [rows, vocab] (any row stride of at least vocab). tokens: int32 [rows]; an id outside the vocabulary gives NaN.
     top: 0 to 64 alternatives. Logits of -inf have probability 0; a row with NaN or +inf, or with nothing above -inf, is NaN."""
     t = _type(logits, "logits")
     _no_gradient(logits, "logits")
